@@ -1,0 +1,250 @@
+"""A paged cache of K and V in 4 bits (C interface: include/mlops_paged.h): pages and slots for a step's new tokens (`assign`), quantise-on-write
+(`append`), read-back (`read`) and attention over the pages (`attend`).
+
+An engine keeps, on the GPU, one pool per layer (`empty`), one block table ``int32 [batch, width]`` for all layers, the requests' lengths, and a ring
+of free page numbers with its two ends. A step of one layer:
+
+    step = paged.assign(table, lengths, added, free, cursor, cache.page_size, tokens)      # once for all layers
+    paged.append(cache, k, v, step.slots)                                                  # k, v [tokens, kv_heads, 128]
+    out = paged.attend(q, cache, table, step.lengths, step.starts)                         # q, out [tokens, q_heads, 128]
+
+Elements take 4.5 bits: E2M1 codes, an E4M3 scale per 16 channels, an FP32 factor per head. The reference has no paged cache; tensors are BF16 or FP16.
+Nothing here synchronises, so that a step can be captured into a CUDA graph.
+"""
+import ctypes
+from dataclasses import dataclass
+from typing import NamedTuple, Optional, Tuple, Union
+
+import torch
+
+from . import _C
+
+HEAD_DIM = 128
+BLOCK, BLOCK_BYTES = 16, 2304  # tokens and bytes of a block of a page, per KV head
+_TYPES = {torch.bfloat16: 0, torch.float16: 1}
+_I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
+
+
+class _Cache(ctypes.Structure):
+    """mlops_paged_cache"""
+    _fields_ = [("units", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p), ("page_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64), ("pages", ctypes.c_int), ("page_size", ctypes.c_int), ("kv_heads", ctypes.c_int)]
+
+
+class _Assign(ctypes.Structure):
+    """mlops_paged_assign_args"""
+    _fields_ = [("batch", ctypes.c_int), ("tokens", ctypes.c_int), ("page_size", ctypes.c_int), ("width", ctypes.c_int), ("table_stride", ctypes.c_int64),
+                ("table", ctypes.c_void_p), ("held", ctypes.c_void_p), ("added", ctypes.c_void_p), ("ring", ctypes.c_void_p), ("ring_size", ctypes.c_int),
+                ("cursor", ctypes.c_void_p), ("slots", ctypes.c_void_p), ("positions", ctypes.c_void_p), ("starts", ctypes.c_void_p),
+                ("lengths", ctypes.c_void_p), ("moved", ctypes.c_void_p)]
+
+
+class _Attend(ctypes.Structure):
+    """mlops_paged_attend_args"""
+    _fields_ = [("batch", ctypes.c_int), ("tokens", ctypes.c_int), ("q_heads", ctypes.c_int), ("type", ctypes.c_int), ("q", ctypes.c_void_p),
+                ("q_token_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64), ("out", ctypes.c_void_p), ("out_token_stride", ctypes.c_int64),
+                ("out_head_stride", ctypes.c_int64), ("lse", ctypes.c_void_p), ("table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+                ("width", ctypes.c_int), ("lengths", ctypes.c_void_p), ("starts", ctypes.c_void_p), ("scale", ctypes.c_float)]
+
+
+_lib, _vp, _int, _i64 = _C._lib, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64
+_lib.mlops_paged_assign.argtypes = [_vp, _vp]
+_lib.mlops_paged_append.argtypes = [_vp, _int, _int, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp]
+_lib.mlops_paged_read.argtypes = [_vp, _int, _int, _vp, _vp, _vp, _vp]
+_lib.mlops_paged_attend.argtypes = [_vp, _vp, _vp, ctypes.c_size_t, _vp]
+_lib.mlops_paged_attend_scratch_bytes.argtypes = [_vp, _int]
+_lib.mlops_paged_attend_scratch_bytes.restype = ctypes.c_size_t
+_lib.mlops_paged_last_error.restype = ctypes.c_char_p
+
+
+def _raise(status, what):
+    message = _lib.mlops_paged_last_error().decode()
+    if status == _C.INVALID_VALUE:
+        raise ValueError(message)
+    raise RuntimeError(f"{what} failed: {message}")
+
+
+@dataclass
+class PagedCache:
+    """A pool of pages for one layer."""
+    units: torch.Tensor    # uint8 [pages, kv_heads, page_size / 16, 2304]; the last two dimensions dense
+    k_scale: torch.Tensor  # float32 [kv_heads]: the heads' factors, positive
+    v_scale: torch.Tensor
+
+    @property
+    def pages(self) -> int:
+        return self.units.size(0)
+
+    @property
+    def page_size(self) -> int:
+        return self.units.size(2) * BLOCK
+
+
+class Step(NamedTuple):
+    """What `assign` says of a step's new tokens. The tensors are for `append` (slots), a rotary embedding (positions) and `attend` (lengths, starts);
+    `lengths` and `cursor` are the next call's."""
+    slots: torch.Tensor      # int32 [tokens]: where each token is stored in the pool, -1: nowhere
+    positions: torch.Tensor  # int32 [tokens]: its position in its request
+    starts: torch.Tensor     # int32 [batch + 1]: request b's tokens are starts[b] .. starts[b + 1] - 1
+    lengths: torch.Tensor    # int32 [batch]: tokens of each request, the new ones among them
+    cursor: torch.Tensor     # int64 [3]: the ring's head and tail after the call, and how many pages were missing
+
+
+def empty(pages: int, kv_heads: int, page_size: int = 64, *, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
+          device="cuda") -> PagedCache:
+    """A pool of ``pages`` pages of ``page_size`` tokens (a multiple of 16). ``k_scale``, ``v_scale``: float32 [kv_heads] factors that bring the heads'
+    values into the scales' range (a block of 16 channels is stored well where its largest value is between 0.1 and 2688 times the factor); default 1."""
+    if pages <= 0 or kv_heads <= 0 or page_size <= 0 or page_size % BLOCK:
+        raise ValueError(f"expected pages, kv_heads > 0 and a page_size that is a multiple of {BLOCK}; got {pages}, {kv_heads}, {page_size}")
+    if pages * page_size >= 1 << 31:
+        raise ValueError(f"a pool has fewer than 2^31 slots; {pages} pages of {page_size} tokens are more")
+    one = torch.ones((kv_heads,), dtype=_F32, device=device)
+    scales = [one.clone() if s is None else s.to(device=device, dtype=_F32).contiguous() for s in (k_scale, v_scale)]
+    return PagedCache(torch.zeros((pages, kv_heads, page_size // BLOCK, BLOCK_BYTES), dtype=torch.uint8, device=device), *scales)
+
+
+def _pool(c):
+    """A pool's arrays, checked: the structure that names them to the library, their device's index."""
+    u, ks, vs = c.units, c.k_scale, c.v_scale
+    index = u.get_device()
+    if not 0 <= index == ks.get_device() == vs.get_device():
+        raise ValueError(f"the arrays of a paged cache have to live on the same CUDA device (units: {u.device}, scales: {ks.device}, {vs.device})")
+    if u.dim() != 4 or u.dtype is not torch.uint8 or u.size(3) != BLOCK_BYTES or u.stride(3) != 1 or (u.size(2) > 1 and u.stride(2) != BLOCK_BYTES):
+        raise ValueError(f"units has to be a uint8 [pages, kv_heads, blocks, {BLOCK_BYTES}] tensor with dense pages; it is {u.dtype} {tuple(u.shape)}, strides {u.stride()}")
+    pages, heads, blocks, _ = u.shape
+    for s in (ks, vs):
+        if s.dtype is not _F32 or s.dim() != 1 or s.size(0) != heads or not s.is_contiguous():
+            raise ValueError(f"k_scale and v_scale have to be contiguous float32 [{heads}] tensors; one is {s.dtype} {tuple(s.shape)}")
+    return _Cache(u.data_ptr(), ks.data_ptr(), vs.data_ptr(), u.stride(0), u.stride(1), pages, blocks * BLOCK, heads), index
+
+
+def _ints(x, index, what, size, dtype=_I32):
+    if x.get_device() != index or x.dtype is not dtype or x.dim() != 1 or not x.is_contiguous() or (size is not None and x.size(0) != size):
+        raise ValueError(f"{what}: expected a contiguous {dtype} [{'n' if size is None else size}] tensor on cuda:{index}; it is {x.dtype} {tuple(x.shape)} on {x.device}")
+    return x.data_ptr()
+
+
+def _table(x, index):
+    if x.get_device() != index or x.dtype is not _I32 or x.dim() != 2 or (x.size(1) > 1 and x.stride(1) != 1):
+        raise ValueError(f"table: expected an int32 [batch, width] tensor with dense rows on cuda:{index}; it is {x.dtype} {tuple(x.shape)} on {x.device}")
+    batch, width = x.shape
+    return x.data_ptr(), (x.stride(0) if batch > 1 else width), batch, width
+
+
+def _rows(x, index, what, heads=None):
+    """[tokens, heads, 128] rows as the library reads them (dense channels, 16-byte pieces aligned), its type"""
+    kind = _TYPES.get(x.dtype)
+    if x.get_device() != index or kind is None or x.dim() != 3 or x.size(2) != HEAD_DIM or (heads is not None and x.size(1) != heads):
+        raise ValueError(f"{what}: expected a bfloat16 or float16 [tokens, {'heads' if heads is None else heads}, {HEAD_DIM}] tensor on cuda:{index}; it is {x.dtype} {tuple(x.shape)} on {x.device}")
+    if x.stride(2) != 1 or x.stride(0) % 8 or x.stride(1) % 8 or x.data_ptr() % 16:
+        x = x.contiguous()
+        if x.data_ptr() % 16:
+            x = x.clone()
+    return x, kind
+
+
+def _on(index):
+    """Whether ``index`` is the current device (calls are made on their tensors' device)."""
+    return torch._C._cuda_getDevice() == index
+
+
+def assign(table: torch.Tensor, held: torch.Tensor, added: torch.Tensor, free: torch.Tensor, cursor: torch.Tensor, page_size: int, tokens: int) -> Step:
+    """Pages and slots for ``added[b]`` new tokens of every request b, which holds ``held[b]``.
+
+    New pages are taken from the ring ``free`` (int32, from ``cursor[0]`` up to ``cursor[1]``, both counted without end and taken modulo the ring's
+    size), in the order of the requests, and entered into ``table`` (int32 [batch, width], in place). ``tokens``: rows of the step, at least the sum of
+    ``added``; rows behind it get slot and position -1. Where the ring runs out or a request outgrows its row, entries and slots are -1 and
+    ``Step.cursor[2]`` counts the pages that were missing. A request's pages are given back by ``free[tail % size ...] = table[b, :n]`` and advancing
+    the tail, ``cursor[1]``."""
+    index = table.get_device()
+    if index < 0:
+        raise ValueError(f"table: expected a CUDA tensor, not one on {table.device}")
+    if not _on(index):
+        with torch.cuda.device(index):
+            return assign(table, held, added, free, cursor, page_size, tokens)
+    entries, stride, batch, width = _table(table, index)
+    tokens = int(tokens)
+    if tokens < 0:
+        raise ValueError(f"tokens may not be negative; it is {tokens}")
+    if cursor.dim() != 1 or cursor.size(0) not in (2, 3):
+        raise ValueError(f"cursor: expected int64 [2] (head, tail) or a Step's; it has shape {tuple(cursor.shape)}")
+    args = (_ints(held, index, "held", batch), _ints(added, index, "added", batch), _ints(free, index, "free", None), free.size(0),
+            _ints(cursor, index, "cursor", None, _I64))
+    slots, positions, starts, lengths = torch.empty((2 * tokens + 2 * batch + 1,), dtype=_I32, device=table.device).split([tokens, tokens, batch + 1, batch])
+    moved = torch.empty((3,), dtype=_I64, device=table.device)
+    call = _Assign(batch, tokens, page_size, width, stride, entries, *args, slots.data_ptr(), positions.data_ptr(), starts.data_ptr(), lengths.data_ptr(), moved.data_ptr())
+    status = _lib.mlops_paged_assign(ctypes.byref(call), _C._raw_stream(index))
+    if status:
+        _raise(status, "mlops_paged_assign")
+    return Step(slots, positions, starts, lengths, moved)
+
+
+@torch.no_grad()
+def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> PagedCache:
+    """Quantise ``k, v [tokens, kv_heads, 128]`` (BF16 or FP16, slices of a fused projection as they are) into the pool's ``slots`` (int32 [tokens]; a
+    slot outside the pool, -1 for instance: the token is left out). In place; the cache is also returned."""
+    pool, index = _pool(cache)
+    if not _on(index):
+        with torch.cuda.device(index):
+            return append(cache, k, v, slots)
+    k, kind = _rows(k, index, "k", pool.kv_heads)
+    v, v_kind = _rows(v, index, "v", pool.kv_heads)
+    tokens = k.size(0)
+    if v.size(0) != tokens or v_kind != kind:
+        raise ValueError(f"k and v have to be alike; k is {k.dtype} {tuple(k.shape)}, v is {v.dtype} {tuple(v.shape)}")
+    status = _lib.mlops_paged_append(ctypes.byref(pool), tokens, kind, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+                                     _ints(slots, index, "slots", tokens), _C._raw_stream(index))
+    if status:
+        _raise(status, "mlops_paged_append")
+    return cache
+
+
+def read(cache: PagedCache, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
+    """What the pool holds in ``slots`` (int32 [tokens]): K and V as ``[tokens, kv_heads, 128]``, rounded once to ``dtype`` (BF16 or FP16). Zeros for a
+    slot outside the pool."""
+    pool, index = _pool(cache)
+    kind = _TYPES.get(dtype)
+    if kind is None:
+        raise ValueError(f"dtype has to be bfloat16 or float16, not {dtype}")
+    if not _on(index):
+        with torch.cuda.device(index):
+            return read(cache, slots, dtype)
+    where = _ints(slots, index, "slots", None)
+    k = torch.empty((slots.size(0), pool.kv_heads, HEAD_DIM), dtype=dtype, device=cache.units.device)
+    v = torch.empty_like(k)
+    status = _lib.mlops_paged_read(ctypes.byref(pool), slots.size(0), kind, where, k.data_ptr(), v.data_ptr(), _C._raw_stream(index))
+    if status:
+        _raise(status, "mlops_paged_read")
+    return k, v
+
+
+@torch.no_grad()
+def attend(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor] = None, *, scale: float = 0.0,
+           return_lse: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """Causal attention of the requests' newest tokens over their pages.
+
+    ``q [tokens, q_heads, 128]`` BF16 or FP16, ``table`` int32 [batch, width], ``lengths`` int32 [batch]: tokens that each request has in the pool, the
+    queries' own among them. ``starts`` int32 [batch + 1]: the rows of request b are ``starts[b] .. starts[b + 1] - 1``, its newest tokens; None: one
+    query per request. Row i of n sees the request's tokens up to ``lengths[b] - n + i``. Returns ``[tokens, q_heads, 128]`` of q's type, zeros for a
+    row that sees nothing and for rows of no request; with ``return_lse`` also the natural log-sum-exp of the rows' scaled scores, float32
+    [tokens, q_heads] (-inf for such rows). ``scale`` 0 selects 1/sqrt(128)."""
+    pool, index = _pool(cache)
+    if not _on(index):
+        with torch.cuda.device(index):
+            return attend(q, cache, table, lengths, starts, scale=scale, return_lse=return_lse)
+    q, kind = _rows(q, index, "q")
+    entries, stride, batch, width = _table(table, index)
+    tokens, heads = q.size(0), q.size(1)
+    where = _ints(lengths, index, "lengths", batch)
+    begins = None if starts is None else _ints(starts, index, "starts", batch + 1)
+    out = torch.empty((tokens, heads, HEAD_DIM), dtype=q.dtype, device=q.device)
+    lse = torch.empty((tokens, heads), dtype=_F32, device=q.device) if return_lse else None
+    call = _Attend(batch, tokens, heads, kind, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), heads * HEAD_DIM, HEAD_DIM,
+                   lse.data_ptr() if return_lse else None, entries, stride, width, where, begins, scale)
+    stream = _C._raw_stream(index)
+    scratch = _C._pool.get(q.device, stream, max(16, _lib.mlops_paged_attend_scratch_bytes(ctypes.byref(call), pool.kv_heads)))
+    with scratch.lock:
+        status = _lib.mlops_paged_attend(ctypes.byref(call), ctypes.byref(pool), scratch.pointer, scratch.bytes, stream)
+    if status:
+        _raise(status, "mlops_paged_attend")
+    return (out, lse) if return_lse else out

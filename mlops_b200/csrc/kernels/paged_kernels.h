@@ -1,0 +1,20 @@
+// The thin C ABI between the host layer of the paged cache (validation) and its CUDA kernels: one launcher per operator, arguments as in
+// include/mlops_paged.h. The host layer checks; nothing here validates.
+#pragma once
+#include "../../../include/mlops_paged.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define PAGED_K_MAX_BATCH 16384  /* requests of one call: their prefix sums live in shared memory */
+
+cudaError_t paged_k_assign_launch(const mlops_paged_assign_args *a, cudaStream_t stream);
+cudaError_t paged_k_append_launch(const mlops_paged_cache *c, int tokens, int type, const void *k, int64_t k_ts, int64_t k_hs, const void *v, int64_t v_ts,
+                                  int64_t v_hs, const int *slots, cudaStream_t stream);
+cudaError_t paged_k_read_launch(const mlops_paged_cache *c, int tokens, int type, const int *slots, void *k, void *v, cudaStream_t stream);
+cudaError_t paged_k_attend_launch(const mlops_paged_attend_args *a, const mlops_paged_cache *c, void *scratch, cudaStream_t stream);
+
+#ifdef __cplusplus
+}
+#endif
