@@ -77,7 +77,7 @@ mlops_fbla_status mlops_paged_append(const mlops_paged_cache *cache, int tokens,
 mlops_fbla_status mlops_paged_read(const mlops_paged_cache *cache, int tokens, int type, const int *slots, void *k, void *v, cudaStream_t stream);
 
 typedef struct mlops_paged_attend_args {
-  int batch, tokens, q_heads, type;    /* tokens: rows of q; kv_heads divides q_heads */
+  int batch, tokens, q_heads, type;    /* tokens: rows of q; kv_heads divides q_heads; batch at most 4096 */
   const void *q;                       /* [tokens][q_heads][128], strides in elements: multiples of 8 */
   int64_t q_token_stride, q_head_stride;
   void *out;                           /* likewise */
@@ -92,7 +92,8 @@ typedef struct mlops_paged_attend_args {
 } mlops_paged_attend_args;
 /* Bytes of scratch a call of this shape needs (0: the arguments are refused). Pointers and strides of args are not looked at. */
 size_t mlops_paged_attend_scratch_bytes(const mlops_paged_attend_args *args, int kv_heads);
-/* Rows of q behind starts[batch] have zeros as their output. The scratch (16-byte aligned) needs no initial contents. */
+/* Rows of q behind starts[batch] have zeros as their output. The scratch (16-byte aligned) is filled with zeros once, before its first call; what a
+ * call leaves in it serves the next one, of whatever shape. Calls that overlap need scratches of their own. */
 mlops_fbla_status mlops_paged_attend(const mlops_paged_attend_args *args, const mlops_paged_cache *cache, void *scratch, size_t scratch_bytes, cudaStream_t stream);
 
 const char *mlops_paged_last_error(void);

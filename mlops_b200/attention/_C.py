@@ -149,9 +149,9 @@ class _Scratch:
     """a decode's scratch; `lock` is held while a call's kernels are enqueued, so that threads on one stream do not mix theirs"""
     __slots__ = ("bytes", "buffer", "pointer", "lock")
 
-    def __init__(self, nbytes, device):
+    def __init__(self, nbytes, device, make=torch.empty):
         self.bytes, self.lock = nbytes, threading.Lock()
-        self.buffer = torch.empty((nbytes,), dtype=torch.uint8, device=device)  # the library needs no initial contents
+        self.buffer = make((nbytes,), dtype=torch.uint8, device=device)
         self.pointer = self.buffer.data_ptr()
 
 
@@ -162,19 +162,19 @@ class _ScratchPool:
     has one of its own, from the graph's memory: a replay may run on any stream and at any later time."""
     BUFFERS = 16
 
-    def __init__(self):
-        self._held, self._lock = collections.OrderedDict(), threading.Lock()
+    def __init__(self, make=torch.empty):  # (the decode needs no initial contents)
+        self._held, self._lock, self._make = collections.OrderedDict(), threading.Lock(), make
 
     def get(self, device, stream, nbytes):
         if device.type == "cuda" and _capturing():
-            return _Scratch(nbytes, device)
+            return _Scratch(nbytes, device, self._make)
         key = device, stream
         with self._lock:
             held = self._held.get(key)
             if held is not None and held.bytes >= nbytes:
                 self._held.move_to_end(key)
                 return held
-            self._held[key] = held = _Scratch(nbytes, device)
+            self._held[key] = held = _Scratch(nbytes, device, self._make)
             self._held.move_to_end(key)
             while len(self._held) > self.BUFFERS:
                 self._held.popitem(last=False)

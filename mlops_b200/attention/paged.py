@@ -57,6 +57,9 @@ _lib.mlops_paged_attend_scratch_bytes.restype = ctypes.c_size_t
 _lib.mlops_paged_last_error.restype = ctypes.c_char_p
 
 
+_scratch = _C._ScratchPool(torch.zeros)  # (zeros at first; every call leaves its counters as it found them)
+
+
 def _raise(status, what):
     message = _lib.mlops_paged_last_error().decode()
     if status == _C.INVALID_VALUE:
@@ -242,7 +245,7 @@ def attend(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, lengths: tor
     call = _Attend(batch, tokens, heads, kind, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), heads * HEAD_DIM, HEAD_DIM,
                    lse.data_ptr() if return_lse else None, entries, stride, width, where, begins, scale)
     stream = _C._raw_stream(index)
-    scratch = _C._pool.get(q.device, stream, max(16, _lib.mlops_paged_attend_scratch_bytes(ctypes.byref(call), pool.kv_heads)))
+    scratch = _scratch.get(q.device, stream, max(16, _lib.mlops_paged_attend_scratch_bytes(ctypes.byref(call), pool.kv_heads)))
     with scratch.lock:
         status = _lib.mlops_paged_attend(ctypes.byref(call), ctypes.byref(pool), scratch.pointer, scratch.bytes, stream)
     if status:

@@ -50,8 +50,23 @@ const char *cache_fault(const mlops_paged_cache *c) {
 bool rows_usable(const void *p, int64_t token_stride, int64_t head_stride) { return aligned(p, 16) && token_stride % 8 == 0 && head_stride % 8 == 0; }
 
 bool attend_shape_acceptable(const mlops_paged_attend_args *a, int kv_heads) {
-  return a && a->batch >= 0 && a->tokens >= 0 && a->batch <= PAGED_K_MAX_BATCH && a->q_heads > 0 && kv_heads > 0 && a->q_heads % kv_heads == 0 &&
+  return a && a->batch >= 0 && a->tokens >= 0 && a->batch <= PAGED_K_MAX_ATTENDED && a->q_heads > 0 && kv_heads > 0 && a->q_heads % kv_heads == 0 &&
          (int64_t)a->tokens * a->q_heads <= INT32_MAX;
+}
+
+// the current device's multiprocessors
+cudaError_t processors(int *sms) {
+  static thread_local int known[64] = {0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 64 && known[dev]) {
+    *sms = known[dev];
+    return cudaSuccess;
+  }
+  e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e == cudaSuccess && dev < 64) known[dev] = *sms;
+  return e;
 }
 
 }  // namespace
@@ -61,8 +76,8 @@ extern "C" {
 mlops_fbla_status mlops_paged_assign(const mlops_paged_assign_args *a, cudaStream_t stream) {
   const char *const fn = "mlops_paged_assign";
   if (!a || !a->starts || !a->moved || !a->cursor) return refuse(fn, "a required pointer is null");
-  if (a->batch < 0 || a->batch > PAGED_K_MAX_BATCH || a->tokens < 0 || a->width < 0 || a->ring_size < 0)
-    return refuse(fn, "needs batch in 0..%d and tokens, width, ring_size >= 0", PAGED_K_MAX_BATCH);
+  if (a->batch < 0 || a->batch > PAGED_K_MAX_ASSIGNED || a->tokens < 0 || a->width < 0 || a->ring_size < 0)
+    return refuse(fn, "needs batch in 0..%d and tokens, width, ring_size >= 0", PAGED_K_MAX_ASSIGNED);
   if (!known_page_size(a->page_size)) return refuse(fn, "page_size %d is no multiple of 16", a->page_size);
   if (a->batch > 0 && (!a->held || !a->added || !a->lengths || (a->width > 0 && !a->table) || a->table_stride < a->width))
     return refuse(fn, "needs held, added, lengths and a table whose stride is at least its width");
@@ -98,14 +113,15 @@ mlops_fbla_status mlops_paged_read(const mlops_paged_cache *c, int tokens, int t
 }
 
 size_t mlops_paged_attend_scratch_bytes(const mlops_paged_attend_args *a, int kv_heads) {
-  return attend_shape_acceptable(a, kv_heads) ? 16 : 0;
+  int sms = 0;
+  return attend_shape_acceptable(a, kv_heads) && processors(&sms) == cudaSuccess ? paged_k_attend_scratch(sms) : 0;
 }
 
 mlops_fbla_status mlops_paged_attend(const mlops_paged_attend_args *a, const mlops_paged_cache *c, void *scratch, size_t scratch_bytes, cudaStream_t stream) {
   const char *const fn = "mlops_paged_attend";
   if (const char *why = cache_fault(c)) return refuse(fn, "%s", why);
   if (!attend_shape_acceptable(a, c->kv_heads))
-    return refuse(fn, "needs batch in 0..%d, tokens >= 0, q_heads that kv_heads divides and fewer than 2^31 rows", PAGED_K_MAX_BATCH);
+    return refuse(fn, "needs batch in 0..%d, tokens >= 0, q_heads that kv_heads divides and fewer than 2^31 rows", PAGED_K_MAX_ATTENDED);
   if (!known_type(a->type)) return refuse(fn, "type %d is neither MLOPS_PAGED_BF16 nor MLOPS_PAGED_FP16", a->type);
   if (!(a->scale >= 0.f) || std::isinf(a->scale)) return refuse(fn, "scale has to be a number that is not negative");
   if (!a->starts && a->tokens != a->batch) return refuse(fn, "without starts there is one query per request, but there are %d for %d", a->tokens, a->batch);
@@ -115,11 +131,13 @@ mlops_fbla_status mlops_paged_attend(const mlops_paged_attend_args *a, const mlo
   if (!rows_usable(a->q, a->q_token_stride, a->q_head_stride) || !rows_usable(a->out, a->out_token_stride, a->out_head_stride) || !aligned(scratch, 16))
     return refuse(fn, "q, out and scratch have to start on 16-byte boundaries, q and out with strides that are multiples of 8 elements");
   if (!aligned(a->lengths, 4) || !aligned(a->starts, 4) || !aligned(a->table, 4) || !aligned(a->lse, 4)) return refuse(fn, "arrays of int and float have to start on 4-byte boundaries");
-  if (scratch_bytes < mlops_paged_attend_scratch_bytes(a, c->kv_heads))
-    return refuse(fn, "the scratch is %zu bytes but this call takes %zu", scratch_bytes, mlops_paged_attend_scratch_bytes(a, c->kv_heads));
+  int sms = 0;
+  const cudaError_t e = scratch_bytes < 16 ? cudaSuccess : processors(&sms);
+  if (e != cudaSuccess) return ended(fn, e);
+  if (scratch_bytes < 16 || scratch_bytes < paged_k_attend_scratch(sms)) return refuse(fn, "the scratch is %zu bytes, which are too few for this call", scratch_bytes);
   mlops_paged_attend_args call = *a;
   if (call.scale == 0.f) call.scale = 1.f / std::sqrt((float)MLOPS_PAGED_HEAD_DIM);
-  return ended(fn, paged_k_attend_launch(&call, c, scratch, stream));
+  return ended(fn, paged_k_attend_launch(&call, c, scratch, sms, stream));
 }
 
 const char *mlops_paged_last_error(void) { return g_message; }

@@ -123,7 +123,7 @@ extern "C" cudaError_t paged_k_assign_launch(const mlops_paged_assign_args *a, c
   int dev = 0;
   cudaGetDevice(&dev);
   if (smem > 48 * 1024 && !(dev < 64 && asked[dev])) {
-    const cudaError_t e = cudaFuncSetAttribute(paged::assign_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * (PAGED_K_MAX_BATCH + 1) * (int)sizeof(int));
+    const cudaError_t e = cudaFuncSetAttribute(paged::assign_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * (PAGED_K_MAX_ASSIGNED + 1) * (int)sizeof(int));
     if (e != cudaSuccess) return e;
     if (dev < 64) asked[dev] = true;
   }
