@@ -90,7 +90,7 @@ typedef struct mlops_paged_attend_args {
   const int *starts;                   /* [batch + 1], or null: one query per request, tokens = batch */
   float scale;                         /* 0: 1 / sqrt(128) */
 } mlops_paged_attend_args;
-/* Bytes of scratch a call of this shape needs (0: the arguments are refused). Pointers and strides of args are not looked at. */
+/* Bytes of scratch a call of this shape needs (0: the arguments are refused). Of the pointers only starts is looked at: null or not. */
 size_t mlops_paged_attend_scratch_bytes(const mlops_paged_attend_args *args, int kv_heads);
 /* Rows of q behind starts[batch] have zeros as their output. The scratch (16-byte aligned) is filled with zeros once, before its first call; what a
  * call leaves in it serves the next one, of whatever shape. Calls that overlap need scratches of their own. */

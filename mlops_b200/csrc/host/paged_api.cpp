@@ -114,7 +114,7 @@ mlops_fbla_status mlops_paged_read(const mlops_paged_cache *c, int tokens, int t
 
 size_t mlops_paged_attend_scratch_bytes(const mlops_paged_attend_args *a, int kv_heads) {
   int sms = 0;
-  return attend_shape_acceptable(a, kv_heads) && processors(&sms) == cudaSuccess ? paged_k_attend_scratch(sms) : 0;
+  return attend_shape_acceptable(a, kv_heads) && processors(&sms) == cudaSuccess ? paged_k_attend_scratch(a, kv_heads, sms) : 0;
 }
 
 mlops_fbla_status mlops_paged_attend(const mlops_paged_attend_args *a, const mlops_paged_cache *c, void *scratch, size_t scratch_bytes, cudaStream_t stream) {
@@ -134,7 +134,7 @@ mlops_fbla_status mlops_paged_attend(const mlops_paged_attend_args *a, const mlo
   int sms = 0;
   const cudaError_t e = scratch_bytes < 16 ? cudaSuccess : processors(&sms);
   if (e != cudaSuccess) return ended(fn, e);
-  if (scratch_bytes < 16 || scratch_bytes < paged_k_attend_scratch(sms)) return refuse(fn, "the scratch is %zu bytes, which are too few for this call", scratch_bytes);
+  if (scratch_bytes < 16 || scratch_bytes < paged_k_attend_scratch(a, c->kv_heads, sms)) return refuse(fn, "the scratch is %zu bytes, which are too few for this call", scratch_bytes);
   mlops_paged_attend_args call = *a;
   if (call.scale == 0.f) call.scale = 1.f / std::sqrt((float)MLOPS_PAGED_HEAD_DIM);
   return ended(fn, paged_k_attend_launch(&call, c, scratch, sms, stream));

@@ -1,0 +1,49 @@
+// Dispatch of the paged cache's attention: requests with few columns (queries times query heads per KV head) are streamed, the others go to the tile kernel.
+#include "paged_attend.cuh"
+
+namespace paged {
+namespace {
+
+constexpr int WIDE = 16;  // columns that a row of the stream kernel has at most
+
+struct Scratch {  // offsets: the counters of both kernels (zeros at first), their partial rows
+  size_t stream_counters, tile_counters, stream_part, tile_part, bytes;
+};
+Scratch scratch_of(int sms, bool tiles) {
+  Scratch s{};
+  const size_t counters = ((size_t)sms * sizeof(int) + 255) / 256 * 256;
+  s.tile_counters = counters;
+  s.stream_part = 2 * counters;
+  s.tile_part = s.stream_part + (size_t)sms * 2 * WIDE * PSTRIDE * sizeof(float);
+  s.bytes = s.tile_part + (tiles ? (size_t)sms * 2 * 256 * PSTRIDE * sizeof(float) : 0);
+  return s;
+}
+// whether some request may have more than WIDE columns
+bool may_be_wide(const mlops_paged_attend_args *a, int kv_heads) { return a->starts || a->q_heads / kv_heads > WIDE; }
+
+template <int TYPE> cudaError_t attend(const Call &k, bool tiles, int sms, cudaStream_t stream) {
+  const cudaError_t e = k.a.starts || k.group > 8 ? launch_stream<TYPE, 2>(k, sms, stream) : launch_stream<TYPE, 1>(k, sms, stream);
+  return e != cudaSuccess || !tiles ? e : launch_tile<TYPE>(k, sms, stream);
+}
+
+}  // namespace
+}  // namespace paged
+
+extern "C" size_t paged_k_attend_scratch(const mlops_paged_attend_args *a, int kv_heads, int sms) { return paged::scratch_of(sms, paged::may_be_wide(a, kv_heads)).bytes; }
+
+extern "C" cudaError_t paged_k_attend_launch(const mlops_paged_attend_args *a, const mlops_paged_cache *c, void *scratch, int sms, cudaStream_t stream) {
+  const bool tiles = paged::may_be_wide(a, c->kv_heads);
+  const paged::Scratch s = paged::scratch_of(sms, tiles);
+  char *const base = static_cast<char *>(scratch);
+  paged::Call k{};
+  k.a = *a;
+  k.c = *c;
+  k.sl = a->scale * 1.4426950408889634f;
+  k.group = a->q_heads / c->kv_heads;
+  k.wide = paged::WIDE;
+  k.stream_counters = reinterpret_cast<int *>(base + s.stream_counters);
+  k.tile_counters = reinterpret_cast<int *>(base + s.tile_counters);
+  k.stream_part = reinterpret_cast<float *>(base + s.stream_part);
+  k.tile_part = reinterpret_cast<float *>(base + s.tile_part);
+  return a->type == MLOPS_PAGED_BF16 ? paged::attend<MLOPS_PAGED_BF16>(k, tiles, sms, stream) : paged::attend<MLOPS_PAGED_FP16>(k, tiles, sms, stream);
+}

@@ -15,8 +15,9 @@ struct Call {
   mlops_paged_cache c;
   float sl;        // softmax scale times log2(e)
   int group;       // queries heads per KV head
-  float *part;     // partial rows, see the kernels
-  int *counters;   // zeros before and after every call
+  int wide;        // requests with more than so many columns (queries times group) are the tile kernel's
+  float *stream_part, *tile_part;          // partial rows, see the kernels
+  int *stream_counters, *tile_counters;    // one per CTA, zeros before and after every call
 };
 
 // request b's queries and tokens, as far as q's rows and the table's width go
@@ -54,5 +55,48 @@ __device__ __forceinline__ void clear_row(const Call &k, int row, int lane) {
   if (k.a.lse)
     for (int i = lane; i < k.a.q_heads; i += 32) k.a.lse[(size_t)row * k.a.q_heads + i] = -FBLA_INF;
 }
+
+// joins `count` partial rows, source(i) the i-th: channels 4 x .. 4 x + 3, the running maximum and sum
+template <class F> __device__ __forceinline__ float4 join(int count, F source, int x, float &m, float &l) {
+  m = NOTHING;
+  for (int i = 0; i < count; ++i) m = fmaxf(m, source(i)[D]);
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  l = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < count; ++i) {
+    const float *const p = source(i);
+    const float f = ex2(p[D] - m);
+    const float4 v = *reinterpret_cast<const float4 *>(p + 4 * x);
+    l += p[D + 1] * f;
+    o = make_float4(o.x + v.x * f, o.y + v.y * f, o.z + v.z * f, o.w + v.w * f);
+  }
+  return o;
+}
+template <int TYPE> __device__ __forceinline__ void store_joined(const Call &k, int row, int kv_head, int head, int x, const float4 &o, float m, float l) {
+  const float f = l == 0.f ? 0.f : __ldg(k.c.v_scale + kv_head) / l;
+  *reinterpret_cast<uint2 *>(out_row(k, row, head) + 4 * x) = make_uint2(from_floats<TYPE>(o.x * f, o.y * f), from_floats<TYPE>(o.z * f, o.w * f));
+  if (k.a.lse && x == 0) k.a.lse[(size_t)row * k.a.q_heads + head] = lse_of(m, l);
+}
+
+// the power of two that puts a query's largest element (its bits: `top`) into [2^8, 2^9), and its inverse; 1 where that is infinite or NaN. As FP16
+// elements down to 2^-22 of the largest are exact, the others are rounded to 2^-33 of it.
+__device__ __forceinline__ float q_factor(uint32_t top, float &inverse) {
+  const uint32_t e = top >> 23, field = e == 255 ? 127 : min(262 - e, 253u);
+  inverse = __uint_as_float((254 - field) << 23);
+  return __uint_as_float(field << 23);
+}
+
+// a kernel's shared memory is above the default limit: asked for once per device and host thread
+template <class K> cudaError_t allow_shared(K *kernel, bool (&ready)[64]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && ready[dev])) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
+  if (e == cudaSuccess && dev < 64) ready[dev] = true;
+  return e;
+}
+// 8 NT: columns of a row of work
+template <int TYPE, int NT> cudaError_t launch_stream(const Call &k, int sms, cudaStream_t stream);
+template <int TYPE> cudaError_t launch_tile(const Call &k, int sms, cudaStream_t stream);
 
 }  // namespace paged

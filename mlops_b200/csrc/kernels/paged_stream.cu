@@ -5,8 +5,7 @@
 // ragged lengths cost nothing; a warp brings its run's blocks through a ring of its own in shared memory with bulk copies.
 //
 // Per block, tokens on the M axis: S^T[16 tokens x 8] = K Q^T and O^T[128 channels x 8] += V^T P^T with mma.sync m16n8k16, FP16 operands, FP32 sums.
-// K and V: code * scale is exact in FP16. Q: each column times a power of two that puts its largest element into [2^8, 2^9) -- exact for elements down
-// to 2^-22 of that, the others are rounded to 2^-33 of it. P: 2^(s - m') with m' between 9 and 15 below the column's largest score so far, rounded to
+// K and V: code * scale is exact in FP16. Q: FP16 after a power of two per column (q_factor). P: 2^(s - m') with m' between 9 and 15 below the column's largest score so far, rounded to
 // FP16 (relative 2^-11, the only rounding of the operands); m' moves, and O and l are rescaled, only where a score would pass 2^15. l sums the
 // unrounded P. Weights below 2^-33 of the largest are lost, 2^17 of them are 2^-16 of the sum.
 //
@@ -22,7 +21,9 @@
 namespace paged {
 namespace {
 
-constexpr int WARPS = 16, STAGES = 3, THREADS = 32 * WARPS;
+template <int NT> constexpr int WARPS = NT == 1 ? 16 : 10;   // what the shared memory has room for beside the rings
+template <int NT> constexpr int STAGES = NT == 1 ? 3 : 4;
+template <int NT> constexpr int THREADS = 32 * WARPS<NT>;
 constexpr int MIN_SHARE = 4;  // units of a warp, at least, where the work allows a choice
 constexpr float TOP = 15.f, REST = 9.f;  // log2 of the largest P, and of a column's largest when m' is set
 
@@ -30,15 +31,15 @@ template <int NT> struct Piece {  // a warp's partial rows of one row of work
   float o[8 * NT][PSTRIDE];        // (o[128], m', l)
 };
 template <int NT> struct __align__(128) Smem {
-  uint8_t ring[WARPS][STAGES][BLOCK_BYTES];
-  Piece<NT> first[WARPS];          // of a run's first row; the last row's piece takes the ring's place when that is through
-  uint64_t full[WARPS][STAGES];
-  long long tag[2 * WARPS];        // pieces in the order of the tokens: the first unit of the piece's row, -1: none
-  long long warp_sum[WARPS];
+  uint8_t ring[WARPS<NT>][STAGES<NT>][BLOCK_BYTES];
+  Piece<NT> first[WARPS<NT>];          // of a run's first row; the last row's piece takes the ring's place when that is through
+  uint64_t full[WARPS<NT>][STAGES<NT>];
+  long long tag[2 * WARPS<NT>];        // pieces in the order of the tokens: the first unit of the piece's row, -1: none
+  long long warp_sum[WARPS<NT>];
   int last;
   long long before[];              // [batch + 1]: the requests' first units
 };
-template <int NT> constexpr bool fits = sizeof(Piece<NT>) <= STAGES * BLOCK_BYTES;
+template <int NT> constexpr bool fits = sizeof(Piece<NT>) <= STAGES<NT> * BLOCK_BYTES;
 
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -75,7 +76,7 @@ template <int NT> struct Row {
 template <int NT> __device__ __forceinline__ int blocks_of(const Request &r) { return (r.tokens + BT - 1) / BT; }
 template <int NT> __device__ __forceinline__ int tiles_of(const Call &k, const Request &r) { return (r.n * k.group + 8 * NT - 1) / (8 * NT); }
 template <int NT> __device__ __forceinline__ long long units_of(const Call &k, const Request &r) {
-  return (long long)k.c.kv_heads * tiles_of<NT>(k, r) * blocks_of<NT>(r);
+  return r.n * k.group > k.wide ? 0 : (long long)k.c.kv_heads * tiles_of<NT>(k, r) * blocks_of<NT>(r);
 }
 
 // the row that unit u (of request b) belongs to
@@ -125,8 +126,8 @@ template <int TYPE, int NT> struct Columns {  // a row's queries, as B fragments
       }
       top = max(top, __shfl_xor_sync(FULL, top, 1));
       top = max(top, __shfl_xor_sync(FULL, top, 2));
-      const uint32_t e = top >> 23, field = e == 255 ? 127 : min(262 - e, 253u);  // (a column with infinities or NaN as it is)
-      const float up = __uint_as_float(field << 23), down = __uint_as_float((254 - field) << 23);
+      float down;
+      const float up = q_factor(top, down);
 #pragma unroll
       for (int i = 0; i < 16; ++i) q[j][i] = from_floats<MLOPS_PAGED_FP16>(x[i].x * up, x[i].y * up);
 #pragma unroll
@@ -297,42 +298,19 @@ template <int NT> __device__ __forceinline__ void store_piece(Piece<NT> &p, Sums
     }
 }
 
-// joins `count` partial rows, source(i) the i-th, for column c and channels 4 x .. 4 x + 3
-template <class F> __device__ __forceinline__ float4 join(int count, F source, int x, float &m, float &l) {
-  m = NOTHING;
-  for (int i = 0; i < count; ++i) m = fmaxf(m, source(i)[D]);
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  l = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < count; ++i) {
-    const float *const p = source(i);
-    const float f = ex2(p[D] - m);
-    const float4 v = *reinterpret_cast<const float4 *>(p + 4 * x);
-    l += p[D + 1] * f;
-    o = make_float4(o.x + v.x * f, o.y + v.y * f, o.z + v.z * f, o.w + v.w * f);
-  }
-  return o;
-}
-template <int TYPE, int NT> __device__ __forceinline__ void store_joined(const Call &k, const Row<NT> &w, int c, int x, const float4 &o, float m, float l) {
-  const int col = w.tile * 8 * NT + c, row = w.r.start + col / k.group, head = w.head * k.group + col % k.group;
-  const float f = l == 0.f ? 0.f : __ldg(k.c.v_scale + w.head) / l;
-  *reinterpret_cast<uint2 *>(out_row(k, row, head) + 4 * x) = make_uint2(from_floats<TYPE>(o.x * f, o.y * f), from_floats<TYPE>(o.z * f, o.w * f));
-  if (k.a.lse && x == 0) k.a.lse[(size_t)row * k.a.q_heads + head] = lse_of(m, l);
-}
-
-template <int TYPE, int NT> __global__ void __launch_bounds__(THREADS, 1) stream_kernel(const Call k) {
+template <int TYPE, int NT> __global__ void __launch_bounds__(THREADS<NT>, 1) stream_kernel(const Call k) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   Smem<NT> &sm = *reinterpret_cast<Smem<NT> *>(smem_raw);
   static_assert(fits<NT>, "a run's last piece lies in the ring");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (lane < STAGES) fbla::mbar_init(&sm.full[warp][lane], 1);
+  if (lane < STAGES<NT>) fbla::mbar_init(&sm.full[warp][lane], 1);
   fbla::mbar_init_fence();
   fbla::wait_previous_pass();
   fbla::allow_next_pass();
 
   // the requests' units
   long long total = 0;
-  for (int b0 = 0; b0 < k.a.batch; b0 += THREADS) {
+  for (int b0 = 0; b0 < k.a.batch; b0 += THREADS<NT>) {
     const int b = b0 + tid;
     const long long n = b < k.a.batch ? units_of<NT>(k, request(k, b)) : 0;
     long long sum = n;
@@ -345,7 +323,7 @@ template <int TYPE, int NT> __global__ void __launch_bounds__(THREADS, 1) stream
     __syncthreads();
     long long base = total;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
+    for (int w = 0; w < WARPS<NT>; ++w) {
       if (w < warp) base += sm.warp_sum[w];
       total += sm.warp_sum[w];
     }
@@ -356,8 +334,8 @@ template <int TYPE, int NT> __global__ void __launch_bounds__(THREADS, 1) stream
   if (lane < 2) sm.tag[2 * warp + lane] = -1;
   __syncthreads();
 
-  const Deal deal{total, (int)gridDim.x * WARPS};
-  const int me = blockIdx.x * WARPS + warp;
+  const Deal deal{total, (int)gridDim.x * WARPS<NT>};
+  const int me = blockIdx.x * WARPS<NT> + warp;
   const long long lo = deal.first(me), hi = deal.first(me + 1);
   const int count = (int)(hi - lo);
   if (count > 0) {
@@ -384,16 +362,16 @@ template <int TYPE, int NT> __global__ void __launch_bounds__(THREADS, 1) stream
     const uint8_t *now = address(lane), *next = address(32 + lane);
     uint32_t now_there = __ballot_sync(FULL, now != nullptr);
     auto issue = [&](int i, const uint8_t *from) {  // by the lane that has block i's address
-      uint64_t *const bar = &sm.full[warp][i % STAGES];
+      uint64_t *const bar = &sm.full[warp][i % STAGES<NT>];
       if (from) {
         fbla::fence_async_smem();
         fbla::mbar_expect_tx(bar, BLOCK_BYTES);
-        fbla::bulk_g2s(sm.ring[warp][i % STAGES], from, BLOCK_BYTES, bar);
+        fbla::bulk_g2s(sm.ring[warp][i % STAGES<NT>], from, BLOCK_BYTES, bar);
       } else {
         asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(fbla::smem_u32(bar)) : "memory");
       }
     };
-    if (lane < STAGES && lane < count) issue(lane, now);
+    if (lane < STAGES<NT> && lane < count) issue(lane, now);
 
     int b = request_at(lo);
     bool first = true, alive = true;
@@ -407,15 +385,15 @@ template <int TYPE, int NT> __global__ void __launch_bounds__(THREADS, 1) stream
       s.clear();
       int token = (int)(lo + i - w.unit0) * BT;
       for (; i < end; ++i, token += BT) {
-        const int stage = i % STAGES;
-        if (alive) alive = fbla::mbar_wait_bounded(&sm.full[warp][stage], (i / STAGES) & 1);
+        const int stage = i % STAGES<NT>;
+        if (alive) alive = fbla::mbar_wait_bounded(&sm.full[warp][stage], (i / STAGES<NT>) & 1);
         alive = __all_sync(FULL, alive);
         if (alive && (now_there >> (i & 31) & 1)) {
           if (token + BT - 1 <= Q.low) take_block<TYPE, NT, false>(sm.ring[warp][stage], Q, s, token, w.r.tokens, lane);
           else take_block<TYPE, NT, true>(sm.ring[warp][stage], Q, s, token, w.r.tokens, lane);
         }
         __syncwarp();
-        const int ahead = i + STAGES;
+        const int ahead = i + STAGES<NT>;
         if (alive && ahead < count && lane == (ahead & 31)) issue(ahead, (ahead >> 5) == (i >> 5) ? now : next);
         if ((i & 31) == 31) {
           now = next;
@@ -440,14 +418,14 @@ template <int TYPE, int NT> __global__ void __launch_bounds__(THREADS, 1) stream
   __syncthreads();
 
   // rows that this CTA's warps share
-  const long long cta_lo = deal.first(blockIdx.x * WARPS), cta_hi = deal.first((blockIdx.x + 1) * WARPS);
+  const long long cta_lo = deal.first(blockIdx.x * WARPS<NT>), cta_hi = deal.first((blockIdx.x + 1) * WARPS<NT>);
   auto piece = [&](int p) -> Piece<NT> & { return p & 1 ? *reinterpret_cast<Piece<NT> *>(sm.ring[p >> 1][0]) : sm.first[p >> 1]; };
-  for (int p = 0; p < 2 * WARPS;) {
+  for (int p = 0; p < 2 * WARPS<NT>;) {
     const long long tag = sm.tag[p];
     if (tag < 0) { ++p; continue; }
-    int list[WARPS + 1], pieces = 0;  // (a row's pieces in this CTA are one per warp)
-    for (; p < 2 * WARPS && (sm.tag[p] == tag || sm.tag[p] < 0); ++p)
-      if (sm.tag[p] == tag && pieces <= WARPS) list[pieces++] = p;
+    int list[WARPS<NT> + 1], pieces = 0;  // (a row's pieces in this CTA are one per warp)
+    for (; p < 2 * WARPS<NT> && (sm.tag[p] == tag || sm.tag[p] < 0); ++p)
+      if (sm.tag[p] == tag && pieces <= WARPS<NT>) list[pieces++] = p;
     int b = 0;
     for (int e = k.a.batch; e - b > 1;) {
       const int mid = (b + e) >> 1;
@@ -455,34 +433,34 @@ template <int TYPE, int NT> __global__ void __launch_bounds__(THREADS, 1) stream
     }
     const Row<NT> w = row_at<NT>(k, sm.before, b, tag);
     const bool whole = tag >= cta_lo && tag + w.blocks <= cta_hi;
-    float *const slot = k.part + ((size_t)blockIdx.x * 2 + (tag < cta_lo ? 0 : 1)) * 8 * NT * PSTRIDE;
-    for (int e = tid; e < w.columns * 32; e += THREADS) {
-      const int c = e >> 5, x = e & 31;
+    float *const slot = k.stream_part + ((size_t)blockIdx.x * 2 + (tag < cta_lo ? 0 : 1)) * 8 * NT * PSTRIDE;
+    for (int e = tid; e < w.columns * 32; e += THREADS<NT>) {
+      const int c = e >> 5, x = e & 31, col = w.tile * 8 * NT + c;
       float m, l;
       const float4 o = join(pieces, [&](int i) { return (const float *)piece(list[i]).o[c]; }, x, m, l);
       if (whole) {
-        store_joined<TYPE, NT>(k, w, c, x, o, m, l);
+        store_joined<TYPE>(k, w.r.start + col / k.group, w.head, w.head * k.group + col % k.group, x, o, m, l);
       } else {
         __stcg(reinterpret_cast<float4 *>(slot + c * PSTRIDE) + x, o);
         if (x == 0) __stcg(reinterpret_cast<float2 *>(slot + c * PSTRIDE + D), make_float2(m, l));
       }
     }
     if (!whole) {  // the last of the row's CTAs joins their slots
-      const int c0 = deal.warp_of(tag) / WARPS, c1 = deal.warp_of(tag + w.blocks - 1) / WARPS;
+      const int c0 = deal.warp_of(tag) / WARPS<NT>, c1 = deal.warp_of(tag + w.blocks - 1) / WARPS<NT>;
       __threadfence();
       __syncthreads();
       if (tid == 0) {
-        sm.last = atomicAdd(k.counters + c0, 1) == c1 - c0;
-        if (sm.last) k.counters[c0] = 0;
+        sm.last = atomicAdd(k.stream_counters + c0, 1) == c1 - c0;
+        if (sm.last) k.stream_counters[c0] = 0;
       }
       __syncthreads();
       if (sm.last) {
         __threadfence();
-        for (int e = tid; e < w.columns * 32; e += THREADS) {
-          const int c = e >> 5, x = e & 31;
+        for (int e = tid; e < w.columns * 32; e += THREADS<NT>) {
+          const int c = e >> 5, x = e & 31, col = w.tile * 8 * NT + c;
           float m, l;
-          const float4 o = join(c1 - c0 + 1, [&](int i) { return k.part + ((size_t)(c0 + i) * 2 + (i ? 0 : 1)) * 8 * NT * PSTRIDE + c * PSTRIDE; }, x, m, l);
-          store_joined<TYPE, NT>(k, w, c, x, o, m, l);
+          const float4 o = join(c1 - c0 + 1, [&](int i) { return k.stream_part + ((size_t)(c0 + i) * 2 + (i ? 0 : 1)) * 8 * NT * PSTRIDE + c * PSTRIDE; }, x, m, l);
+          store_joined<TYPE>(k, w.r.start + col / k.group, w.head, w.head * k.group + col % k.group, x, o, m, l);
         }
       }
     }
@@ -498,26 +476,18 @@ template <int TYPE, int NT> __global__ void __launch_bounds__(THREADS, 1) stream
     for (int row = max(__ldg(k.a.starts + k.a.batch), 0) + me; row < k.a.tokens; row += deal.warps) clear_row(k, row, lane);
 }
 
-template <int TYPE, int NT> cudaError_t stream(const Call &k, int sms, cudaStream_t stream) {
-  static thread_local int configured[64] = {0};
-  const size_t smem = sizeof(Smem<NT>) + ((size_t)k.a.batch + 1) * sizeof(long long);
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (!(dev < 64 && configured[dev])) {
-    const cudaError_t e = cudaFuncSetAttribute(stream_kernel<TYPE, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
-    if (e != cudaSuccess) return e;
-    if (dev < 64) configured[dev] = 1;
-  }
-  return fbla::launch(true, 1, stream_kernel<TYPE, NT>, dim3(sms), THREADS, smem, stream, k);
-}
-
 }  // namespace
+
+template <int TYPE, int NT> cudaError_t launch_stream(const Call &k, int sms, cudaStream_t stream) {
+  static thread_local bool ready[64] = {false};
+  const cudaError_t e = allow_shared(stream_kernel<TYPE, NT>, ready);
+  if (e != cudaSuccess) return e;
+  return fbla::launch(true, 1, stream_kernel<TYPE, NT>, dim3(sms), THREADS<NT>, offsetof(Smem<NT>, before) + ((size_t)k.a.batch + 1) * sizeof(long long), stream, k);
+}
+template cudaError_t launch_stream<MLOPS_PAGED_BF16, 1>(const Call &, int, cudaStream_t);
+template cudaError_t launch_stream<MLOPS_PAGED_FP16, 1>(const Call &, int, cudaStream_t);
+template cudaError_t launch_stream<MLOPS_PAGED_BF16, 2>(const Call &, int, cudaStream_t);
+template cudaError_t launch_stream<MLOPS_PAGED_FP16, 2>(const Call &, int, cudaStream_t);
+
 }  // namespace paged
 
-extern "C" size_t paged_k_attend_scratch(int sms) { return ((size_t)sms * sizeof(int) + 255) / 256 * 256 + (size_t)sms * 2 * 8 * paged::PSTRIDE * sizeof(float); }
-
-extern "C" cudaError_t paged_k_attend_launch(const mlops_paged_attend_args *a, const mlops_paged_cache *c, void *scratch, int sms, cudaStream_t stream) {
-  const size_t counters = ((size_t)sms * sizeof(int) + 255) / 256 * 256;
-  const paged::Call k{*a, *c, a->scale * 1.4426950408889634f, a->q_heads / c->kv_heads, reinterpret_cast<float *>(static_cast<char *>(scratch) + counters), static_cast<int *>(scratch)};
-  return a->type == MLOPS_PAGED_BF16 ? paged::stream<MLOPS_PAGED_BF16, 1>(k, sms, stream) : paged::stream<MLOPS_PAGED_FP16, 1>(k, sms, stream);
-}
