@@ -77,7 +77,7 @@ mlops_fbla_status mlops_paged_append(const mlops_paged_cache *cache, int tokens,
 mlops_fbla_status mlops_paged_read(const mlops_paged_cache *cache, int tokens, int type, const int *slots, void *k, void *v, cudaStream_t stream);
 
 typedef struct mlops_paged_attend_args {
-  int batch, tokens, q_heads, type;    /* tokens: rows of q; kv_heads divides q_heads; batch at most 4096 */
+  int batch, tokens, q_heads, type;    /* tokens: rows of q; kv_heads divides q_heads; batch at most 2048 */
   const void *q;                       /* [tokens][q_heads][128], strides in elements: multiples of 8 */
   int64_t q_token_stride, q_head_stride;
   void *out;                           /* likewise */

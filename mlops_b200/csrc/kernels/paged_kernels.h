@@ -9,7 +9,7 @@ extern "C" {
 
 /* requests of one call: their prefix sums live in shared memory */
 #define PAGED_K_MAX_ASSIGNED 16384
-#define PAGED_K_MAX_ATTENDED 4096
+#define PAGED_K_MAX_ATTENDED 2048
 
 cudaError_t paged_k_assign_launch(const mlops_paged_assign_args *a, cudaStream_t stream);
 cudaError_t paged_k_append_launch(const mlops_paged_cache *c, int tokens, int type, const void *k, int64_t k_ts, int64_t k_hs, const void *v, int64_t v_ts,
