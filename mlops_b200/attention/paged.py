@@ -12,6 +12,7 @@ Elements take 4.5 bits: E2M1 codes, an E4M3 scale per 16 channels, an FP32 facto
 Nothing here synchronises, so that a step can be captured into a CUDA graph.
 """
 import ctypes
+import struct
 from dataclasses import dataclass
 from typing import NamedTuple, Optional, Tuple, Union
 
@@ -55,7 +56,9 @@ _lib.mlops_paged_attend.argtypes = [_vp, _vp, _vp, ctypes.c_size_t, _vp]
 _lib.mlops_paged_attend_scratch_bytes.argtypes = [_vp, _int]
 _lib.mlops_paged_attend_scratch_bytes.restype = ctypes.c_size_t
 _lib.mlops_paged_last_error.restype = ctypes.c_char_p
-
+# the structures as the calls below pass them: their bytes (a third of the host's time that ctypes takes to fill one; addresses of 0 are null)
+_CACHE, _ASSIGN, _ATTEND = struct.Struct("@PPPqqiii4x"), struct.Struct("@iiiiqPPPPiPPPPPP"), struct.Struct("@iiiiPqqPqqPPqiPPf4x")
+assert (_CACHE.size, _ASSIGN.size, _ATTEND.size) == (ctypes.sizeof(_Cache), ctypes.sizeof(_Assign), ctypes.sizeof(_Attend))
 
 _scratch = _C._ScratchPool(torch.zeros)  # (zeros at first; every call leaves its counters as it found them)
 
@@ -107,43 +110,47 @@ def empty(pages: int, kv_heads: int, page_size: int = 64, *, k_scale: Optional[t
 
 
 def _pool(c):
-    """A pool's arrays, checked: the structure that names them to the library, their device's index."""
+    """A pool's arrays, checked: the structure that names them to the library, its pages' KV heads, its device's index."""
     u, ks, vs = c.units, c.k_scale, c.v_scale
     index = u.get_device()
     if not 0 <= index == ks.get_device() == vs.get_device():
         raise ValueError(f"the arrays of a paged cache have to live on the same CUDA device (units: {u.device}, scales: {ks.device}, {vs.device})")
-    if u.dim() != 4 or u.dtype is not torch.uint8 or u.size(3) != BLOCK_BYTES or u.stride(3) != 1 or (u.size(2) > 1 and u.stride(2) != BLOCK_BYTES):
-        raise ValueError(f"units has to be a uint8 [pages, kv_heads, blocks, {BLOCK_BYTES}] tensor with dense pages; it is {u.dtype} {tuple(u.shape)}, strides {u.stride()}")
-    pages, heads, blocks, _ = u.shape
-    for s in (ks, vs):
-        if s.dtype is not _F32 or s.dim() != 1 or s.size(0) != heads or not s.is_contiguous():
-            raise ValueError(f"k_scale and v_scale have to be contiguous float32 [{heads}] tensors; one is {s.dtype} {tuple(s.shape)}")
-    return _Cache(u.data_ptr(), ks.data_ptr(), vs.data_ptr(), u.stride(0), u.stride(1), pages, blocks * BLOCK, heads), index
+    shape, strides = u.shape, u.stride()
+    if u.dtype is not torch.uint8 or len(shape) != 4 or shape[3] != BLOCK_BYTES or strides[3] != 1 or (strides[2] != BLOCK_BYTES and shape[2] > 1):
+        raise ValueError(f"units has to be a uint8 [pages, kv_heads, blocks, {BLOCK_BYTES}] tensor with dense pages; it is {u.dtype} {tuple(shape)}, strides {strides}")
+    pages, heads, blocks, _ = shape
+    if not (ks.dtype is vs.dtype is _F32 and ks.shape == vs.shape == (heads,) and ks.is_contiguous() and vs.is_contiguous()):
+        raise ValueError(f"k_scale and v_scale have to be contiguous float32 [{heads}] tensors; they are {ks.dtype} {tuple(ks.shape)} and {vs.dtype} {tuple(vs.shape)}")
+    return _CACHE.pack(u.data_ptr(), ks.data_ptr(), vs.data_ptr(), strides[0], strides[1], pages, blocks * BLOCK, heads), heads, index
 
 
-def _ints(x, index, what, size, dtype=_I32):
-    if x.get_device() != index or x.dtype is not dtype or x.dim() != 1 or not x.is_contiguous() or (size is not None and x.size(0) != size):
-        raise ValueError(f"{what}: expected a contiguous {dtype} [{'n' if size is None else size}] tensor on cuda:{index}; it is {x.dtype} {tuple(x.shape)} on {x.device}")
+def _ints(x, index, what, size=None, dtype=_I32):
+    shape = x.shape
+    if x.get_device() != index or x.dtype is not dtype or len(shape) != 1 or not x.is_contiguous() or (size is not None and shape[0] != size):
+        raise ValueError(f"{what}: expected a contiguous {dtype} [{'n' if size is None else size}] tensor on cuda:{index}; it is {x.dtype} {tuple(shape)} on {x.device}")
     return x.data_ptr()
 
 
 def _table(x, index):
-    if x.get_device() != index or x.dtype is not _I32 or x.dim() != 2 or (x.size(1) > 1 and x.stride(1) != 1):
-        raise ValueError(f"table: expected an int32 [batch, width] tensor with dense rows on cuda:{index}; it is {x.dtype} {tuple(x.shape)} on {x.device}")
-    batch, width = x.shape
-    return x.data_ptr(), (x.stride(0) if batch > 1 else width), batch, width
+    shape, strides = x.shape, x.stride()
+    if x.get_device() != index or x.dtype is not _I32 or len(shape) != 2 or (strides[1] != 1 and shape[1] > 1):
+        raise ValueError(f"table: expected an int32 [batch, width] tensor with dense rows on cuda:{index}; it is {x.dtype} {tuple(shape)} on {x.device}")
+    batch, width = shape
+    return x.data_ptr(), (strides[0] if batch > 1 else width), batch, width
 
 
 def _rows(x, index, what, heads=None):
-    """[tokens, heads, 128] rows as the library reads them (dense channels, 16-byte pieces aligned), its type"""
-    kind = _TYPES.get(x.dtype)
-    if x.get_device() != index or kind is None or x.dim() != 3 or x.size(2) != HEAD_DIM or (heads is not None and x.size(1) != heads):
-        raise ValueError(f"{what}: expected a bfloat16 or float16 [tokens, {'heads' if heads is None else heads}, {HEAD_DIM}] tensor on cuda:{index}; it is {x.dtype} {tuple(x.shape)} on {x.device}")
-    if x.stride(2) != 1 or x.stride(0) % 8 or x.stride(1) % 8 or x.data_ptr() % 16:
+    """[tokens, heads, 128] rows as the library reads them (dense channels, 16-byte pieces aligned), their shape, strides and type"""
+    kind, shape = _TYPES.get(x.dtype), x.shape
+    if x.get_device() != index or kind is None or len(shape) != 3 or shape[2] != HEAD_DIM or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{what}: expected a bfloat16 or float16 [tokens, {'heads' if heads is None else heads}, {HEAD_DIM}] tensor on cuda:{index}; it is {x.dtype} {tuple(shape)} on {x.device}")
+    by_token, by_head, by_channel = x.stride()
+    if by_channel != 1 or by_token % 8 or by_head % 8 or x.data_ptr() % 16:
         x = x.contiguous()
         if x.data_ptr() % 16:
             x = x.clone()
-    return x, kind
+        by_token, by_head, _ = x.stride()
+    return x, shape, by_token, by_head, kind
 
 
 def _on(index):
@@ -171,31 +178,30 @@ def assign(table: torch.Tensor, held: torch.Tensor, added: torch.Tensor, free: t
         raise ValueError(f"tokens may not be negative; it is {tokens}")
     if cursor.dim() != 1 or cursor.size(0) not in (2, 3):
         raise ValueError(f"cursor: expected int64 [2] (head, tail) or a Step's; it has shape {tuple(cursor.shape)}")
-    args = (_ints(held, index, "held", batch), _ints(added, index, "added", batch), _ints(free, index, "free", None), free.size(0),
-            _ints(cursor, index, "cursor", None, _I64))
-    slots, positions, starts, lengths = torch.empty((2 * tokens + 2 * batch + 1,), dtype=_I32, device=table.device).split([tokens, tokens, batch + 1, batch])
-    moved = torch.empty((3,), dtype=_I64, device=table.device)
-    call = _Assign(batch, tokens, page_size, width, stride, entries, *args, slots.data_ptr(), positions.data_ptr(), starts.data_ptr(), lengths.data_ptr(), moved.data_ptr())
-    status = _lib.mlops_paged_assign(ctypes.byref(call), _C._raw_stream(index))
+    held_at, added_at, free_at, cursor_at = _ints(held, index, "held", batch), _ints(added, index, "added", batch), _ints(free, index, "free"), _ints(cursor, index, "cursor", None, _I64)
+    moved = torch.empty_like(cursor) if cursor.size(0) == 3 else cursor.new_empty(3)
+    words = held.new_empty(2 * tokens + 2 * batch + 1)
+    at = words.data_ptr()
+    status = _lib.mlops_paged_assign(_ASSIGN.pack(batch, tokens, page_size, width, stride, entries, held_at, added_at, free_at, free.size(0), cursor_at, at, at + 4 * tokens,
+                                                  at + 8 * tokens, at + 8 * tokens + 4 * batch + 4, moved.data_ptr()), _C._raw_stream(index))
     if status:
         _raise(status, "mlops_paged_assign")
-    return Step(slots, positions, starts, lengths, moved)
+    return Step(*words.split_with_sizes([tokens, tokens, batch + 1, batch]), moved)
 
 
-@torch.no_grad()
 def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> PagedCache:
     """Quantise ``k, v [tokens, kv_heads, 128]`` (BF16 or FP16, slices of a fused projection as they are) into the pool's ``slots`` (int32 [tokens]; a
     slot outside the pool, -1 for instance: the token is left out). In place; the cache is also returned."""
-    pool, index = _pool(cache)
+    pool, heads, index = _pool(cache)
     if not _on(index):
         with torch.cuda.device(index):
             return append(cache, k, v, slots)
-    k, kind = _rows(k, index, "k", pool.kv_heads)
-    v, v_kind = _rows(v, index, "v", pool.kv_heads)
-    tokens = k.size(0)
-    if v.size(0) != tokens or v_kind != kind:
+    k, shape, k_by_token, k_by_head, kind = _rows(k, index, "k", heads)
+    v, v_shape, v_by_token, v_by_head, v_kind = _rows(v, index, "v", heads)
+    tokens = shape[0]
+    if v_shape[0] != tokens or v_kind != kind:
         raise ValueError(f"k and v have to be alike; k is {k.dtype} {tuple(k.shape)}, v is {v.dtype} {tuple(v.shape)}")
-    status = _lib.mlops_paged_append(ctypes.byref(pool), tokens, kind, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+    status = _lib.mlops_paged_append(pool, tokens, kind, k.data_ptr(), k_by_token, k_by_head, v.data_ptr(), v_by_token, v_by_head,
                                      _ints(slots, index, "slots", tokens), _C._raw_stream(index))
     if status:
         _raise(status, "mlops_paged_append")
@@ -205,23 +211,22 @@ def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Ten
 def read(cache: PagedCache, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
     """What the pool holds in ``slots`` (int32 [tokens]): K and V as ``[tokens, kv_heads, 128]``, rounded once to ``dtype`` (BF16 or FP16). Zeros for a
     slot outside the pool."""
-    pool, index = _pool(cache)
+    pool, heads, index = _pool(cache)
     kind = _TYPES.get(dtype)
     if kind is None:
         raise ValueError(f"dtype has to be bfloat16 or float16, not {dtype}")
     if not _on(index):
         with torch.cuda.device(index):
             return read(cache, slots, dtype)
-    where = _ints(slots, index, "slots", None)
-    k = torch.empty((slots.size(0), pool.kv_heads, HEAD_DIM), dtype=dtype, device=cache.units.device)
+    where, tokens = _ints(slots, index, "slots"), slots.size(0)
+    k = torch.empty((tokens, heads, HEAD_DIM), dtype=dtype, device=slots.device)
     v = torch.empty_like(k)
-    status = _lib.mlops_paged_read(ctypes.byref(pool), slots.size(0), kind, where, k.data_ptr(), v.data_ptr(), _C._raw_stream(index))
+    status = _lib.mlops_paged_read(pool, tokens, kind, where, k.data_ptr(), v.data_ptr(), _C._raw_stream(index))
     if status:
         _raise(status, "mlops_paged_read")
     return k, v
 
 
-@torch.no_grad()
 def attend(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor] = None, *, scale: float = 0.0,
            return_lse: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """Causal attention of the requests' newest tokens over their pages.
@@ -231,23 +236,22 @@ def attend(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, lengths: tor
     query per request. Row i of n sees the request's tokens up to ``lengths[b] - n + i``. Returns ``[tokens, q_heads, 128]`` of q's type, zeros for a
     row that sees nothing and for rows of no request; with ``return_lse`` also the natural log-sum-exp of the rows' scaled scores, float32
     [tokens, q_heads] (-inf for such rows). ``scale`` 0 selects 1/sqrt(128)."""
-    pool, index = _pool(cache)
+    pool, kv_heads, index = _pool(cache)
     if not _on(index):
         with torch.cuda.device(index):
             return attend(q, cache, table, lengths, starts, scale=scale, return_lse=return_lse)
-    q, kind = _rows(q, index, "q")
+    q, (tokens, heads, _), by_token, by_head, kind = _rows(q, index, "q")
     entries, stride, batch, width = _table(table, index)
-    tokens, heads = q.size(0), q.size(1)
     where = _ints(lengths, index, "lengths", batch)
-    begins = None if starts is None else _ints(starts, index, "starts", batch + 1)
-    out = torch.empty((tokens, heads, HEAD_DIM), dtype=q.dtype, device=q.device)
-    lse = torch.empty((tokens, heads), dtype=_F32, device=q.device) if return_lse else None
-    call = _Attend(batch, tokens, heads, kind, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), heads * HEAD_DIM, HEAD_DIM,
-                   lse.data_ptr() if return_lse else None, entries, stride, width, where, begins, scale)
+    begins = 0 if starts is None else _ints(starts, index, "starts", batch + 1)
+    out = q.new_empty((tokens, heads, HEAD_DIM))
+    lse = q.new_empty((tokens, heads), dtype=_F32) if return_lse else None
+    call = _ATTEND.pack(batch, tokens, heads, kind, q.data_ptr(), by_token, by_head, out.data_ptr(), heads * HEAD_DIM, HEAD_DIM, lse.data_ptr() if return_lse else 0,
+                        entries, stride, width, where, begins, scale)
     stream = _C._raw_stream(index)
-    scratch = _scratch.get(q.device, stream, max(16, _lib.mlops_paged_attend_scratch_bytes(ctypes.byref(call), pool.kv_heads)))
+    scratch = _scratch.get(q.device, stream, max(16, _lib.mlops_paged_attend_scratch_bytes(call, kv_heads)))
     with scratch.lock:
-        status = _lib.mlops_paged_attend(ctypes.byref(call), ctypes.byref(pool), scratch.pointer, scratch.bytes, stream)
+        status = _lib.mlops_paged_attend(call, pool, scratch.pointer, scratch.bytes, stream)
     if status:
         _raise(status, "mlops_paged_attend")
     return (out, lse) if return_lse else out
