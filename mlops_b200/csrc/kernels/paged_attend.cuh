@@ -68,19 +68,21 @@ __device__ __forceinline__ void clear_row(const Call &k, int row, int lane) {
     for (int i = lane; i < k.a.q_heads; i += 32) k.a.lse[(size_t)row * k.a.q_heads + i] = -FBLA_INF;
 }
 
-// joins `count` partial rows, source(i) the i-th: channels 4 x .. 4 x + 3, the running maximum and sum
+// joins `count` partial rows of other CTAs, source(i) the i-th: channels 4 x .. 4 x + 3, the running maximum and sum
 template <class F> __device__ __forceinline__ float4 join(int count, F source, int x, float &m, float &l) {
   m = NOTHING;
-  for (int i = 0; i < count; ++i) m = fmaxf(m, source(i)[D]);
+#pragma unroll 8
+  for (int i = 0; i < count; ++i) m = fmaxf(m, __ldcg(source(i) + D));
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   l = 0.f;
 #pragma unroll 4
   for (int i = 0; i < count; ++i) {
     const float *const p = source(i);
-    const float f = ex2(p[D] - m);
-    const float4 v = *reinterpret_cast<const float4 *>(p + 4 * x);
-    l += p[D + 1] * f;
-    o = make_float4(o.x + v.x * f, o.y + v.y * f, o.z + v.z * f, o.w + v.w * f);
+    const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p + D));
+    const float f = ex2(ml.x - m);
+    const float4 v = __ldcg(reinterpret_cast<const float4 *>(p) + x);
+    l += ml.y * f;
+    o = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w));
   }
   return o;
 }

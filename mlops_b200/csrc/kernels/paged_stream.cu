@@ -1,13 +1,13 @@
 // Attention over the paged cache for few queries per request (mlops_paged_attend): the pages are streamed once, bound by their bytes.
 //
 // A row of work is (request, KV head, tile of 8 NT columns); a column is one of the request's queries with one of the KV head's query heads. A row's
-// unit is a block of 16 tokens, 2304 contiguous bytes. All rows' units form one list, which the grid's warps share out in equal contiguous runs, so that
-// ragged lengths cost nothing; a warp brings its run's blocks through a ring of its own in shared memory with bulk copies.
+// unit is a pair of blocks, 32 tokens, 2304 contiguous bytes each. All rows' units form one list, which the grid's warps share out in equal contiguous runs,
+// so that ragged lengths cost nothing; a warp brings its run's blocks through a ring of its own in shared memory with bulk copies.
 //
 // Per block, tokens on the M axis: S^T[16 tokens x 8] = K Q^T and O^T[128 channels x 8] += V^T P^T with mma.sync m16n8k16, FP16 operands, FP32 sums.
-// K and V: code * scale is exact in FP16. Q: FP16 after a power of two per column (q_factor). P: 2^(s - m') with m' between 9 and 15 below the column's largest score so far, rounded to
-// FP16 (relative 2^-11, the only rounding of the operands); m' moves, and O and l are rescaled, only where a score would pass 2^15. l sums the
-// unrounded P. Weights below 2^-33 of the largest are lost, 2^17 of them are 2^-16 of the sum.
+// K and V: code * scale is exact in FP16. Q: FP16 after a power of two per column (q_factor). P: 2^(s - m') with m' between 9 and 15 below the column's
+// largest score so far, rounded to FP16 (relative 2^-11, the only rounding of the operands); m' moves, and O and l are rescaled, only where a score would
+// pass 2^15. l sums the unrounded P. Weights below 2^-33 of the largest are lost, 2^17 of them are 2^-16 of the sum.
 //
 // Channels and tokens are dealt to the fragments so that a lane's operands are whole words: for K lane (g, t) takes channels 32 t .. 32 t + 31 of its two
 // tokens (the order of the K extent of a product is free as long as Q has the same); for V it takes channels 16 g .. 16 g + 15 of four tokens, and two
@@ -21,25 +21,25 @@
 namespace paged {
 namespace {
 
-template <int NT> constexpr int WARPS = NT == 1 ? 16 : 10;   // what the shared memory has room for beside the rings
-template <int NT> constexpr int STAGES = NT == 1 ? 3 : 4;
+template <int NT> constexpr int WARPS = NT == 1 ? 16 : 10;  // what the shared memory has room for beside the rings
+constexpr int STAGES = 2, UNIT = 2 * BT;  // tokens of a unit
 template <int NT> constexpr int THREADS = 32 * WARPS<NT>;
-constexpr int MIN_SHARE = 4;  // units of a warp, at least, where the work allows a choice
+constexpr int MIN_SHARE = 2;  // units of a warp, at least, where the work allows a choice
 constexpr float TOP = 15.f, REST = 9.f;  // log2 of the largest P, and of a column's largest when m' is set
 
 template <int NT> struct Piece {  // a warp's partial rows of one row of work
   float o[8 * NT][PSTRIDE];        // (o[128], m', l)
 };
 template <int NT> struct __align__(128) Smem {
-  uint8_t ring[WARPS<NT>][STAGES<NT>][BLOCK_BYTES];
-  Piece<NT> first[WARPS<NT>];          // of a run's first row; the last row's piece takes the ring's place when that is through
-  uint64_t full[WARPS<NT>][STAGES<NT>];
-  long long tag[2 * WARPS<NT>];        // pieces in the order of the tokens: the first unit of the piece's row, -1: none
-  long long warp_sum[WARPS<NT>];
+  uint8_t ring[WARPS<NT>][STAGES][2][BLOCK_BYTES];
+  Piece<NT> first[WARPS<NT>];      // of a run's first row; the last row's piece takes the ring's place when that is through
+  uint64_t full[WARPS<NT>][STAGES];
+  int tag[32];                     // pieces in the order of the tokens, two per warp: the first unit of the piece's row, -1: none
+  int warp_sum[WARPS<NT>];
   int last;
-  long long before[];              // [batch + 1]: the requests' first units
+  int before[];                    // [batch + 1]: the requests' first units
 };
-template <int NT> constexpr bool fits = sizeof(Piece<NT>) <= STAGES<NT> * BLOCK_BYTES;
+template <int NT> constexpr bool fits = sizeof(Piece<NT>) <= STAGES * 2 * BLOCK_BYTES;
 
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -57,39 +57,52 @@ __device__ __forceinline__ uint32_t times(uint32_t a, uint32_t b) {
 // token of the block in row r < 8 of the S^T fragment: two even and two odd tokens wherever four or two lanes read at once
 __device__ __forceinline__ int token_of(int r) { return ((r >> 1) ^ (r & 1)) + 4 * (r & 1); }
 
-// How the units are dealt: warp w has units [first(w), first(w + 1)).
+// How the units are dealt: warp w has units [first(w), first(w + 1)), whole + 1 of them for w < more and `whole` for the others (for few units MIN_SHARE,
+// and nothing for the warps behind).
 struct Deal {
-  long long total;
-  int warps;
-  __device__ __forceinline__ bool even() const { return total >= (long long)MIN_SHARE * warps; }
-  __device__ __forceinline__ long long first(int w) const { return even() ? total * w / warps : min(total, (long long)MIN_SHARE * w); }
-  __device__ __forceinline__ int warp_of(long long u) const { return even() ? (int)(((u + 1) * warps - 1) / total) : (int)(u / MIN_SHARE); }
+  int total, whole, more;
+  __device__ __forceinline__ Deal(int total, int warps) : total(total) {
+    const bool few = total < MIN_SHARE * warps;
+    whole = few ? MIN_SHARE : total / warps;
+    more = few ? 0 : total - whole * warps;
+  }
+  __device__ __forceinline__ int first(int w) const { return min(w * whole + min(w, more), total); }
+  __device__ __forceinline__ int warp_of(int u) const { return u < more * (whole + 1) ? u / (whole + 1) : (u - more) / whole; }
 };
 
 // a row of work
 template <int NT> struct Row {
   Request r;
-  int b, head, tile, columns, blocks;
-  long long unit0;  // its first unit
+  int b, head, tile, columns, units;
+  int unit0;  // its first unit
 };
 
-template <int NT> __device__ __forceinline__ int blocks_of(const Request &r) { return (r.tokens + BT - 1) / BT; }
+__device__ __forceinline__ int units_of(const Request &r) { return (r.tokens + UNIT - 1) / UNIT; }  // of each of a request's rows of work
 template <int NT> __device__ __forceinline__ int tiles_of(const Call &k, const Request &r) { return (r.n * k.group + 8 * NT - 1) / (8 * NT); }
-template <int NT> __device__ __forceinline__ long long units_of(const Call &k, const Request &r) {
-  return r.n * k.group > k.wide ? 0 : (long long)k.c.kv_heads * tiles_of<NT>(k, r) * blocks_of<NT>(r);
+template <int NT> __device__ __forceinline__ int all_units_of(const Call &k, const Request &r) {
+  return r.n * k.group > k.wide ? 0 : k.c.kv_heads * tiles_of<NT>(k, r) * units_of(r);
 }
 
+// the request that unit u belongs to: before[b] <= u < before[b + 1]
+__device__ __forceinline__ int request_at(const Call &k, const int *before, int u) {
+  int a = 0;
+  for (int b = k.a.batch; b - a > 1;) {
+    const int mid = (a + b) >> 1;
+    if (before[mid] <= u) a = mid; else b = mid;
+  }
+  return a;
+}
 // the row that unit u (of request b) belongs to
-template <int NT> __device__ __forceinline__ Row<NT> row_at(const Call &k, const long long *before, int b, long long u) {
+template <int NT> __device__ __forceinline__ Row<NT> row_at(const Call &k, const int *before, int b, int u) {
   Row<NT> w;
   w.b = b;
   w.r = request(k, b);
-  w.blocks = blocks_of<NT>(w.r);
-  const int tiles = tiles_of<NT>(k, w.r), row = (int)((u - before[b]) / w.blocks);
-  w.head = row / tiles;
-  w.tile = row % tiles;
+  w.units = units_of(w.r);
+  const int tiles = tiles_of<NT>(k, w.r), row = (u - before[b]) / w.units;
+  w.head = tiles == 1 ? row : row / tiles;
+  w.tile = row - w.head * tiles;
   w.columns = min(w.r.n * k.group - w.tile * 8 * NT, 8 * NT);
-  w.unit0 = before[b] + (long long)row * w.blocks;
+  w.unit0 = before[b] + row * w.units;
   return w;
 }
 
@@ -102,14 +115,16 @@ template <int TYPE, int NT> struct Columns {  // a row's queries, as B fragments
   __device__ __forceinline__ void load(const Call &k, const Row<NT> &w, int lane) {
     const int g = lane >> 2, t = lane & 3;
     const float base = k.sl * __ldg(k.c.k_scale + w.head);
-    low = w.r.length - w.r.n + w.tile * 8 * NT / k.group;
+    low = w.r.length - w.r.n + query_of(k, w.tile * 8 * NT);
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       const int c = 8 * j + g, col = w.tile * 8 * NT + c;
       uint4 raw[4] = {};
       if (c < w.columns) {
-        const uint16_t *const src = static_cast<const uint16_t *>(k.a.q) + (int64_t)(w.r.start + col / k.group) * k.a.q_token_stride +
-                                    (int64_t)(w.head * k.group + col % k.group) * k.a.q_head_stride + 32 * t;
+        int query, head;
+        split_column(k, col, query, head);
+        const uint16_t *const src = static_cast<const uint16_t *>(k.a.q) + (int64_t)(w.r.start + query) * k.a.q_token_stride +
+                                    (int64_t)(w.head * k.group + head) * k.a.q_head_stride + 32 * t;
 #pragma unroll
         for (int e = 0; e < 4; ++e) raw[e] = __ldg(reinterpret_cast<const uint4 *>(src) + e);
       }
@@ -132,9 +147,9 @@ template <int TYPE, int NT> struct Columns {  // a row's queries, as B fragments
       for (int i = 0; i < 16; ++i) q[j][i] = from_floats<MLOPS_PAGED_FP16>(x[i].x * up, x[i].y * up);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        mult[j][i] = base * __shfl_sync(FULL, down, (2 * t + i) * 4);
+        mult[j][i] = fmaxf(base * __shfl_sync(FULL, down, (2 * t + i) * 4), 1e-37f);  // (not 0: masked scores are -infinity)
         const int cc = 8 * j + 2 * t + i;
-        limit[j][i] = cc < w.columns ? w.r.length - w.r.n + (w.tile * 8 * NT + cc) / k.group : -1;
+        limit[j][i] = cc < w.columns ? w.r.length - w.r.n + query_of(k, w.tile * 8 * NT + cc) : -1;
       }
     }
   }
@@ -164,75 +179,36 @@ template <int NT> struct Sums {
   }
 };
 
-// one block of 16 tokens, the first of which is `token`; EDGE: some column does not see all of it
-template <int TYPE, int NT, bool EDGE>
-__device__ __forceinline__ void take_block(const uint8_t *block, const Columns<TYPE, NT> &Q, Sums<NT> &s, int token, int tokens, int lane) {
-  const int g = lane >> 2, t = lane & 3, row = token_of(g);
-  float acc[NT][4], odd[NT][4];
+// S^T of a block, in score units of the product
+template <int TYPE, int NT> __device__ __forceinline__ void scores(const uint8_t *block, const Columns<TYPE, NT> &Q, float (&acc)[NT][4], int lane) {
+  const int t = lane & 3, row = token_of(lane >> 2);
 #pragma unroll
   for (int j = 0; j < NT; ++j)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[j][e] = odd[j][e] = 0.f;
-  {
-    const uint4 ka = fbla::lds128(block + row * CODE_BYTES + 16 * t), kb = fbla::lds128(block + (row + 8) * CODE_BYTES + 16 * t);
-    const uint32_t sa = scales_to_half2(*reinterpret_cast<const uint16_t *>(block + K_SCALES + row * SCALE_BYTES + 2 * t));
-    const uint32_t sb = scales_to_half2(*reinterpret_cast<const uint16_t *>(block + K_SCALES + (row + 8) * SCALE_BYTES + 2 * t));
-    const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+    for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
+  const uint4 ka = fbla::lds128(block + row * CODE_BYTES + 16 * t), kb = fbla::lds128(block + (row + 8) * CODE_BYTES + 16 * t);
+  const uint32_t sa = scales_to_half2(*reinterpret_cast<const uint16_t *>(block + K_SCALES + row * SCALE_BYTES + 2 * t));
+  const uint32_t sb = scales_to_half2(*reinterpret_cast<const uint16_t *>(block + K_SCALES + (row + 8) * SCALE_BYTES + 2 * t));
+  const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t ha[4], hb[4];
-      codes_to_half2(wa[i], ha);
-      codes_to_half2(wb[i], hb);
-      const uint32_t xa = __byte_perm(sa, 0, i < 2 ? 0x1010 : 0x3232), xb = __byte_perm(sb, 0, i < 2 ? 0x1010 : 0x3232);
+  for (int i = 0; i < 4; ++i) {
+    uint32_t ha[4], hb[4];
+    codes_to_half2(wa[i], ha);
+    codes_to_half2(wb[i], hb);
+    const uint32_t xa = __byte_perm(sa, 0, i < 2 ? 0x1010 : 0x3232), xb = __byte_perm(sb, 0, i < 2 ? 0x1010 : 0x3232);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) ha[e] = times(ha[e], xa), hb[e] = times(hb[e], xb);
+    for (int e = 0; e < 4; ++e) ha[e] = times(ha[e], xa), hb[e] = times(hb[e], xb);
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        mma(acc[j], ha[0], hb[0], ha[1], hb[1], Q.q[j][4 * i], Q.q[j][4 * i + 1]);
-        mma(odd[j], ha[2], hb[2], ha[3], hb[3], Q.q[j][4 * i + 2], Q.q[j][4 * i + 3]);
-      }
+    for (int j = 0; j < NT; ++j) {
+      mma(acc[j], ha[0], hb[0], ha[1], hb[1], Q.q[j][4 * i], Q.q[j][4 * i + 1]);
+      mma(acc[j], ha[2], hb[2], ha[3], hb[3], Q.q[j][4 * i + 2], Q.q[j][4 * i + 3]);
     }
   }
-  // scores in log2 units, element e of the fragment: token row + 8 (e / 2), column 2 t + e % 2
-  float high = NOTHING;
-#pragma unroll
-  for (int j = 0; j < NT; ++j)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float x = (acc[j][e] + odd[j][e]) * Q.mult[j][e & 1];
-      if (EDGE && token + row + 8 * (e >> 1) > Q.limit[j][e & 1]) x = -FBLA_INF;
-      acc[j][e] = x;
-      high = fmaxf(high, x - s.m[j][e & 1]);
-    }
-  if (__any_sync(FULL, high > TOP)) {
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float x = fmaxf(acc[j][i], acc[j][2 + i]);
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(FULL, x, d));
-        if (x - s.m[j][i] > TOP) {
-          const float m = x - REST, keep = ex2(s.m[j][i] - m);
-          s.m[j][i] = m;
-          s.l[j][i] *= keep;
-#pragma unroll
-          for (int n = 0; n < 8; ++n) s.o[j][n][i] *= keep, s.o[j][n][2 + i] *= keep;
-        }
-      }
-  }
-  uint32_t p[NT][2];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      acc[j][e] = ex2(acc[j][e] - s.m[j][e & 1]);
-      s.l[j][e & 1] += acc[j][e];
-    }
-    p[j][0] = transpose8(from_floats<MLOPS_PAGED_FP16>(acc[j][0], acc[j][1]));
-    p[j][1] = transpose8(from_floats<MLOPS_PAGED_FP16>(acc[j][2], acc[j][3]));
-  }
-  // V: rows 2 t, 2 t + 1 (and + 8) of the K extent are tokens t, (t ^ 1) + 4 (and + 8)
+}
+// O^T += V^T P^T of a block; of its tokens only the first `tokens` count (EDGE: they may be fewer than 16)
+template <int NT, bool EDGE> __device__ __forceinline__ void values(const uint8_t *block, const uint32_t (&p)[NT][2], Sums<NT> &s, int tokens, int lane) {
+  const int g = lane >> 2, t = lane & 3;
+  // rows 2 t, 2 t + 1 (and + 8) of the K extent are tokens t, (t ^ 1) + 4 (and + 8)
   const int at[4] = {t, (t ^ 1) + 4, t + 8, (t ^ 1) + 12};
   uint2 v[4];
   uint32_t sv[4];
@@ -240,7 +216,7 @@ __device__ __forceinline__ void take_block(const uint8_t *block, const Columns<T
   for (int i = 0; i < 4; ++i) {
     v[i] = fbla::lds64(block + V_CODES + at[i] * CODE_BYTES + 8 * g);
     sv[i] = block[V_SCALES + at[i] * SCALE_BYTES + g];
-    if (EDGE && token + at[i] >= tokens) sv[i] = 0;  // (what is stored behind the last token may be anything, NaN too)
+    if (EDGE && at[i] >= tokens) sv[i] = 0;  // (what is stored behind the last token may be anything, NaN too)
   }
   const uint32_t s01 = scales_to_half2(sv[0] | sv[1] << 8), s23 = scales_to_half2(sv[2] | sv[3] << 8);
 #pragma unroll
@@ -261,6 +237,74 @@ __device__ __forceinline__ void take_block(const uint8_t *block, const Columns<T
   }
 }
 
+// a unit: two blocks of 16 tokens, the first token of which is `token`, of a request of `tokens`; EDGE: some column does not see all of them, or a block is
+// not `there` (bits 0, 1)
+template <int TYPE, int NT, bool EDGE>
+__device__ __forceinline__ void take_unit(const uint8_t (&block)[2][BLOCK_BYTES], const Columns<TYPE, NT> &Q, Sums<NT> &s, int token, int tokens, int there, int lane) {
+  const int row = token_of(lane >> 2);
+  float x[2][NT][4];
+#pragma unroll
+  for (int n = 0; n < 2; ++n) scores<TYPE, NT>(block[n], Q, x[n], lane);
+  // exponents, element e of the fragment: token row + 8 (e / 2) of the block, column 2 t + e % 2
+  float high = NOTHING;
+#pragma unroll
+  for (int n = 0; n < 2; ++n)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (EDGE && (token + 16 * n + row + 8 * (e >> 1) > Q.limit[j][e & 1] || !(there >> n & 1))) x[n][j][e] = -FBLA_INF;
+        x[n][j][e] = fmaf(x[n][j][e], Q.mult[j][e & 1], -s.m[j][e & 1]);
+      }
+      high = fbla::max3(fbla::max3(high, x[n][j][0], x[n][j][1]), x[n][j][2], x[n][j][3]);
+    }
+  if (__any_sync(FULL, high > TOP)) {
+    // m' moves for the columns that need it; from the scores again, since what was subtracted may have been NOTHING
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      scores<TYPE, NT>(block[n], Q, x[n], lane);
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (EDGE && (token + 16 * n + row + 8 * (e >> 1) > Q.limit[j][e & 1] || !(there >> n & 1))) x[n][j][e] = -FBLA_INF;
+          x[n][j][e] *= Q.mult[j][e & 1];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float top = fmaxf(fmaxf(x[0][j][i], x[0][j][2 + i]), fmaxf(x[1][j][i], x[1][j][2 + i]));
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, d));
+        if (top - s.m[j][i] > TOP) {
+          const float m = top - REST, keep = ex2(s.m[j][i] - m);
+          s.m[j][i] = m;
+          s.l[j][i] *= keep;
+#pragma unroll
+          for (int n = 0; n < 8; ++n) s.o[j][n][i] *= keep, s.o[j][n][2 + i] *= keep;
+        }
+#pragma unroll
+        for (int n = 0; n < 2; ++n) x[n][j][i] -= s.m[j][i], x[n][j][2 + i] -= s.m[j][i];
+      }
+  }
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    uint32_t p[NT][2];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[n][j][e] = ex2(x[n][j][e]);
+      s.l[j][0] += x[n][j][0] + x[n][j][2];
+      s.l[j][1] += x[n][j][1] + x[n][j][3];
+      p[j][0] = transpose8(from_floats<MLOPS_PAGED_FP16>(x[n][j][0], x[n][j][1]));
+      p[j][1] = transpose8(from_floats<MLOPS_PAGED_FP16>(x[n][j][2], x[n][j][3]));
+    }
+    values<NT, EDGE>(block[n], p, s, there >> n & 1 ? tokens - token - 16 * n : 0, lane);
+  }
+}
+
 // a finished row to the output: by the warp that has all of it
 template <int TYPE, int NT> __device__ __forceinline__ void store_row(const Call &k, const Row<NT> &w, Sums<NT> &s, int lane) {
   const int g = lane >> 2, t = lane & 3;
@@ -272,7 +316,10 @@ template <int TYPE, int NT> __device__ __forceinline__ void store_row(const Call
     for (int i = 0; i < 2; ++i) {
       const int c = 8 * j + 2 * t + i, col = w.tile * 8 * NT + c;
       if (c >= w.columns) continue;
-      const int row = w.r.start + col / k.group, head = w.head * k.group + col % k.group;
+      int query, head;
+      split_column(k, col, query, head);
+      const int row = w.r.start + query;
+      head += w.head * k.group;
       const float f = s.l[j][i] == 0.f ? 0.f : vs / s.l[j][i];
       uint4 *const dst = reinterpret_cast<uint4 *>(out_row(k, row, head) + 16 * g);
 #pragma unroll
@@ -303,25 +350,24 @@ template <int TYPE, int NT> __global__ void __launch_bounds__(THREADS<NT>, 1) st
   Smem<NT> &sm = *reinterpret_cast<Smem<NT> *>(smem_raw);
   static_assert(fits<NT>, "a run's last piece lies in the ring");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (lane < STAGES<NT>) fbla::mbar_init(&sm.full[warp][lane], 1);
+  if (lane < STAGES) fbla::mbar_init(&sm.full[warp][lane], 1);
   fbla::mbar_init_fence();
   fbla::wait_previous_pass();
   fbla::allow_next_pass();
 
   // the requests' units
-  long long total = 0;
+  int total = 0;
   for (int b0 = 0; b0 < k.a.batch; b0 += THREADS<NT>) {
-    const int b = b0 + tid;
-    const long long n = b < k.a.batch ? units_of<NT>(k, request(k, b)) : 0;
-    long long sum = n;
+    const int b = b0 + tid, n = b < k.a.batch ? all_units_of<NT>(k, request(k, b)) : 0;
+    int sum = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long x = __shfl_up_sync(FULL, sum, o);
+      const int x = __shfl_up_sync(FULL, sum, o);
       if (lane >= o) sum += x;
     }
     if (lane == 31) sm.warp_sum[warp] = sum;
     __syncthreads();
-    long long base = total;
+    int base = total;
 #pragma unroll
     for (int w = 0; w < WARPS<NT>; ++w) {
       if (w < warp) base += sm.warp_sum[w];
@@ -331,85 +377,92 @@ template <int TYPE, int NT> __global__ void __launch_bounds__(THREADS<NT>, 1) st
     __syncthreads();
   }
   if (tid == 0) sm.before[k.a.batch] = total;
-  if (lane < 2) sm.tag[2 * warp + lane] = -1;
+  if (tid < 32) sm.tag[tid] = -1;
   __syncthreads();
 
-  const Deal deal{total, (int)gridDim.x * WARPS<NT>};
-  const int me = blockIdx.x * WARPS<NT> + warp;
-  const long long lo = deal.first(me), hi = deal.first(me + 1);
-  const int count = (int)(hi - lo);
+  const int me = blockIdx.x * WARPS<NT> + warp, all = gridDim.x * WARPS<NT>;
+  const Deal deal(total, all);
+  const int lo = deal.first(me), hi = deal.first(me + 1), count = hi - lo;
   if (count > 0) {
-    // addresses of the run's blocks, 32 at a time: lane i has that of block 32 w + i of the run in window w, 0 where the table names no page
-    const int per_page = k.c.page_size / BT;
-    auto request_at = [&](long long u) {  // before[b] <= u < before[b + 1]
-      int a = 0, b = k.a.batch;
-      while (b - a > 1) {
-        const int mid = (a + b) >> 1;
-        if (sm.before[mid] <= u) a = mid; else b = mid;
-      }
-      return a;
+    // addresses of the run's blocks, 32 units at a time: lane i has those of unit 32 w + i of the run in window w, null where the table names no page or the
+    // request has no such block
+    struct Place {
+      const uint8_t *block[2];
     };
-    int lane_b = request_at(min(lo + lane, hi - 1));
-    auto address = [&](int i) -> const uint8_t * {
-      const long long u = lo + i;
-      if (u >= hi) return nullptr;
+    int lane_b = request_at(k, sm.before, min(lo + lane, hi - 1));
+    const int per_page = k.c.page_size / BT;
+    auto look_up = [&](int i) {
+      Place p{{nullptr, nullptr}};
+      const int u = lo + i;
+      if (u >= hi) return p;
       while (sm.before[lane_b + 1] <= u) ++lane_b;
       const Row<NT> w = row_at<NT>(k, sm.before, lane_b, u);
-      const int block = (int)(u - w.unit0), column = block / per_page, page = __ldg(k.a.table + (size_t)lane_b * k.a.table_stride + column);
-      if ((unsigned)page >= (unsigned)k.c.pages) return nullptr;
-      return k.c.units + (size_t)page * k.c.page_stride + (size_t)w.head * k.c.head_stride + (size_t)(block - column * per_page) * BLOCK_BYTES;
-    };
-    const uint8_t *now = address(lane), *next = address(32 + lane);
-    uint32_t now_there = __ballot_sync(FULL, now != nullptr);
-    auto issue = [&](int i, const uint8_t *from) {  // by the lane that has block i's address
-      uint64_t *const bar = &sm.full[warp][i % STAGES<NT>];
-      if (from) {
-        fbla::fence_async_smem();
-        fbla::mbar_expect_tx(bar, BLOCK_BYTES);
-        fbla::bulk_g2s(sm.ring[warp][i % STAGES<NT>], from, BLOCK_BYTES, bar);
-      } else {
-        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(fbla::smem_u32(bar)) : "memory");
+      const int number = 2 * (u - w.unit0);
+      int column = number / per_page, at = number - column * per_page;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        if ((number + n) * BT < w.r.tokens) {
+          const int page = __ldg(k.a.table + (size_t)lane_b * k.a.table_stride + column);
+          if ((unsigned)page < (unsigned)k.c.pages)
+            p.block[n] = k.c.units + (size_t)page * k.c.page_stride + (size_t)w.head * k.c.head_stride + (size_t)at * BLOCK_BYTES;
+        }
+        if (++at == per_page) at = 0, ++column;
       }
+      return p;
     };
-    if (lane < STAGES<NT> && lane < count) issue(lane, now);
+    Place now = look_up(lane), next;
+    uint32_t there[2] = {__ballot_sync(FULL, now.block[0] != nullptr), __ballot_sync(FULL, now.block[1] != nullptr)};
+    auto issue = [&](int i, const Place &from) {  // by the lane that has unit i's addresses
+      uint64_t *const bar = &sm.full[warp][i % STAGES];
+      fbla::fence_async_smem();
+      fbla::mbar_expect_tx(bar, (from.block[0] ? BLOCK_BYTES : 0) + (from.block[1] ? BLOCK_BYTES : 0));
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+        if (from.block[n]) fbla::bulk_g2s(sm.ring[warp][i % STAGES][n], from.block[n], BLOCK_BYTES, bar);
+    };
+    if (lane < STAGES && lane < count) issue(lane, now);
+    next = look_up(32 + lane);
 
-    int b = request_at(lo);
+    int b = request_at(k, sm.before, lo);
     bool first = true, alive = true;
     Columns<TYPE, NT> Q;
     Sums<NT> s;
     for (int i = 0; i < count;) {
       while (sm.before[b + 1] <= lo + i) ++b;
       const Row<NT> w = row_at<NT>(k, sm.before, b, lo + i);
-      const int end = (int)min(w.unit0 + w.blocks - lo, (long long)count);
+      const int end = min(w.unit0 + w.units - lo, count);
       Q.load(k, w, lane);
       s.clear();
-      int token = (int)(lo + i - w.unit0) * BT;
-      for (; i < end; ++i, token += BT) {
-        const int stage = i % STAGES<NT>;
-        if (alive) alive = fbla::mbar_wait_bounded(&sm.full[warp][stage], (i / STAGES<NT>) & 1);
-        alive = __all_sync(FULL, alive);
-        if (alive && (now_there >> (i & 31) & 1)) {
-          if (token + BT - 1 <= Q.low) take_block<TYPE, NT, false>(sm.ring[warp][stage], Q, s, token, w.r.tokens, lane);
-          else take_block<TYPE, NT, true>(sm.ring[warp][stage], Q, s, token, w.r.tokens, lane);
+      int token = (lo + i - w.unit0) * UNIT;
+#pragma unroll 1
+      for (; i < end; ++i, token += UNIT) {
+        const int stage = i % STAGES, here = (there[0] >> (i & 31) & 1) | (there[1] >> (i & 31) & 1) << 1;
+        if (alive) alive = fbla::mbar_wait_bounded(&sm.full[warp][stage], (i / STAGES) & 1);
+        if (__all_sync(FULL, alive)) {
+          if (token + UNIT - 1 <= Q.low && here == 3) take_unit<TYPE, NT, false>(sm.ring[warp][stage], Q, s, token, w.r.tokens, 3, lane);
+          else if (here) take_unit<TYPE, NT, true>(sm.ring[warp][stage], Q, s, token, w.r.tokens, here, lane);
+          __syncwarp();
+          const int ahead = i + STAGES;
+          if (ahead < count && lane == (ahead & 31)) issue(ahead, (ahead >> 5) == (i >> 5) ? now : next);
+        } else {
+          alive = false;
         }
-        __syncwarp();
-        const int ahead = i + STAGES<NT>;
-        if (alive && ahead < count && lane == (ahead & 31)) issue(ahead, (ahead >> 5) == (i >> 5) ? now : next);
         if ((i & 31) == 31) {
           now = next;
-          now_there = __ballot_sync(FULL, now != nullptr);
-          next = address(i + 33 + lane);
+          there[0] = __ballot_sync(FULL, now.block[0] != nullptr);
+          there[1] = __ballot_sync(FULL, now.block[1] != nullptr);
+          next = look_up(i + 33 + lane);
         }
       }
       if (!alive) {  // (a wait that gave up: the row is NaN)
 #pragma unroll
         for (int j = 0; j < NT; ++j) s.l[j][0] = s.l[j][1] = __int_as_float(0x7fc00000);
       }
-      const bool whole = w.unit0 >= lo && w.unit0 + w.blocks <= hi;
+      const bool whole = w.unit0 >= lo && w.unit0 + w.units <= hi;
       if (whole) {
         store_row<TYPE, NT>(k, w, s, lane);
       } else {
-        store_piece<NT>(first ? sm.first[warp] : *reinterpret_cast<Piece<NT> *>(sm.ring[warp][0]), s, lane);
+        store_piece<NT>(first ? sm.first[warp] : *reinterpret_cast<Piece<NT> *>(sm.ring[warp][0][0]), s, lane);
         if (lane == 0) sm.tag[2 * warp + (first ? 0 : 1)] = w.unit0;
       }
       first = false;
@@ -418,35 +471,41 @@ template <int TYPE, int NT> __global__ void __launch_bounds__(THREADS<NT>, 1) st
   __syncthreads();
 
   // rows that this CTA's warps share
-  const long long cta_lo = deal.first(blockIdx.x * WARPS<NT>), cta_hi = deal.first((blockIdx.x + 1) * WARPS<NT>);
-  auto piece = [&](int p) -> Piece<NT> & { return p & 1 ? *reinterpret_cast<Piece<NT> *>(sm.ring[p >> 1][0]) : sm.first[p >> 1]; };
-  for (int p = 0; p < 2 * WARPS<NT>;) {
-    const long long tag = sm.tag[p];
-    if (tag < 0) { ++p; continue; }
-    int list[WARPS<NT> + 1], pieces = 0;  // (a row's pieces in this CTA are one per warp)
-    for (; p < 2 * WARPS<NT> && (sm.tag[p] == tag || sm.tag[p] < 0); ++p)
-      if (sm.tag[p] == tag && pieces <= WARPS<NT>) list[pieces++] = p;
-    int b = 0;
-    for (int e = k.a.batch; e - b > 1;) {
-      const int mid = (b + e) >> 1;
-      if (sm.before[mid] <= tag) b = mid; else e = mid;
-    }
-    const Row<NT> w = row_at<NT>(k, sm.before, b, tag);
-    const bool whole = tag >= cta_lo && tag + w.blocks <= cta_hi;
+  const int cta_lo = deal.first(blockIdx.x * WARPS<NT>), cta_hi = deal.first((blockIdx.x + 1) * WARPS<NT>), my_tag = sm.tag[lane];
+  auto piece = [&](int p) -> Piece<NT> & { return p & 1 ? *reinterpret_cast<Piece<NT> *>(sm.ring[p >> 1][0][0]) : sm.first[p >> 1]; };
+  for (uint32_t left = __ballot_sync(FULL, my_tag >= 0); left;) {
+    const int tag = __shfl_sync(FULL, my_tag, __ffs(left) - 1);
+    const uint32_t pieces = __ballot_sync(FULL, my_tag == tag);  // (one of a warp)
+    left &= ~pieces;
+    const Row<NT> w = row_at<NT>(k, sm.before, request_at(k, sm.before, tag), tag);
+    const bool whole = tag >= cta_lo && tag + w.units <= cta_hi;
     float *const slot = k.stream_part + ((size_t)blockIdx.x * 2 + (tag < cta_lo ? 0 : 1)) * 8 * NT * PSTRIDE;
+    auto store = [&](int c, int x, const float4 &o, float m, float l) {
+      int query, head;
+      split_column(k, w.tile * 8 * NT + c, query, head);
+      store_joined<TYPE>(k, w.r.start + query, w.head, w.head * k.group + head, x, o, m, l);
+    };
     for (int e = tid; e < w.columns * 32; e += THREADS<NT>) {
-      const int c = e >> 5, x = e & 31, col = w.tile * 8 * NT + c;
-      float m, l;
-      const float4 o = join(pieces, [&](int i) { return (const float *)piece(list[i]).o[c]; }, x, m, l);
+      const int c = e >> 5, x = e & 31;
+      float m = NOTHING, l = 0.f;
+      for (uint32_t p = pieces; p; p &= p - 1) m = fmaxf(m, piece(__ffs(p) - 1).o[c][D]);
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (uint32_t p = pieces; p; p &= p - 1) {
+        const float *const from = piece(__ffs(p) - 1).o[c];
+        const float f = ex2(from[D] - m);
+        const float4 v = *reinterpret_cast<const float4 *>(from + 4 * x);
+        l += from[D + 1] * f;
+        o = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w));
+      }
       if (whole) {
-        store_joined<TYPE>(k, w.r.start + col / k.group, w.head, w.head * k.group + col % k.group, x, o, m, l);
+        store(c, x, o, m, l);
       } else {
         __stcg(reinterpret_cast<float4 *>(slot + c * PSTRIDE) + x, o);
         if (x == 0) __stcg(reinterpret_cast<float2 *>(slot + c * PSTRIDE + D), make_float2(m, l));
       }
     }
     if (!whole) {  // the last of the row's CTAs joins their slots
-      const int c0 = deal.warp_of(tag) / WARPS<NT>, c1 = deal.warp_of(tag + w.blocks - 1) / WARPS<NT>;
+      const int c0 = deal.warp_of(tag) / WARPS<NT>, c1 = deal.warp_of(tag + w.units - 1) / WARPS<NT>;
       __threadfence();
       __syncthreads();
       if (tid == 0) {
@@ -457,23 +516,23 @@ template <int TYPE, int NT> __global__ void __launch_bounds__(THREADS<NT>, 1) st
       if (sm.last) {
         __threadfence();
         for (int e = tid; e < w.columns * 32; e += THREADS<NT>) {
-          const int c = e >> 5, x = e & 31, col = w.tile * 8 * NT + c;
+          const int c = e >> 5, x = e & 31;
           float m, l;
           const float4 o = join(c1 - c0 + 1, [&](int i) { return k.stream_part + ((size_t)(c0 + i) * 2 + (i ? 0 : 1)) * 8 * NT * PSTRIDE + c * PSTRIDE; }, x, m, l);
-          store_joined<TYPE>(k, w.r.start + col / k.group, w.head, w.head * k.group + col % k.group, x, o, m, l);
+          store(c, x, o, m, l);
         }
       }
     }
   }
 
   // rows of requests without tokens, rows of no request
-  for (int b = me; b < k.a.batch; b += deal.warps) {
+  for (int b = me; b < k.a.batch; b += all) {
     const Request r = request(k, b);
     if (r.tokens == 0)
       for (int i = 0; i < r.n; ++i) clear_row(k, r.start + i, lane);
   }
   if (k.a.starts)
-    for (int row = max(__ldg(k.a.starts + k.a.batch), 0) + me; row < k.a.tokens; row += deal.warps) clear_row(k, row, lane);
+    for (int row = max(__ldg(k.a.starts + k.a.batch), 0) + me; row < k.a.tokens; row += all) clear_row(k, row, lane);
 }
 
 }  // namespace
@@ -482,12 +541,15 @@ template <int TYPE, int NT> cudaError_t launch_stream(const Call &k, int sms, cu
   static thread_local bool ready[64] = {false};
   const cudaError_t e = allow_shared(stream_kernel<TYPE, NT>, ready);
   if (e != cudaSuccess) return e;
-  return fbla::launch(true, 1, stream_kernel<TYPE, NT>, dim3(sms), THREADS<NT>, offsetof(Smem<NT>, before) + ((size_t)k.a.batch + 1) * sizeof(long long), stream, k);
+  return fbla::launch(true, 1, stream_kernel<TYPE, NT>, dim3(sms), THREADS<NT>, offsetof(Smem<NT>, before) + ((size_t)k.a.batch + 1) * sizeof(int), stream, k);
 }
 template cudaError_t launch_stream<MLOPS_PAGED_BF16, 1>(const Call &, int, cudaStream_t);
 template cudaError_t launch_stream<MLOPS_PAGED_FP16, 1>(const Call &, int, cudaStream_t);
 template cudaError_t launch_stream<MLOPS_PAGED_BF16, 2>(const Call &, int, cudaStream_t);
 template cudaError_t launch_stream<MLOPS_PAGED_FP16, 2>(const Call &, int, cudaStream_t);
+
+static_assert(offsetof(Smem<1>, before) + (PAGED_K_MAX_ATTENDED + 1) * sizeof(int) <= 232448 && offsetof(Smem<2>, before) + (PAGED_K_MAX_ATTENDED + 1) * sizeof(int) <= 232448,
+              "the rings and the largest batch fit");
 
 }  // namespace paged
 

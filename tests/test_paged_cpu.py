@@ -85,7 +85,7 @@ def test_attend_refusals(paged):
         return a
     for changes, words in (({"batch": -1}, "batch"), ({"batch": 16385, "tokens": 16385}, "batch"), ({"tokens": -1}, "tokens"), ({"q_heads": 0}, "q_heads"), ({"q_heads": 33}, "divides"),
                            ({"type": 2}, "type"), ({"scale": -1.0}, "scale"), ({"scale": math.nan}, "scale"), ({"scale": math.inf}, "scale"), ({"tokens": 3}, "one query per request"),
-                           ({"width": -1}, "width"), ({"table_stride": 9}, "stride"), ({"q": None}, "null"), ({"out": None}, "null"), ({"lengths": None}, "null"), ({"table": None}, "null"),
+                           ({"width": -1}, "width"), ({"table_stride": 9}, "stride"), ({"width": 1 << 27, "table_stride": 1 << 27}, "split the batch"), ({"q": None}, "null"), ({"out": None}, "null"), ({"lengths": None}, "null"), ({"table": None}, "null"),
                            ({"q": 4104}, "16-byte"), ({"out": 4100}, "16-byte"), ({"q_token_stride": 4100}, "multiples of 8"), ({"q_head_stride": 4}, "multiples of 8"),
                            ({"out_head_stride": 130}, "multiples of 8"), ({"lengths": 4098}, "4-byte"), ({"starts": 4097}, "4-byte"), ({"lse": 4098}, "4-byte")):
         refused(paged, lib.mlops_paged_attend(ctypes.byref(args(**changes)), c, 4096, 1 << 40, None), words)
