@@ -68,24 +68,6 @@ __device__ __forceinline__ void clear_row(const Call &k, int row, int lane) {
     for (int i = lane; i < k.a.q_heads; i += 32) k.a.lse[(size_t)row * k.a.q_heads + i] = -FBLA_INF;
 }
 
-// joins `count` partial rows of other CTAs, source(i) the i-th: channels 4 x .. 4 x + 3, the running maximum and sum
-template <class F> __device__ __forceinline__ float4 join(int count, F source, int x, float &m, float &l) {
-  m = NOTHING;
-#pragma unroll 8
-  for (int i = 0; i < count; ++i) m = fmaxf(m, __ldcg(source(i) + D));
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  l = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < count; ++i) {
-    const float *const p = source(i);
-    const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p + D));
-    const float f = ex2(ml.x - m);
-    const float4 v = __ldcg(reinterpret_cast<const float4 *>(p) + x);
-    l += ml.y * f;
-    o = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w));
-  }
-  return o;
-}
 template <int TYPE> __device__ __forceinline__ void store_joined(const Call &k, int row, int kv_head, int head, int x, const float4 &o, float m, float l) {
   const float f = l == 0.f ? 0.f : __ldg(k.c.v_scale + kv_head) / l;
   *reinterpret_cast<uint2 *>(out_row(k, row, head) + 4 * x) = make_uint2(from_floats<TYPE>(o.x * f, o.y * f), from_floats<TYPE>(o.z * f, o.w * f));

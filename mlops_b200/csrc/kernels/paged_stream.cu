@@ -24,8 +24,14 @@ namespace {
 template <int NT> constexpr int WARPS = NT == 1 ? 16 : 10;  // what the shared memory has room for beside the rings
 constexpr int STAGES = 2, UNIT = 2 * BT;  // tokens of a unit
 template <int NT> constexpr int THREADS = 32 * WARPS<NT>;
-constexpr int MIN_SHARE = 2;  // units of a warp, at least, where the work allows a choice
 constexpr float TOP = 15.f, REST = 9.f;  // log2 of the largest P, and of a column's largest when m' is set
+
+// a row of work
+template <int NT> struct Row {
+  Request r;
+  int b, head, tile, columns, units;
+  int unit0;  // its first unit
+};
 
 template <int NT> struct Piece {  // a warp's partial rows of one row of work
   float o[8 * NT][PSTRIDE];        // (o[128], m', l)
@@ -35,8 +41,10 @@ template <int NT> struct __align__(128) Smem {
   Piece<NT> first[WARPS<NT>];      // of a run's first row; the last row's piece takes the ring's place when that is through
   uint64_t full[WARPS<NT>][STAGES];
   int tag[32];                     // pieces in the order of the tokens, two per warp: the first unit of the piece's row, -1: none
+  Row<NT> row[32];                 // the pieces' rows
+  float2 total[8 * NT];            // (m', l) of a row that CTAs share
   int warp_sum[WARPS<NT>];
-  int last;
+  int last[2];
   int before[];                    // [batch + 1]: the requests' first units
 };
 template <int NT> constexpr bool fits = sizeof(Piece<NT>) <= STAGES * 2 * BLOCK_BYTES;
@@ -57,24 +65,16 @@ __device__ __forceinline__ uint32_t times(uint32_t a, uint32_t b) {
 // token of the block in row r < 8 of the S^T fragment: two even and two odd tokens wherever four or two lanes read at once
 __device__ __forceinline__ int token_of(int r) { return ((r >> 1) ^ (r & 1)) + 4 * (r & 1); }
 
-// How the units are dealt: warp w has units [first(w), first(w + 1)), whole + 1 of them for w < more and `whole` for the others (for few units MIN_SHARE,
-// and nothing for the warps behind).
+// How the units are dealt: warp w has units [first(w), first(w + 1)), whole + 1 of them for w < more and `whole` for the others (one for each of the first
+// warps where there are fewer units than warps).
 struct Deal {
   int total, whole, more;
   __device__ __forceinline__ Deal(int total, int warps) : total(total) {
-    const bool few = total < MIN_SHARE * warps;
-    whole = few ? MIN_SHARE : total / warps;
-    more = few ? 0 : total - whole * warps;
+    whole = total < warps ? 1 : total / warps;
+    more = total < warps ? 0 : total - whole * warps;
   }
   __device__ __forceinline__ int first(int w) const { return min(w * whole + min(w, more), total); }
   __device__ __forceinline__ int warp_of(int u) const { return u < more * (whole + 1) ? u / (whole + 1) : (u - more) / whole; }
-};
-
-// a row of work
-template <int NT> struct Row {
-  Request r;
-  int b, head, tile, columns, units;
-  int unit0;  // its first unit
 };
 
 __device__ __forceinline__ int units_of(const Request &r) { return (r.tokens + UNIT - 1) / UNIT; }  // of each of a request's rows of work
@@ -112,39 +112,44 @@ template <int TYPE, int NT> struct Columns {  // a row's queries, as B fragments
   int limit[NT][2];    // the last token that the column sees, -1: none
   int low;             // the smallest limit of the row's columns
 
-  __device__ __forceinline__ void load(const Call &k, const Row<NT> &w, int lane) {
+  // q[j] takes the column's 32 channels as they are; `convert` follows
+  __device__ __forceinline__ void fetch(const Call &k, const Row<NT> &w, int lane) {
     const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int c = 8 * j + g;
+      int query, head;
+      split_column(k, w.tile * 8 * NT + c, query, head);
+      const uint16_t *const src = static_cast<const uint16_t *>(k.a.q) + (int64_t)(w.r.start + query) * k.a.q_token_stride +
+                                  (int64_t)(w.head * k.group + head) * k.a.q_head_stride + 32 * t;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint4 raw = c < w.columns ? __ldg(reinterpret_cast<const uint4 *>(src) + e) : make_uint4(0, 0, 0, 0);
+        q[j][4 * e] = raw.x; q[j][4 * e + 1] = raw.y; q[j][4 * e + 2] = raw.z; q[j][4 * e + 3] = raw.w;
+      }
+    }
+  }
+  __device__ __forceinline__ void convert(const Call &k, const Row<NT> &w, int lane) {
+    const int t = lane & 3;
     const float base = k.sl * __ldg(k.c.k_scale + w.head);
     low = w.r.length - w.r.n + query_of(k, w.tile * 8 * NT);
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      const int c = 8 * j + g, col = w.tile * 8 * NT + c;
-      uint4 raw[4] = {};
-      if (c < w.columns) {
-        int query, head;
-        split_column(k, col, query, head);
-        const uint16_t *const src = static_cast<const uint16_t *>(k.a.q) + (int64_t)(w.r.start + query) * k.a.q_token_stride +
-                                    (int64_t)(w.head * k.group + head) * k.a.q_head_stride + 32 * t;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) raw[e] = __ldg(reinterpret_cast<const uint4 *>(src) + e);
-      }
-      float2 x[16];
       uint32_t top = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t word[4] = {raw[e].x, raw[e].y, raw[e].z, raw[e].w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[4 * e + i] = to_floats<TYPE>(word[i]);
-          top = max(top, max(__float_as_uint(x[4 * e + i].x) & 0x7fffffffu, __float_as_uint(x[4 * e + i].y) & 0x7fffffffu));
-        }
+      for (int i = 0; i < 16; ++i) {
+        const float2 x = to_floats<TYPE>(q[j][i]);
+        top = max(top, max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu));
       }
       top = max(top, __shfl_xor_sync(FULL, top, 1));
       top = max(top, __shfl_xor_sync(FULL, top, 2));
       float down;
       const float up = q_factor(top, down);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) q[j][i] = from_floats<MLOPS_PAGED_FP16>(x[i].x * up, x[i].y * up);
+      for (int i = 0; i < 16; ++i) {
+        const float2 x = to_floats<TYPE>(q[j][i]);
+        q[j][i] = from_floats<MLOPS_PAGED_FP16>(x.x * up, x.y * up);
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         mult[j][i] = fmaxf(base * __shfl_sync(FULL, down, (2 * t + i) * 4), 1e-37f);  // (not 0: masked scores are -infinity)
@@ -158,15 +163,18 @@ template <int TYPE, int NT> struct Columns {  // a row's queries, as B fragments
 // running sums of a row: O^T, m' and l of the lane's columns (l of its own tokens until `fold`)
 template <int NT> struct Sums {
   float o[NT][8][4], m[NT][2], l[NT][2];
-  __device__ __forceinline__ void clear() {
+  __device__ __forceinline__ void clear(const int (&limit)[NT][2]) {
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[j][i][e] = 0.f;
-      m[j][0] = m[j][1] = NOTHING;
-      l[j][0] = l[j][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        m[j][i] = limit[j][i] < 0 ? 0.f : NOTHING;  // (a column that sees nothing never waits for its first score)
+        l[j][i] = 0.f;
+      }
     }
   }
   __device__ __forceinline__ void fold() {
@@ -245,32 +253,24 @@ __device__ __forceinline__ void take_unit(const uint8_t (&block)[2][BLOCK_BYTES]
   float x[2][NT][4];
 #pragma unroll
   for (int n = 0; n < 2; ++n) scores<TYPE, NT>(block[n], Q, x[n], lane);
-  // exponents, element e of the fragment: token row + 8 (e / 2) of the block, column 2 t + e % 2
+  // exponents, element e of the fragment: token row + 8 (e / 2) of the block, column 2 t + e % 2. A column that has no m' yet takes 0 for it.
   float high = NOTHING;
+  bool open = false;
 #pragma unroll
-  for (int n = 0; n < 2; ++n)
+  for (int j = 0; j < NT; ++j) {
+    const float m[2] = {s.m[j][0] == NOTHING ? 0.f : s.m[j][0], s.m[j][1] == NOTHING ? 0.f : s.m[j][1]};
+    open |= s.m[j][0] == NOTHING || s.m[j][1] == NOTHING;
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
+    for (int n = 0; n < 2; ++n) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         if (EDGE && (token + 16 * n + row + 8 * (e >> 1) > Q.limit[j][e & 1] || !(there >> n & 1))) x[n][j][e] = -FBLA_INF;
-        x[n][j][e] = fmaf(x[n][j][e], Q.mult[j][e & 1], -s.m[j][e & 1]);
+        x[n][j][e] = fmaf(x[n][j][e], Q.mult[j][e & 1], -m[e & 1]);
       }
       high = fbla::max3(fbla::max3(high, x[n][j][0], x[n][j][1]), x[n][j][2], x[n][j][3]);
     }
-  if (__any_sync(FULL, high > TOP)) {
-    // m' moves for the columns that need it; from the scores again, since what was subtracted may have been NOTHING
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      scores<TYPE, NT>(block[n], Q, x[n], lane);
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (EDGE && (token + 16 * n + row + 8 * (e >> 1) > Q.limit[j][e & 1] || !(there >> n & 1))) x[n][j][e] = -FBLA_INF;
-          x[n][j][e] *= Q.mult[j][e & 1];
-        }
-    }
+  }
+  if (__any_sync(FULL, open || high > TOP)) {  // m' moves for the columns that need it
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -278,15 +278,16 @@ __device__ __forceinline__ void take_unit(const uint8_t (&block)[2][BLOCK_BYTES]
         float top = fmaxf(fmaxf(x[0][j][i], x[0][j][2 + i]), fmaxf(x[1][j][i], x[1][j][2 + i]));
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, d));
-        if (top - s.m[j][i] > TOP) {
-          const float m = top - REST, keep = ex2(s.m[j][i] - m);
-          s.m[j][i] = m;
+        const bool none = s.m[j][i] == NOTHING;
+        if (top > (none ? -FBLA_INF : TOP)) {
+          const float shift = top - REST, keep = none ? 0.f : ex2(-shift);
+          s.m[j][i] = none ? shift : s.m[j][i] + shift;
           s.l[j][i] *= keep;
 #pragma unroll
           for (int n = 0; n < 8; ++n) s.o[j][n][i] *= keep, s.o[j][n][2 + i] *= keep;
-        }
 #pragma unroll
-        for (int n = 0; n < 2; ++n) x[n][j][i] -= s.m[j][i], x[n][j][2 + i] -= s.m[j][i];
+          for (int n = 0; n < 2; ++n) x[n][j][i] -= shift, x[n][j][2 + i] -= shift;
+        }
       }
   }
 #pragma unroll
@@ -341,7 +342,7 @@ template <int NT> __device__ __forceinline__ void store_piece(Piece<NT> &p, Sums
       for (int h = 0; h < 4; ++h)
         *reinterpret_cast<float4 *>(dst + 16 * g + 4 * h) = make_float4(s.o[j][4 * (h & 1)][2 * (h >> 1) + i], s.o[j][4 * (h & 1) + 1][2 * (h >> 1) + i],
                                                                         s.o[j][4 * (h & 1) + 2][2 * (h >> 1) + i], s.o[j][4 * (h & 1) + 3][2 * (h >> 1) + i]);
-      if (g == 0) dst[D] = s.m[j][i], dst[D + 1] = s.l[j][i];
+      if (g == 0) dst[D] = s.l[j][i] == 0.f ? NOTHING : s.m[j][i], dst[D + 1] = s.l[j][i];
     }
 }
 
@@ -389,7 +390,10 @@ template <int TYPE, int NT> __global__ void __launch_bounds__(THREADS<NT>, 1) st
     struct Place {
       const uint8_t *block[2];
     };
-    int lane_b = request_at(k, sm.before, min(lo + lane, hi - 1));
+    int b = request_at(k, sm.before, lo), lane_b = b;
+    Row<NT> w = row_at<NT>(k, sm.before, b, lo);
+    Columns<TYPE, NT> Q;
+    Q.fetch(k, w, lane);
     const int per_page = k.c.page_size / BT;
     auto look_up = [&](int i) {
       Place p{{nullptr, nullptr}};
@@ -421,18 +425,19 @@ template <int TYPE, int NT> __global__ void __launch_bounds__(THREADS<NT>, 1) st
         if (from.block[n]) fbla::bulk_g2s(sm.ring[warp][i % STAGES][n], from.block[n], BLOCK_BYTES, bar);
     };
     if (lane < STAGES && lane < count) issue(lane, now);
-    next = look_up(32 + lane);
 
-    int b = request_at(k, sm.before, lo);
     bool first = true, alive = true;
-    Columns<TYPE, NT> Q;
     Sums<NT> s;
     for (int i = 0; i < count;) {
-      while (sm.before[b + 1] <= lo + i) ++b;
-      const Row<NT> w = row_at<NT>(k, sm.before, b, lo + i);
+      if (i) {
+        while (sm.before[b + 1] <= lo + i) ++b;
+        w = row_at<NT>(k, sm.before, b, lo + i);
+        Q.fetch(k, w, lane);
+      }
       const int end = min(w.unit0 + w.units - lo, count);
-      Q.load(k, w, lane);
-      s.clear();
+      Q.convert(k, w, lane);
+      if (i == 0 && count > 32) next = look_up(32 + lane);
+      s.clear(Q.limit);
       int token = (lo + i - w.unit0) * UNIT;
 #pragma unroll 1
       for (; i < end; ++i, token += UNIT) {
@@ -463,65 +468,133 @@ template <int TYPE, int NT> __global__ void __launch_bounds__(THREADS<NT>, 1) st
         store_row<TYPE, NT>(k, w, s, lane);
       } else {
         store_piece<NT>(first ? sm.first[warp] : *reinterpret_cast<Piece<NT> *>(sm.ring[warp][0][0]), s, lane);
-        if (lane == 0) sm.tag[2 * warp + (first ? 0 : 1)] = w.unit0;
+        if (lane == 0) {
+          sm.tag[2 * warp + (first ? 0 : 1)] = w.unit0;
+          sm.row[2 * warp + (first ? 0 : 1)] = w;
+        }
       }
       first = false;
     }
   }
   __syncthreads();
 
-  // rows that this CTA's warps share
+  // Rows that several of the CTA's warps share, or that go on in other CTAs, a warp per row and column. A row's pieces are its first one, p, and the first
+  // pieces of the warps behind p's; lane i has the weight of piece i.
   const int cta_lo = deal.first(blockIdx.x * WARPS<NT>), cta_hi = deal.first((blockIdx.x + 1) * WARPS<NT>), my_tag = sm.tag[lane];
-  auto piece = [&](int p) -> Piece<NT> & { return p & 1 ? *reinterpret_cast<Piece<NT> *>(sm.ring[p >> 1][0][0]) : sm.first[p >> 1]; };
-  for (uint32_t left = __ballot_sync(FULL, my_tag >= 0); left;) {
-    const int tag = __shfl_sync(FULL, my_tag, __ffs(left) - 1);
-    const uint32_t pieces = __ballot_sync(FULL, my_tag == tag);  // (one of a warp)
-    left &= ~pieces;
-    const Row<NT> w = row_at<NT>(k, sm.before, request_at(k, sm.before, tag), tag);
-    const bool whole = tag >= cta_lo && tag + w.units <= cta_hi;
-    float *const slot = k.stream_part + ((size_t)blockIdx.x * 2 + (tag < cta_lo ? 0 : 1)) * 8 * NT * PSTRIDE;
-    auto store = [&](int c, int x, const float4 &o, float m, float l) {
-      int query, head;
-      split_column(k, w.tile * 8 * NT + c, query, head);
-      store_joined<TYPE>(k, w.r.start + query, w.head, w.head * k.group + head, x, o, m, l);
-    };
-    for (int e = tid; e < w.columns * 32; e += THREADS<NT>) {
-      const int c = e >> 5, x = e & 31;
-      float m = NOTHING, l = 0.f;
-      for (uint32_t p = pieces; p; p &= p - 1) m = fmaxf(m, piece(__ffs(p) - 1).o[c][D]);
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (uint32_t p = pieces; p; p &= p - 1) {
-        const float *const from = piece(__ffs(p) - 1).o[c];
-        const float f = ex2(from[D] - m);
-        const float4 v = *reinterpret_cast<const float4 *>(from + 4 * x);
-        l += from[D + 1] * f;
-        o = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w));
-      }
-      if (whole) {
-        store(c, x, o, m, l);
-      } else {
-        __stcg(reinterpret_cast<float4 *>(slot + c * PSTRIDE) + x, o);
-        if (x == 0) __stcg(reinterpret_cast<float2 *>(slot + c * PSTRIDE + D), make_float2(m, l));
-      }
+  const uint32_t same = __match_any_sync(FULL, my_tag);  // pieces of the row of piece `lane`
+  const uint32_t leaders = __ballot_sync(FULL, my_tag >= 0 && __ffs(same) - 1 == lane);
+  auto piece = [&](int p, int i) -> const Piece<NT> & { return i == 0 && (p & 1) ? *reinterpret_cast<const Piece<NT> *>(sm.ring[p >> 1][0][0]) : sm.first[(p >> 1) + i]; };
+  auto is_cut = [&](const Row<NT> &w) { return w.unit0 < cta_lo || w.unit0 + w.units > cta_hi; };
+  auto store = [&](const Row<NT> &w, int c, const float4 &o, float m, float l) {  // column c, a lane's four channels
+    int query, head;
+    split_column(k, w.tile * 8 * NT + c, query, head);
+    store_joined<TYPE>(k, w.r.start + query, w.head, w.head * k.group + head, lane, o, m, l);
+  };
+  for (int f = warp; f < __popc(leaders) * 8 * NT; f += WARPS<NT>) {
+    const int nth = f / (8 * NT), c = f % (8 * NT);
+    const int p = __ffs(__ballot_sync(FULL, (leaders >> lane & 1) && __popc(leaders & ((1u << lane) - 1)) == nth)) - 1;
+    const int pieces = __popc(__shfl_sync(FULL, same, p));
+    const Row<NT> &w = sm.row[p];
+    if (c >= w.columns) continue;
+    const float2 y = lane < pieces ? *reinterpret_cast<const float2 *>(piece(p, lane).o[c] + D) : make_float2(NOTHING, 0.f);
+    float m = y.x;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, d));
+    const float weight = ex2(y.x - m), l = fbla::warp_sum(y.y * weight);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int i = 0; i < pieces; ++i) {
+      const float f = __shfl_sync(FULL, weight, i);
+      const float4 v = *reinterpret_cast<const float4 *>(piece(p, i).o[c] + 4 * lane);
+      o = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w));
     }
-    if (!whole) {  // the last of the row's CTAs joins their slots
-      const int c0 = deal.warp_of(tag) / WARPS<NT>, c1 = deal.warp_of(tag + w.units - 1) / WARPS<NT>;
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) {
-        sm.last = atomicAdd(k.stream_counters + c0, 1) == c1 - c0;
-        if (sm.last) k.stream_counters[c0] = 0;
-      }
-      __syncthreads();
-      if (sm.last) {
-        __threadfence();
-        for (int e = tid; e < w.columns * 32; e += THREADS<NT>) {
-          const int c = e >> 5, x = e & 31;
-          float m, l;
-          const float4 o = join(c1 - c0 + 1, [&](int i) { return k.stream_part + ((size_t)(c0 + i) * 2 + (i ? 0 : 1)) * 8 * NT * PSTRIDE + c * PSTRIDE; }, x, m, l);
-          store(c, x, o, m, l);
+    if (is_cut(w)) {
+      float *const slot = k.stream_part + (((size_t)blockIdx.x * 2 + (w.unit0 < cta_lo ? 0 : 1)) * 8 * NT + c) * PSTRIDE;
+      __stcg(reinterpret_cast<float4 *>(slot) + lane, o);
+      if (lane == 0) __stcg(reinterpret_cast<float2 *>(slot + D), make_float2(m, l));
+    } else {
+      store(w, c, o, m, l);
+    }
+  }
+  // rows that go on in other CTAs, this one's first and last at most: the CTA that comes last joins their slots
+  const int ends[2] = {__ffs(leaders) - 1, 31 - __clz(leaders)};
+  if (leaders && (is_cut(sm.row[ends[0]]) || is_cut(sm.row[ends[1]]))) {
+    __threadfence();
+    __syncthreads();
+    if (tid < 2) {
+      const Row<NT> &w = sm.row[ends[tid]];
+      sm.last[tid] = -1;
+      if (is_cut(w) && !(tid && ends[0] == ends[1])) {
+        const int c0 = deal.warp_of(w.unit0) / WARPS<NT>, c1 = deal.warp_of(w.unit0 + w.units - 1) / WARPS<NT>;
+        if (atomicAdd(k.stream_counters + c0, 1) == c1 - c0) {
+          k.stream_counters[c0] = 0;
+          sm.last[tid] = c0;
         }
       }
+    }
+    __syncthreads();
+    for (int side = 0; side < 2; ++side) {
+      const int c0 = sm.last[side];
+      if (c0 < 0) continue;
+      __threadfence();
+      const Row<NT> &w = sm.row[ends[side]];
+      const int slots = deal.warp_of(w.unit0 + w.units - 1) / WARPS<NT> - c0 + 1;
+      // a warp per column and slice of the slots, every slices-th one; everything it reads is on its way before the first value is used. The slices' sums
+      // meet in shared memory.
+      const int slices = max(WARPS<NT> / w.columns, 1);
+      float4(*const sums)[32] = reinterpret_cast<float4(*)[32]>(sm.ring);  // [column * slices + slice][lane]
+      float *const weights = reinterpret_cast<float *>(sm.first[warp].o);  // of the slots
+      for (int f = warp; f < w.columns * slices; f += WARPS<NT>) {
+        const int c = f / slices, slice = f - c * slices;
+        const float *const slot0 = k.stream_part + ((size_t)c0 * 2 * 8 * NT + c) * PSTRIDE;
+        auto slot = [&](int i) { return slot0 + (i ? i * 2 : 1) * (8 * NT * PSTRIDE); };
+        float2 y[4];
+        float4 v[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = 32 * i + lane < slots ? __ldcg(reinterpret_cast<const float2 *>(slot(32 * i + lane) + D)) : make_float2(NOTHING, 0.f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = slice + i * slices < slots ? __ldcg(reinterpret_cast<const float4 *>(slot(slice + i * slices)) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+        float m = fmaxf(fmaxf(y[0].x, y[1].x), fmaxf(y[2].x, y[3].x)), l = 0.f;
+        for (int i = 128 + lane; i < slots; i += 32) m = fmaxf(m, __ldcg(slot(i) + D));
+#pragma unroll
+        for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, d));
+        __syncwarp();
+        for (int i = lane; i < slots; i += 32) {
+          const float2 z = i < 32 ? y[0] : i < 64 ? y[1] : i < 96 ? y[2] : i < 128 ? y[3] : __ldcg(reinterpret_cast<const float2 *>(slot(i) + D));
+          weights[i] = ex2(z.x - m);
+          l += z.y * weights[i];
+        }
+        __syncwarp();
+        l = fbla::warp_sum(l);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i0 = slice;;) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float g = i0 + i * slices < slots ? weights[i0 + i * slices] : 0.f;
+            o = make_float4(fmaf(v[i].x, g, o.x), fmaf(v[i].y, g, o.y), fmaf(v[i].z, g, o.z), fmaf(v[i].w, g, o.w));
+          }
+          i0 += 8 * slices;
+          if (i0 >= slots) break;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = i0 + i * slices < slots ? __ldcg(reinterpret_cast<const float4 *>(slot(i0 + i * slices)) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        if (slices == 1) {
+          store(w, c, o, m, l);
+        } else {
+          sums[f][lane] = o;
+          if (lane == 0 && slice == 0) sm.total[c] = make_float2(m, l);
+        }
+      }
+      __syncthreads();
+      if (slices > 1 && warp < w.columns) {
+        float4 o = sums[warp * slices][lane];
+        for (int i = 1; i < slices; ++i) {
+          const float4 v = sums[warp * slices + i][lane];
+          o = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
+        }
+        store(w, warp, o, sm.total[warp].x, sm.total[warp].y);
+      }
+      __syncthreads();
     }
   }
 
