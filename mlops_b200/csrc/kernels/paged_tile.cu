@@ -275,46 +275,57 @@ __device__ __forceinline__ void produce(Smem &sm, int warp, int lane) {
 }
 
 // ---- products -------------------------------------------------------------------------------------------------------------------
+// The way from P to the next scores is what a tile takes: nothing else is waited for or released on it. A stage is free when both X have read it; where a tile
+// is one X's alone, that one arrives for the other.
 __device__ __forceinline__ void issue(const Call &k, Smem &sm, long long hi, int x) {  // by one thread
   const uint32_t s_at = sm.tmem + 128 * x, o_at = sm.tmem + 256 + 128 * x;
-  uint32_t at = 0, mine = 0, items = 0;
+  uint32_t row_at = 0, mine = 0, items = 0;  // tiles of the run before the row, of this X; rows of work
   bool ok = true;
   Row w = sm.begin;
   do {
-    const Part part{w.halves(k), tiles_of_half(k, w, x)};
-    ok = ok && wait(sm, &sm.q_ready[x], items++ & 1);
-    bool first = true;
-    for (int n = w.n0; n < w.n1 && ok; ++n, ++at) {
-      const int stage = at % STAGES;
-      const uint32_t parity = at / STAGES & 1;
-      ok = wait(sm, &sm.k_full[stage], parity);
-      if (!part.has(n, x)) {
-        if (mine) ok = ok && wait(sm, &sm.o_done[x], (mine - 1) & 1);  // (not ahead of its own softmax, which reads `there`)
-        tc::mbar_arrive(&sm.k_empty[stage]);
-        ok = ok && wait(sm, &sm.v_full[stage], parity);
-        tc::mbar_arrive(&sm.v_empty[stage]);
-        continue;
-      }
-      if (mine) ok = ok && wait(sm, &sm.o_done[x], (mine - 1) & 1);  // (P is in S's place)
-      if (!ok) break;
+    const bool shared = w.halves(k);
+    const int step = shared ? 2 : 1, end = shared ? w.n1 : min(w.n1, tiles_of_half(k, w, x)), both = shared ? 0 : tiles_of_half(k, w, 0);  // tiles below `both` are both X's
+    const uint8_t *const q = sm.q[shared ? 0 : x];
+    int n = w.n0 + (shared && (w.n0 & 1) != x);
+    auto at = [&](int n) { return row_at + (n - w.n0); };
+    auto scores = [&]() {
+      const int stage = at(n) % STAGES;
       tc::tc_fence_after();
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const uint32_t offset = (i >> 2) * SLAB + (i & 3) * 32;
-        tc::mma_f16(s_at, tc::smem_desc_at(sm.q[part.shared ? 0 : x], offset), tc::smem_desc_at(sm.k[stage], offset), IDESC_S, i > 0);
+        tc::mma_f16(s_at, tc::smem_desc_at(q, offset), tc::smem_desc_at(sm.k[stage], offset), IDESC_S, i > 0);
       }
       tc::mma_commit(&sm.s_ready[x]);
       tc::mma_commit(&sm.k_empty[stage]);
-      ok = wait(sm, &sm.p_ready[x], mine & 1) && wait(sm, &sm.v_full[stage], parity);
+      if (n >= both) tc::mbar_arrive(&sm.k_empty[stage]);
+    };
+    ok = ok && wait(sm, &sm.q_ready[x], items++ & 1);
+    if (n < end) {
+      ok = ok && wait(sm, &sm.k_full[at(n) % STAGES], at(n) / STAGES & 1);
+      if (ok) scores();
+    }
+    for (bool first = true; n < end && ok; first = false) {
+      const int stage = at(n) % STAGES, alone = n >= both;
+      ok = wait(sm, &sm.v_full[stage], at(n) / STAGES & 1) && wait(sm, &sm.p_ready[x], mine & 1);
       if (!ok) break;
       tc::tc_fence_after();
 #pragma unroll
       for (int i = 0; i < 8; ++i) tc::mma_f16_ts(o_at, s_at + 64 * (i >> 2) + 8 * (i & 3), v_desc(sm.v[stage], i * 2048), IDESC_O, !first || i > 0);
       tc::mma_commit(&sm.o_done[x]);
-      tc::mma_commit(&sm.v_empty[stage]);
-      first = false;
+      n += step;
+      if (n < end) {
+        // (P is in S's place: its product has to be through before the next scores)
+        ok = wait(sm, &sm.k_full[at(n) % STAGES], at(n) / STAGES & 1) && wait(sm, &sm.o_done[x], mine & 1);
+        if (ok) scores();
+        tc::mbar_arrive(&sm.v_empty[stage]);
+      } else {
+        tc::mma_commit(&sm.v_empty[stage]);
+      }
+      if (alone) tc::mbar_arrive(&sm.v_empty[stage]);
       ++mine;
     }
+    row_at += w.n1 - w.n0;
   } while (next_row(k, sm.before, hi, w));
 }
 
