@@ -30,6 +30,7 @@ constexpr int ROWS = 128, TOKENS = 128;     // of a product
 constexpr int SLAB = 128 * 128, TILE = 2 * SLAB;  // bytes of a slab (128 rows of 64 channels) and of an operand
 constexpr int STAGES = 2, PRODUCER0 = 8, PRODUCERS = 8, ISSUER0 = 16, FINDER = 18, THREADS = 20 * 32;  // (four warps share a register count: 19 idles)
 constexpr int HEAD = 4;  // units of a row of work beside its tiles: what loading Q, the first tile and storing O cost (26 000 cycles beside 5 300 per tile)
+constexpr int WINDOW = 16;  // tiles whose blocks are looked up at a time
 constexpr int NO_TILE = -0x7fffffff;
 constexpr float TOP = 15.f, REST = 9.f;
 constexpr long long WAIT_CYCLES = 2000000000;
@@ -48,9 +49,9 @@ struct Row {
 struct __align__(1024) Smem {
   uint8_t q[2][TILE];
   uint8_t k[STAGES][TILE], v[STAGES][TILE];
-  const uint8_t *block[64][8];  // [tile of the run % 64][block]: where it lies; null: the table names no page, or the request has no such block
-  int left[64];                 // tokens of the request from the tile's first on
-  uint64_t places_full[2], places_empty[2];  // of 32 tiles each
+  const uint8_t *block[2 * WINDOW][8];  // [tile of the run % (2 WINDOW)][block]: where it lies; null: the table names no page, or the request has no such block
+  int left[2 * WINDOW];         // tokens of the request from the tile's first on
+  uint64_t places_full[2], places_empty[2];  // of WINDOW tiles each
   uint64_t q_ready[2], k_full[STAGES], v_full[STAGES], k_empty[STAGES], v_empty[STAGES], s_ready[2], p_ready[2], o_done[2];
   uint8_t there[4][8];  // [tile of tokens % 4][block]: 1 where the table names a page
   float down[2][ROWS];      // the rows' factors
@@ -191,34 +192,35 @@ __device__ __forceinline__ void store_operand(uint8_t *tile, const Raw &x, int r
   }
 }
 
-// Where the run's blocks lie, a lane per tile, 32 tiles ahead of the producers, NO_TILE behind the last one: by one warp.
+// Where the run's blocks lie, two lanes per tile, up to 32 tiles ahead of the producers, NO_TILE behind the last one: by one warp.
 __device__ __forceinline__ void look_up(const Call &k, Smem &sm, long long hi, int lane) {
-  const int per_page = k.c.page_size / BT;
+  const int per_page = k.c.page_size / BT, half = lane & 1;
   Row w = sm.begin;
   int reached = 0, n = w.n0;  // the tile that this lane looked up last, in the run and in its row of work
   bool ok = true, more = true;
   for (int i = 0; ok && __all_sync(FULL, more); ++i) {
     if (i >= 2) ok = wait(sm, &sm.places_empty[i & 1], (i / 2 & 1) ^ 1);
-    const int tile = 32 * i + lane;
+    const int tile = WINDOW * i + (lane >> 1);
     n += tile - reached;
     reached = tile;
     while (more && n >= w.n1) {
       n -= w.n1;
       more = next_row(k, sm.before, hi, w);
     }
-    sm.left[tile & 63] = more ? w.r.tokens - TOKENS * n : NO_TILE;
+    if (half == 0) sm.left[tile % (2 * WINDOW)] = more ? w.r.tokens - TOKENS * n : NO_TILE;
     if (more) {
       const int *const entries = k.a.table + (size_t)w.b * k.a.table_stride;
       const uint8_t *const head = k.c.units + (size_t)w.head * k.c.head_stride;
-      int column = 8 * n / per_page, at = 8 * n - column * per_page;
+      const int number = 8 * n + 4 * half;
+      int column = number / per_page, at = number - column * per_page;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < 4; ++j) {
         const uint8_t *block = nullptr;
-        if ((8 * n + j) * BT < w.r.tokens) {
+        if ((number + j) * BT < w.r.tokens) {
           const int page = __ldg(entries + column);
           if ((unsigned)page < (unsigned)k.c.pages) block = head + (size_t)page * k.c.page_stride + (size_t)at * BLOCK_BYTES;
         }
-        sm.block[tile & 63][j] = block;
+        sm.block[tile % (2 * WINDOW)][4 * half + j] = block;
         if (++at == per_page) at = 0, ++column;
       }
     }
@@ -227,15 +229,26 @@ __device__ __forceinline__ void look_up(const Call &k, Smem &sm, long long hi, i
   }
 }
 
-// Producer warp `warp` turns block `warp` of every tile into rows 16 warp .. of the operands; a tile's codes are loaded while the one before it is converted.
+// Producer warp `warp` turns block `warp` of every tile into rows 16 warp .. of the operands, K of a tile before V of the tile before it, which is wanted
+// later; a tensor's codes are loaded while its last tile's are waited for and used.
 __device__ __forceinline__ void produce(Smem &sm, int warp, int lane) {
-  Raw rk, rv;
-  const uint8_t *block;
-  int left;
-  bool ok = wait(sm, &sm.places_full[0], 0);
+  struct Place {
+    const uint8_t *block;
+    int left;  // the request's tokens from the block's first on; NO_TILE: behind the run
+  };
+  bool ok = true;
   auto place = [&](int tile) {
-    left = ok ? sm.left[tile & 63] : NO_TILE;
-    block = left == NO_TILE ? nullptr : sm.block[tile & 63][warp];
+    if (tile % WINDOW == 0) {
+      const int i = tile / WINDOW;
+      if (i && lane == 0) tc::mbar_arrive(&sm.places_empty[(i & 1) ^ 1]);
+      ok = ok && wait(sm, &sm.places_full[i & 1], i >> 1 & 1);
+    }
+    Place p{nullptr, ok ? sm.left[tile % (2 * WINDOW)] : NO_TILE};
+    if (p.left != NO_TILE) {
+      p.block = sm.block[tile % (2 * WINDOW)][warp];
+      p.left -= BT * warp;
+    }
+    return p;
   };
   auto store = [&](uint8_t *tile, const Raw &x, uint64_t *full) {
     store_operand(tile, x, 16 * warp, lane);
@@ -243,34 +256,39 @@ __device__ __forceinline__ void produce(Smem &sm, int warp, int lane) {
     __syncwarp();
     if (lane == 0) tc::mbar_arrive(full);
   };
-  place(0);
-  load_raw(rk, block, 0, K_SCALES, lane);
-  load_raw(rv, block, V_CODES, V_SCALES, lane);
-#pragma unroll 1
-  for (int at = 0; left != NO_TILE && ok; ++at) {
-    const int stage = at % STAGES, tokens = left - BT * warp;
-    const uint32_t parity = (at / STAGES & 1) ^ 1;
-    const bool there = block != nullptr;
-    if ((at & 31) == 31) {  // the next tile is the first one of a window
-      const int i = (at + 1) >> 5;
-      if (lane == 0) tc::mbar_arrive(&sm.places_empty[(i & 1) ^ 1]);
-      ok = wait(sm, &sm.places_full[i & 1], i >> 1 & 1);
-    }
-    place(at + 1);
-    if (at >= STAGES) ok = ok && wait(sm, &sm.k_empty[stage], parity);
-    if (lane == 0) sm.there[at & 3][warp] = there;
+  auto store_k = [&](int tile, const Raw &x, bool there) {
+    const int stage = tile % STAGES;
+    if (tile >= STAGES) ok = ok && wait(sm, &sm.k_empty[stage], (tile / STAGES & 1) ^ 1);
     ok = __all_sync(FULL, ok);
-    store(sm.k[stage], rk, &sm.k_full[stage]);
-    load_raw(rk, block, 0, K_SCALES, lane);
-    if (tokens < BT) {  // (what is stored behind the last token may be anything, NaN too)
+    if (lane == 0) sm.there[tile & 3][warp] = there;
+    store(sm.k[stage], x, &sm.k_full[stage]);
+  };
+  Raw rk, rv;
+  Place now = place(0), next;
+  load_raw(rk, now.block, 0, K_SCALES, lane);
+  load_raw(rv, now.block, V_CODES, V_SCALES, lane);
+  store_k(0, rk, now.block != nullptr);
+  next = place(1);
+  load_raw(rk, next.block, 0, K_SCALES, lane);
+#pragma unroll 1
+  for (int at = 0; now.left != NO_TILE && ok; ++at) {
+    Place behind = next;
+    if (next.left != NO_TILE) {
+      behind = place(at + 2);
+      store_k(at + 1, rk, next.block != nullptr);
+      load_raw(rk, behind.block, 0, K_SCALES, lane);
+    }
+    if (now.left < BT) {  // (what is stored behind the last token may be anything, NaN too)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        if (8 * i + (lane & 7) >= tokens) rv.scales[i] = 0;
+        if (8 * i + (lane & 7) >= now.left) rv.scales[i] = 0;
     }
-    if (at >= STAGES && ok) ok = wait(sm, &sm.v_empty[stage], parity);
+    if (at >= STAGES) ok = ok && wait(sm, &sm.v_empty[at % STAGES], (at / STAGES & 1) ^ 1);
     ok = __all_sync(FULL, ok);
-    store(sm.v[stage], rv, &sm.v_full[stage]);
-    load_raw(rv, block, V_CODES, V_SCALES, lane);
+    store(sm.v[at % STAGES], rv, &sm.v_full[at % STAGES]);
+    load_raw(rv, next.block, V_CODES, V_SCALES, lane);
+    now = next;
+    next = behind;
   }
 }
 
