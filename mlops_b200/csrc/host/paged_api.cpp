@@ -95,6 +95,7 @@ mlops_fbla_status mlops_paged_append(const mlops_paged_cache *c, int tokens, int
   const char *const fn = "mlops_paged_append";
   if (const char *why = cache_fault(c)) return refuse(fn, "%s", why);
   if (tokens < 0 || !known_type(type)) return refuse(fn, "needs tokens >= 0 and a type of MLOPS_PAGED_BF16 or MLOPS_PAGED_FP16");
+  if ((int64_t)tokens * c->kv_heads > INT32_MAX) return refuse(fn, "tokens * kv_heads has to be below 2^31: split the tokens");
   if (tokens == 0) return nothing_to_do();
   if (!k || !v || !slots) return refuse(fn, "a required pointer is null");
   if (!rows_usable(k, k_ts, k_hs) || !rows_usable(v, v_ts, v_hs) || !aligned(slots, 4))
@@ -106,6 +107,7 @@ mlops_fbla_status mlops_paged_read(const mlops_paged_cache *c, int tokens, int t
   const char *const fn = "mlops_paged_read";
   if (const char *why = cache_fault(c)) return refuse(fn, "%s", why);
   if (tokens < 0 || !known_type(type)) return refuse(fn, "needs tokens >= 0 and a type of MLOPS_PAGED_BF16 or MLOPS_PAGED_FP16");
+  if ((int64_t)tokens * c->kv_heads > INT32_MAX) return refuse(fn, "tokens * kv_heads has to be below 2^31: split the tokens");
   if (tokens == 0) return nothing_to_do();
   if (!k || !v || !slots) return refuse(fn, "a required pointer is null");
   if (!aligned(k, 16) || !aligned(v, 16) || !aligned(slots, 4)) return refuse(fn, "k and v have to start on 16-byte boundaries");

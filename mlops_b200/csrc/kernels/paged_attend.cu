@@ -40,7 +40,7 @@ extern "C" cudaError_t paged_k_attend_launch(const mlops_paged_attend_args *a, c
   k.c = *c;
   k.sl = a->scale * 1.4426950408889634f;
   k.group = a->q_heads / c->kv_heads;
-  k.group_inverse = k.group == 1 ? 0u : (uint32_t)(((1ull << 32) + k.group - 1) / k.group);
+  k.by_group = paged::Divisor(k.group);
   k.wide = paged::WIDE;
   k.stream_counters = reinterpret_cast<int *>(base + s.stream_counters);
   k.tile_counters = reinterpret_cast<int *>(base + s.tile_counters);

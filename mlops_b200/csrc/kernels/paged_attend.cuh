@@ -15,18 +15,14 @@ struct Call {
   mlops_paged_cache c;
   float sl;        // softmax scale times log2(e)
   int group;       // query heads per KV head
-  uint32_t group_inverse;  // 2^32 / group, rounded up (0 for 1)
+  Divisor by_group;
   int wide;        // requests with more than so many columns (queries times group) are the tile kernel's
   float *stream_part, *tile_part;          // partial rows, see the kernels
   int *stream_counters, *tile_counters;    // one per CTA, zeros before and after every call
 };
 
 // a column's query and its query head among the KV head's: column / group, column % group
-__device__ __forceinline__ int query_of(const Call &k, int column) {
-  if (k.group == 1) return column;
-  const int q = (int)__umulhi((uint32_t)column, k.group_inverse);  // at most one too many
-  return q - (q * k.group > column);
-}
+__device__ __forceinline__ int query_of(const Call &k, int column) { return k.by_group.divide(column); }
 __device__ __forceinline__ void split_column(const Call &k, int column, int &query, int &head) {
   query = query_of(k, column);
   head = column - query * k.group;

@@ -15,11 +15,19 @@ constexpr int CODE_BYTES = D / 2, SCALE_BYTES = D / 16;  // a token's, of one te
 constexpr int V_CODES = BT * CODE_BYTES, K_SCALES = 2 * V_CODES, V_SCALES = K_SCALES + BT * SCALE_BYTES;
 static_assert(V_SCALES + BT * SCALE_BYTES == BLOCK_BYTES, "the block's four arrays fill it");
 
-// the block that holds slot `slot` of head `head`
-__device__ __forceinline__ uint8_t *block_of(const mlops_paged_cache &c, int slot, int head) {
-  const int page = slot / c.page_size, at = slot - page * c.page_size;
-  return c.units + (size_t)page * c.page_stride + (size_t)head * c.head_stride + (size_t)(at / BT) * BLOCK_BYTES;
-}
+// x / d for 0 <= x < 2^31 from inverse = 2^32 / d, rounded up (0 for d = 1): the product's high word is at most one too large
+struct Divisor {
+  int d;
+  uint32_t inverse;
+  __host__ explicit Divisor(int d) : d(d), inverse(d == 1 ? 0u : (uint32_t)(((1ull << 32) + d - 1) / d)) {}
+  Divisor() = default;
+  __device__ __forceinline__ int divide(int x) const {
+    if (d == 1) return x;
+    const int q = (int)__umulhi((uint32_t)x, inverse);
+    return q - ((int64_t)q * d > x);
+  }
+};
+
 __device__ __forceinline__ bool is_slot(const mlops_paged_cache &c, int slot) { return (unsigned)slot < (unsigned)(c.pages * c.page_size); }
 
 // eight codes of a word as four pairs of FP16 (exact): pair i is channels 2 i, 2 i + 1

@@ -48,12 +48,12 @@ def test_a_pool_that_cannot_be_used(paged, changes, words):
 def test_append_and_read_refusals(paged):
     lib, c = paged._lib, pool(paged)
     good = [1, 0, 4096, 1024, 128, 4096, 1024, 128, 4096]
-    for at, value, words in ((0, -1, "tokens"), (1, 2, "type"), (1, -1, "type"), (2, None, "null"), (5, None, "null"), (8, None, "null"), (2, 4104, "16-byte"), (3, 1028, "multiples of 8"),
+    for at, value, words in ((0, -1, "tokens"), (0, 1 << 28, "split the tokens"), (1, 2, "type"), (1, -1, "type"), (2, None, "null"), (5, None, "null"), (8, None, "null"), (2, 4104, "16-byte"), (3, 1028, "multiples of 8"),
                              (4, 129, "multiples of 8"), (5, 4098, "16-byte"), (6, 4, "multiples of 8"), (7, 4, "multiples of 8")):
         call = list(good)
         call[at] = value
         refused(paged, lib.mlops_paged_append(c, *call, None), words)
-    for at, value, words in ((0, -1, "tokens"), (1, 7, "type"), (2, None, "null"), (3, None, "null"), (4, None, "null"), (3, 4104, "16-byte"), (4, 4100, "16-byte")):
+    for at, value, words in ((0, -1, "tokens"), (0, 1 << 28, "split the tokens"), (1, 7, "type"), (2, None, "null"), (3, None, "null"), (4, None, "null"), (3, 4104, "16-byte"), (4, 4100, "16-byte")):
         call = [1, 0, 4096, 4096, 4096]
         call[at] = value
         refused(paged, lib.mlops_paged_read(c, *call, None), words)
