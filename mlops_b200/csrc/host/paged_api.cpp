@@ -100,7 +100,9 @@ mlops_fbla_status mlops_paged_append(const mlops_paged_cache *c, int tokens, int
   if (!k || !v || !slots) return refuse(fn, "a required pointer is null");
   if (!rows_usable(k, k_ts, k_hs) || !rows_usable(v, v_ts, v_hs) || !aligned(slots, 4))
     return refuse(fn, "k and v have to start on 16-byte boundaries and have strides that are multiples of 8 elements");
-  return ended(fn, paged_k_append_launch(c, tokens, type, k, k_ts, k_hs, v, v_ts, v_hs, slots, stream));
+  int sms = 0;
+  const cudaError_t e = processors(&sms);
+  return ended(fn, e != cudaSuccess ? e : paged_k_append_launch(c, tokens, type, k, k_ts, k_hs, v, v_ts, v_hs, slots, sms, stream));
 }
 
 mlops_fbla_status mlops_paged_read(const mlops_paged_cache *c, int tokens, int type, const int *slots, void *k, void *v, cudaStream_t stream) {
@@ -111,7 +113,9 @@ mlops_fbla_status mlops_paged_read(const mlops_paged_cache *c, int tokens, int t
   if (tokens == 0) return nothing_to_do();
   if (!k || !v || !slots) return refuse(fn, "a required pointer is null");
   if (!aligned(k, 16) || !aligned(v, 16) || !aligned(slots, 4)) return refuse(fn, "k and v have to start on 16-byte boundaries");
-  return ended(fn, paged_k_read_launch(c, tokens, type, slots, k, v, stream));
+  int sms = 0;
+  const cudaError_t e = processors(&sms);
+  return ended(fn, e != cudaSuccess ? e : paged_k_read_launch(c, tokens, type, slots, k, v, sms, stream));
 }
 
 size_t mlops_paged_attend_scratch_bytes(const mlops_paged_attend_args *a, int kv_heads) {
