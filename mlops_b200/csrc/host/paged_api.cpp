@@ -133,7 +133,7 @@ mlops_fbla_status mlops_paged_attend(const mlops_paged_attend_args *a, const mlo
   if (!a->starts && a->tokens != a->batch) return refuse(fn, "without starts there is one query per request, but there are %d for %d", a->tokens, a->batch);
   if (a->tokens == 0) return nothing_to_do();
   if (a->width < 0 || a->table_stride < a->width) return refuse(fn, "the table's stride has to be at least its width, and that not negative");
-  if (a->width > 0 && (int64_t)a->batch * c->kv_heads > INT32_MAX / (2 * (((int64_t)a->width * c->page_size + 31) / 32)))
+  if (a->width > 0 && (int64_t)a->batch * c->kv_heads > INT32_MAX / (4 * (((int64_t)a->width * c->page_size + 31) / 32)))
     return refuse(fn, "batch * kv_heads * width * page_size is more than a call takes: split the batch");
   if (!a->q || !a->out || !scratch || (a->batch > 0 && !a->lengths) || (a->batch > 0 && a->width > 0 && !a->table)) return refuse(fn, "a required pointer is null");
   if (!rows_usable(a->q, a->q_token_stride, a->q_head_stride) || !rows_usable(a->out, a->out_token_stride, a->out_head_stride) || !aligned(scratch, 16))

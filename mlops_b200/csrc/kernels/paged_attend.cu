@@ -4,7 +4,7 @@
 namespace paged {
 namespace {
 
-constexpr int WIDE = 16;  // columns that a row of the stream kernel has at most
+constexpr int WIDE = 32;  // columns of a request that is streamed, at most
 
 struct Scratch {  // offsets: the counters of both kernels (zeros at first), their partial rows
   size_t stream_counters, tile_counters, stream_part, tile_part, bytes;
@@ -14,7 +14,7 @@ Scratch scratch_of(int sms, bool tiles) {
   const size_t counters = ((size_t)sms * sizeof(int) + 255) / 256 * 256;
   s.tile_counters = counters;
   s.stream_part = 2 * counters;
-  s.tile_part = s.stream_part + (size_t)sms * 2 * WIDE * PSTRIDE * sizeof(float);
+  s.tile_part = s.stream_part + (size_t)sms * 2 * 16 * PSTRIDE * sizeof(float);
   s.bytes = s.tile_part + (tiles ? (size_t)sms * 2 * 256 * PSTRIDE * sizeof(float) : 0);
   return s;
 }

@@ -21,8 +21,11 @@
 namespace paged {
 namespace {
 
-template <int NT> constexpr int WARPS = NT == 1 ? 16 : 10;  // what the shared memory has room for beside the rings
-constexpr int STAGES = 2, UNIT = 2 * BT;  // tokens of a unit
+// One tile of columns: sixteen warps of 128 registers. Two: eight of 255; with twelve of 168 the registers do not hold a block's words (106 us for drafted tokens of 16
+// requests, against 102).
+template <int NT> constexpr int WARPS = NT == 1 ? 16 : 8;
+template <int NT> constexpr int STAGES = NT == 1 ? 2 : 3;
+constexpr int UNIT = 2 * BT;  // tokens of a unit
 template <int NT> constexpr int THREADS = 32 * WARPS<NT>;
 constexpr float TOP = 15.f, REST = 9.f;  // log2 of the largest P, and of a column's largest when m' is set
 
@@ -37,9 +40,9 @@ template <int NT> struct Piece {  // a warp's partial rows of one row of work
   float o[8 * NT][PSTRIDE];        // (o[128], m', l)
 };
 template <int NT> struct __align__(128) Smem {
-  uint8_t ring[WARPS<NT>][STAGES][2][BLOCK_BYTES];
+  uint8_t ring[WARPS<NT>][STAGES<NT>][2][BLOCK_BYTES];
   Piece<NT> first[WARPS<NT>];      // of a run's first row; the last row's piece takes the ring's place when that is through
-  uint64_t full[WARPS<NT>][STAGES];
+  uint64_t full[WARPS<NT>][STAGES<NT>];
   int tag[32];                     // pieces in the order of the tokens, two per warp: the first unit of the piece's row, -1: none
   Row<NT> row[32];                 // the pieces' rows
   float2 total[8 * NT];            // (m', l) of a row that CTAs share
@@ -47,7 +50,7 @@ template <int NT> struct __align__(128) Smem {
   int last[2];
   int before[];                    // [batch + 1]: the requests' first units
 };
-template <int NT> constexpr bool fits = sizeof(Piece<NT>) <= STAGES * 2 * BLOCK_BYTES;
+template <int NT> constexpr bool fits = sizeof(Piece<NT>) <= STAGES<NT> * 2 * BLOCK_BYTES;
 
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -351,7 +354,7 @@ template <int TYPE, int NT> __global__ void __launch_bounds__(THREADS<NT>, 1) st
   Smem<NT> &sm = *reinterpret_cast<Smem<NT> *>(smem_raw);
   static_assert(fits<NT>, "a run's last piece lies in the ring");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (lane < STAGES) fbla::mbar_init(&sm.full[warp][lane], 1);
+  if (lane < STAGES<NT>) fbla::mbar_init(&sm.full[warp][lane], 1);
   fbla::mbar_init_fence();
   fbla::wait_previous_pass();
   fbla::allow_next_pass();
@@ -417,14 +420,14 @@ template <int TYPE, int NT> __global__ void __launch_bounds__(THREADS<NT>, 1) st
     Place now = look_up(lane), next;
     uint32_t there[2] = {__ballot_sync(FULL, now.block[0] != nullptr), __ballot_sync(FULL, now.block[1] != nullptr)};
     auto issue = [&](int i, const Place &from) {  // by the lane that has unit i's addresses
-      uint64_t *const bar = &sm.full[warp][i % STAGES];
+      uint64_t *const bar = &sm.full[warp][i % STAGES<NT>];
       fbla::fence_async_smem();
       fbla::mbar_expect_tx(bar, (from.block[0] ? BLOCK_BYTES : 0) + (from.block[1] ? BLOCK_BYTES : 0));
 #pragma unroll
       for (int n = 0; n < 2; ++n)
-        if (from.block[n]) fbla::bulk_g2s(sm.ring[warp][i % STAGES][n], from.block[n], BLOCK_BYTES, bar);
+        if (from.block[n]) fbla::bulk_g2s(sm.ring[warp][i % STAGES<NT>][n], from.block[n], BLOCK_BYTES, bar);
     };
-    if (lane < STAGES && lane < count) issue(lane, now);
+    if (lane < STAGES<NT> && lane < count) issue(lane, now);
 
     bool first = true, alive = true;
     Sums<NT> s;
@@ -441,13 +444,13 @@ template <int TYPE, int NT> __global__ void __launch_bounds__(THREADS<NT>, 1) st
       int token = (lo + i - w.unit0) * UNIT;
 #pragma unroll 1
       for (; i < end; ++i, token += UNIT) {
-        const int stage = i % STAGES, here = (there[0] >> (i & 31) & 1) | (there[1] >> (i & 31) & 1) << 1;
-        if (alive) alive = fbla::mbar_wait_bounded(&sm.full[warp][stage], (i / STAGES) & 1);
+        const int stage = i % STAGES<NT>, here = (there[0] >> (i & 31) & 1) | (there[1] >> (i & 31) & 1) << 1;
+        if (alive) alive = fbla::mbar_wait_bounded(&sm.full[warp][stage], (i / STAGES<NT>) & 1);
         if (__all_sync(FULL, alive)) {
           if (token + UNIT - 1 <= Q.low && here == 3) take_unit<TYPE, NT, false>(sm.ring[warp][stage], Q, s, token, w.r.tokens, 3, lane);
           else if (here) take_unit<TYPE, NT, true>(sm.ring[warp][stage], Q, s, token, w.r.tokens, here, lane);
           __syncwarp();
-          const int ahead = i + STAGES;
+          const int ahead = i + STAGES<NT>;
           if (ahead < count && lane == (ahead & 31)) issue(ahead, (ahead >> 5) == (i >> 5) ? now : next);
         } else {
           alive = false;
