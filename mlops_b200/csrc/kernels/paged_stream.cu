@@ -15,6 +15,11 @@
 //
 // Rows that several warps share are joined in shared memory, those that several CTAs share by the CTA that comes last (a counter per CTA), always in the
 // order of the tokens: the result does not depend on who that is.
+//
+// Bound by instructions beside the bytes: some 290 per block and tile of columns, of which a conversion and a scaling of every pair of codes are 128. Measured, 32 / 8 heads:
+// 64 requests of 1K-64K tokens 193 us = 4.7 TB/s (its loop alone 5.7, 0.87 of the copy rate; without the products and conversions 165 us); 131 072 tokens 41.6 us,
+// of which 28 are the loop, 6.5 what comes before (lengths, table, queries: five dependent reads) and 8 the joining; 4096 tokens 11 us on the device. Units of one block
+// instead of two: 227 us, 384 instructions per block. Twelve warps instead of sixteen: the same.
 #include "fbla_launch.h"
 #include "paged_attend.cuh"
 

@@ -11,8 +11,12 @@
 // memory. m' moves only where a score would pass 2^15, then O and l are rescaled; l sums the unrounded P. Rows of at most 128 use both halves too: the
 // even tiles of tokens go to X = 0, the odd ones to X = 1, with the same queries, and the halves are joined at the end.
 //
-// The exponentials of a tile take as long as its two products. Eight warps do those of X = 0 and then those of X = 1, so that the tensor cores work for one X while
-// the other one's softmax runs.
+// The exponentials of a tile take as long as its two products: 16 per cycle and SM, 2048 cycles for both X. Eight warps do those of X = 0 and then those of X = 1, so that
+// the tensor cores work for one X while the other one's softmax runs. A tile then takes the softmax of one X (1800 cycles, of which the exponentials are 1024) and the way
+// of the other from P to its next scores (2500: two products of 512 among the other X's, three hand-overs through barriers): 4300 cycles where the products alone are
+// 2048. Two prompts of 8192 tokens, 32 / 8 heads: 1.38 ms = 799 TFLOP/s, 0.49 of the measured burst rate. Tried: a thread per row and both X's softmax at once
+// (7600 cycles: both wait for the tensor cores together); a third of the exponentials as polynomials on the FMA units (1.07 times the time: packed FP32, maxima and
+// conversions share their issue slots); operand warps that look up their blocks themselves (the registers spill, and every load is waited for at once).
 //
 // Warps 0-7 (two threads per row): softmax. Warps 8-15: operands, from packed pages to two stages each of K and V in shared
 // memory, token rows of 128 bytes (64 channels) with 16-byte chunk c of row r at c ^ (r % 8): for S that is K-major, for O V's MN-major. Warps 16, 17: one thread
@@ -29,7 +33,8 @@ namespace tc = fbla::tc;
 constexpr int ROWS = 128, TOKENS = 128;     // of a product
 constexpr int SLAB = 128 * 128, TILE = 2 * SLAB;  // bytes of a slab (128 rows of 64 channels) and of an operand
 constexpr int STAGES = 2, PRODUCER0 = 8, PRODUCERS = 8, ISSUER0 = 16, FINDER = 18, THREADS = 20 * 32;  // (four warps share a register count: 19 idles)
-constexpr int HEAD = 4;  // units of a row of work beside its tiles: what loading Q, the first tile and storing O cost (26 000 cycles beside 5 300 per tile)
+constexpr int HEAD = 4;  // units of a row of work beside its tiles: what loading Q, the first tile and storing O cost (17 000 cycles beside 4 300 per
+                         // tile; us for two prompts of 8192 with 0, 2, 4, 6, 8: 2006, 1833, 1732, 1757, 1754 when they were 26 000 and 5 300)
 constexpr int WINDOW = 16;  // tiles whose blocks are looked up at a time
 constexpr int NO_TILE = -0x7fffffff;
 constexpr float TOP = 15.f, REST = 9.f;

@@ -365,3 +365,90 @@ def test_a_step_from_pages_to_attention(paged):
                     assert bool(((out[first + i, x].double() - p @ vals).abs() <= bound).all())
             first += m
     assert cursor.tolist()[2] == 0
+
+
+@pytest.mark.parametrize("heads, group, counts", [(2, 4, [8, 9, 1, 2]), (1, 8, [4, 5, 1]), (1, 16, [2, 3]), (1, 32, [1, 2]), (1, 40, [1, 1]), (4, 1, [31, 32, 33, 8]), (1, 33, [1])])
+def test_on_both_sides_of_the_kernels_limits(paged, heads, group, counts):
+    """8, 16, 32 columns and one more; groups that are streamed with and without `starts`"""
+    lengths = [1200 + 77 * i for i in range(len(counts))]
+    gen, table, cache = paged_case(paged, sum(counts) + group, lengths, heads, 32)
+    q = torch.randn((sum(counts), heads * group, 128), generator=gen, device="cuda").to(torch.bfloat16)
+    check_attend(paged, q, cache, table, lengths, counts, starts_of(counts), "bf16")
+    if max(counts) == 1:
+        check_attend(paged, q, cache, table, lengths, counts, None, "bf16")
+
+
+def test_long_runs_of_tiles(paged):
+    """some seventy tiles of tokens per CTA, rows of work of one tile to fifty"""
+    lengths, counts = [6144], [6144]
+    gen, table, cache = paged_case(paged, 21, lengths, 2, 64)
+    q = torch.randn((6144, 16, 128), generator=gen, device="cuda").to(torch.bfloat16)
+    check_attend(paged, q, cache, table, lengths, counts, starts_of(counts), "bf16")
+
+
+def test_calls_of_all_shapes_one_after_the_other(paged):
+    """sixty calls on one stream without a wait between them, from one query to whole prompts: each leaves the scratch as the next one needs it"""
+    rng, shapes = random.Random(5), []
+    for i in range(12):
+        batch = rng.randint(1, 9)
+        counts = [rng.choice([1, 1, 2, 7, 40, 300]) for _ in range(batch)] if i % 3 else [1] * batch
+        shapes.append(([n + rng.randint(0, 4000) for n in counts], counts, rng.choice([1, 2, 8]), rng.choice([1, 4, 6])))
+    calls = []
+    for seed, (lengths, counts, heads, group) in enumerate(shapes):
+        gen, table, cache = paged_case(paged, 100 + seed, lengths, heads, 64)
+        q = torch.randn((sum(counts), heads * group, 128), generator=gen, device="cuda").to(torch.bfloat16)
+        calls.append((q, cache, table, ints(lengths), None if max(counts) == 1 else starts_of(counts)))
+    torch.cuda.synchronize()
+    results = [paged.attend(*c, return_lse=True) for _ in range(5) for c in calls]
+    for i, (out, lse) in enumerate(results[12:]):
+        assert torch.equal(out, results[i % 12][0]) and torch.equal(lse, results[i % 12][1])
+    for (q, cache, table, lengths, _), (_, counts, _, _), (out, lse) in zip(calls, shapes, results):
+        want, weight, want_lse = pu.attend(q, cache.units, cache.k_scale, cache.v_scale, table, lengths.tolist(), counts)
+        assert bool(((out.double() - want).abs() <= 2.0 ** -10 * weight + 2.0 ** -8 * want.abs() + 1e-7).all())
+        assert bool(((lse.double() - want_lse).abs() <= 2.0 ** -12 * (1 + want_lse.abs() / 8)).all())
+
+
+def test_a_captured_step_follows_lengths_and_tables(paged):
+    """append and attention captured once, replayed for a growing request: the tables, lengths and slots of the moment count; two streams at once"""
+    heads, group, P, width = 2, 4, 16, 40
+    gen = generator(31)
+    table = torch.randperm(width, generator=gen, device="cuda").to(torch.int32).view(1, width)
+    caches = [paged.empty(width, heads, P) for _ in range(2)]
+    k, v, q = (torch.zeros((1, n, 128), dtype=torch.bfloat16, device="cuda") for n in (heads, heads, heads * group))
+    slots, lengths = ints([0]), ints([1])
+    streams, graphs, outs = [torch.cuda.Stream() for _ in range(2)], [], []
+    for stream, cache in zip(streams, caches):
+        with torch.cuda.stream(stream):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                paged.append(cache, k, v, slots)
+                outs.append(paged.attend(q, cache, table, lengths))
+            graphs.append(graph)
+    torch.cuda.synchronize()
+    for step in range(70):
+        for x in (k, v, q):
+            x.copy_(torch.randn(x.shape, generator=gen, device="cuda"))
+        slots.copy_(table[0, step // P] * P + step % P)
+        lengths.fill_(step + 1)
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], outs[1]) and torch.equal(caches[0].units, caches[1].units)
+        if step % 23 == 0 or step == 69:
+            want, weight, _ = pu.attend(q, caches[0].units, caches[0].k_scale, caches[0].v_scale, table, [step + 1], [1])
+            assert bool(((outs[0].double() - want).abs() <= 2.0 ** -10 * weight + 2.0 ** -8 * want.abs() + 1e-7).all())
+
+
+def test_the_serving_example(paged):
+    """examples/paged_serving.py: lengths and finite outputs, the same again for the same numbers"""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "paged_serving.py")
+    spec = importlib.util.spec_from_file_location("paged_serving", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    lengths, out, _ = example.serve(requests=3, steps=70, prompt=200)
+    assert lengths == [1 + 200 * (i + 1) // 3 + 70 for i in range(3)] and bool(torch.isfinite(out).all())
+    assert torch.equal(out, example.serve(requests=3, steps=70, prompt=200)[1])
