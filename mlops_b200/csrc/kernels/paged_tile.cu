@@ -669,19 +669,31 @@ template <int TYPE> __device__ __forceinline__ void join_row(const Call &k, Smem
     if (k.a.lse) k.a.lse[(size_t)(w.r.start + query) * k.a.q_heads + w.head * k.group + head] = lse_of(m, l);
   }
   __syncthreads();
-#pragma unroll 4
-  for (int e = tid; e < rows * 32; e += THREADS) {
-    const int c = e >> 5, x = e & 31;
-    int query, head;
-    split_column(k, 2 * ROWS * w.pair + c, query, head);
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
+  constexpr int AHEAD = 8;  // float4 of a thread that are on their way at once
+  for (int e0 = tid; e0 < rows * 32; e0 += AHEAD * THREADS) {
+    float4 o[AHEAD] = {};
     for (int i = 0; i < pieces; ++i) {
-      const float f = weights[c * pieces + i];
-      const float4 y = __ldcg(reinterpret_cast<const float4 *>(piece(i) + c * PSTRIDE) + x);
-      o = make_float4(fmaf(y.x, f, o.x), fmaf(y.y, f, o.y), fmaf(y.z, f, o.z), fmaf(y.w, f, o.w));
+      const float *const from = piece(i);
+      float4 y[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const int e = min(e0 + j * THREADS, rows * 32 - 1);
+        y[j] = __ldcg(reinterpret_cast<const float4 *>(from + (e >> 5) * PSTRIDE) + (e & 31));
+      }
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const float f = weights[(min(e0 + j * THREADS, rows * 32 - 1) >> 5) * pieces + i];
+        o[j] = make_float4(fmaf(y[j].x, f, o[j].x), fmaf(y[j].y, f, o[j].y), fmaf(y[j].z, f, o[j].z), fmaf(y[j].w, f, o[j].w));
+      }
     }
-    reinterpret_cast<uint2 *>(out_row(k, w.r.start + query, w.head * k.group + head))[x] = make_uint2(from_floats<TYPE>(o.x, o.y), from_floats<TYPE>(o.z, o.w));
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int e = e0 + j * THREADS;
+      if (e >= rows * 32) break;
+      int query, head;
+      split_column(k, 2 * ROWS * w.pair + (e >> 5), query, head);
+      reinterpret_cast<uint2 *>(out_row(k, w.r.start + query, w.head * k.group + head))[e & 31] = make_uint2(from_floats<TYPE>(o[j].x, o[j].y), from_floats<TYPE>(o[j].z, o[j].w));
+    }
   }
   __syncthreads();
 }
