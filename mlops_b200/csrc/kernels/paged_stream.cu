@@ -195,31 +195,41 @@ template <int NT> struct Sums {
   }
 };
 
-// S^T of a block, in score units of the product
-template <int TYPE, int NT> __device__ __forceinline__ void scores(const uint8_t *block, const Columns<TYPE, NT> &Q, float (&acc)[NT][4], int lane) {
+// S^T of the unit's blocks, in score units of the product
+template <int TYPE, int NT> __device__ __forceinline__ void scores(const uint8_t (&block)[2][BLOCK_BYTES], const Columns<TYPE, NT> &Q, float (&acc)[2][NT][4], int lane) {
   const int t = lane & 3, row = token_of(lane >> 2);
+  uint32_t w[2][2][4], s[2][2];  // [block][token row, row + 8]
 #pragma unroll
-  for (int j = 0; j < NT; ++j)
+  for (int n = 0; n < 2; ++n) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
-  const uint4 ka = fbla::lds128(block + row * CODE_BYTES + 16 * t), kb = fbla::lds128(block + (row + 8) * CODE_BYTES + 16 * t);
-  const uint32_t sa = scales_to_half2(*reinterpret_cast<const uint16_t *>(block + K_SCALES + row * SCALE_BYTES + 2 * t));
-  const uint32_t sb = scales_to_half2(*reinterpret_cast<const uint16_t *>(block + K_SCALES + (row + 8) * SCALE_BYTES + 2 * t));
-  const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t ha[4], hb[4];
-    codes_to_half2(wa[i], ha);
-    codes_to_half2(wb[i], hb);
-    const uint32_t xa = __byte_perm(sa, 0, i < 2 ? 0x1010 : 0x3232), xb = __byte_perm(sb, 0, i < 2 ? 0x1010 : 0x3232);
+      for (int e = 0; e < 4; ++e) acc[n][j][e] = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) ha[e] = times(ha[e], xa), hb[e] = times(hb[e], xb);
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      mma(acc[j], ha[0], hb[0], ha[1], hb[1], Q.q[j][4 * i], Q.q[j][4 * i + 1]);
-      mma(acc[j], ha[2], hb[2], ha[3], hb[3], Q.q[j][4 * i + 2], Q.q[j][4 * i + 3]);
+    for (int r = 0; r < 2; ++r) {
+      const uint4 x = fbla::lds128(block[n] + (row + 8 * r) * CODE_BYTES + 16 * t);
+      w[n][r][0] = x.x; w[n][r][1] = x.y; w[n][r][2] = x.z; w[n][r][3] = x.w;
+      s[n][r] = scales_to_half2(*reinterpret_cast<const uint16_t *>(block[n] + K_SCALES + (row + 8 * r) * SCALE_BYTES + 2 * t));
     }
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      uint32_t h[2][4];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        codes_to_half2(w[n][r][i], h[r]);
+        const uint32_t x = __byte_perm(s[n][r], 0, i < 2 ? 0x1010 : 0x3232);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) h[r][e] = times(h[r][e], x);
+      }
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        mma(acc[n][j], h[0][0], h[1][0], h[0][1], h[1][1], Q.q[j][4 * i], Q.q[j][4 * i + 1]);
+        mma(acc[n][j], h[0][2], h[1][2], h[0][3], h[1][3], Q.q[j][4 * i + 2], Q.q[j][4 * i + 3]);
+      }
+    }
 }
 // O^T += V^T P^T of a block; of its tokens only the first `tokens` count (EDGE: they may be fewer than 16)
 template <int NT, bool EDGE> __device__ __forceinline__ void values(const uint8_t *block, const uint32_t (&p)[NT][2], Sums<NT> &s, int tokens, int lane) {
@@ -259,8 +269,7 @@ template <int TYPE, int NT, bool EDGE>
 __device__ __forceinline__ void take_unit(const uint8_t (&block)[2][BLOCK_BYTES], const Columns<TYPE, NT> &Q, Sums<NT> &s, int token, int tokens, int there, int lane) {
   const int row = token_of(lane >> 2);
   float x[2][NT][4];
-#pragma unroll
-  for (int n = 0; n < 2; ++n) scores<TYPE, NT>(block[n], Q, x[n], lane);
+  scores<TYPE, NT>(block, Q, x, lane);
   // exponents, element e of the fragment: token row + 8 (e / 2) of the block, column 2 t + e % 2. A column that has no m' yet takes 0 for it.
   float high = NOTHING;
   bool open = false;
