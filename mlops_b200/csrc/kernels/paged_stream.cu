@@ -17,7 +17,7 @@
 // order of the tokens: the result does not depend on who that is.
 //
 // Bound by instructions beside the bytes: some 290 per block and tile of columns, of which a conversion and a scaling of every pair of codes are 128. Measured, 32 / 8 heads:
-// 64 requests of 1K-64K tokens 193 us = 4.7 TB/s (its loop alone 5.7, 0.87 of the copy rate; without the products and conversions 165 us); 131 072 tokens 41.6 us,
+// 64 requests of 1K-64K tokens 200 us = 4.6 TB/s (its loop alone 5.7, 0.87 of the copy rate; without the products and conversions 165 us); 131 072 tokens 42.7 us,
 // of which 28 are the loop, 6.5 what comes before (lengths, table, queries: five dependent reads) and 8 the joining; 4096 tokens 11 us on the device. Units of one block
 // instead of two: 227 us, 384 instructions per block. Twelve warps instead of sixteen: the same.
 #include "fbla_launch.h"
@@ -27,7 +27,7 @@ namespace paged {
 namespace {
 
 // One tile of columns: sixteen warps of 128 registers. Two: eight of 255; with twelve of 168 the registers do not hold a block's words (106 us for drafted tokens of 16
-// requests, against 102).
+// requests, against 102). Three do not pay: requests of 24 columns 123 us instead of 145, but of 16 columns 108 instead of 95 and of 32 168 instead of 146.
 template <int NT> constexpr int WARPS = NT == 1 ? 16 : 8;
 template <int NT> constexpr int STAGES = NT == 1 ? 2 : 3;
 constexpr int UNIT = 2 * BT;  // tokens of a unit

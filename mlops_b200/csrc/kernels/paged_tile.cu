@@ -14,7 +14,7 @@
 // The exponentials of a tile take as long as its two products: 16 per cycle and SM, 2048 cycles for both X. Eight warps do those of X = 0 and then those of X = 1, so that
 // the tensor cores work for one X while the other one's softmax runs. A tile then takes the softmax of one X (1800 cycles, of which the exponentials are 1024) and the way
 // of the other from P to its next scores (2500: two products of 512 among the other X's, three hand-overs through barriers): 4300 cycles where the products alone are
-// 2048. Two prompts of 8192 tokens, 32 / 8 heads: 1.38 ms = 799 TFLOP/s, 0.49 of the measured burst rate. Tried: a thread per row and both X's softmax at once
+// 2048. Two prompts of 8192 tokens, 32 / 8 heads: 1.39 ms = 793 TFLOP/s, 0.49 of the measured burst rate. Tried: a thread per row and both X's softmax at once
 // (7600 cycles: both wait for the tensor cores together); a third of the exponentials as polynomials on the FMA units (1.07 times the time: packed FP32, maxima and
 // conversions share their issue slots); operand warps that look up their blocks themselves (the registers spill, and every load is waited for at once).
 //

@@ -378,6 +378,15 @@ def test_on_both_sides_of_the_kernels_limits(paged, heads, group, counts):
         check_attend(paged, q, cache, table, lengths, counts, None, "bf16")
 
 
+@pytest.mark.parametrize("heads, group, counts", [(2, 4, [1] * 20 + [8, 9, 3]), (3, 8, [1, 1, 1, 0]), (2, 2, [4, 4]), (2, 2, [4, 5]), (1, 1, [1, 0, 30, 2, 7, 0, 1])])
+def test_on_both_sides_of_the_average(paged, heads, group, counts):
+    """up to 8 columns per request on average and more, with single requests of more than that"""
+    lengths = [900 + 131 * i for i in range(len(counts))]
+    gen, table, cache = paged_case(paged, sum(counts) + group, lengths, heads, 16)
+    q = torch.randn((sum(counts), heads * group, 128), generator=gen, device="cuda").to(torch.float16)
+    check_attend(paged, q, cache, table, lengths, counts, starts_of(counts), "fp16")
+
+
 def test_long_runs_of_tiles(paged):
     """some seventy tiles of tokens per CTA, rows of work of one tile to fifty"""
     lengths, counts = [6144], [6144]
