@@ -234,7 +234,7 @@ def attend(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, lengths: tor
     ``q [tokens, q_heads, 128]`` BF16 or FP16, ``table`` int32 [batch, width], ``lengths`` int32 [batch]: tokens that each request has in the pool, the
     queries' own among them. ``starts`` int32 [batch + 1]: the rows of request b are ``starts[b] .. starts[b + 1] - 1``, its newest tokens; None: one
     query per request. Row i of n sees the request's tokens up to ``lengths[b] - n + i``. Returns ``[tokens, q_heads, 128]`` of q's type, zeros for a
-    row that sees nothing and for rows of no request; with ``return_lse`` also the natural log-sum-exp of the rows' scaled scores, float32
+    row that sees nothing and for rows of no request, before ``starts[0]`` and behind ``starts[batch]``; with ``return_lse`` also the natural log-sum-exp of the rows' scaled scores, float32
     [tokens, q_heads] (-inf for such rows). ``scale`` 0 selects 1/sqrt(128)."""
     pool, kv_heads, index = _pool(cache)
     if not _on(index):

@@ -621,8 +621,10 @@ template <int TYPE, int NT> __global__ void __launch_bounds__(THREADS<NT>, 1) st
     if (r.tokens == 0)
       for (int i = 0; i < r.n; ++i) clear_row(k, r.start + i, lane);
   }
-  if (k.a.starts)
-    for (int row = max(__ldg(k.a.starts + k.a.batch), 0) + me; row < k.a.tokens; row += all) clear_row(k, row, lane);
+  if (k.a.starts) {
+    const int first = min(max(__ldg(k.a.starts), 0), k.a.tokens), end = min(max(__ldg(k.a.starts + k.a.batch), first), k.a.tokens);
+    for (int i = me; i < first + k.a.tokens - end; i += all) clear_row(k, i < first ? i : i - first + end, lane);
+  }
 }
 
 }  // namespace
