@@ -19,7 +19,9 @@
  * request that holds length[b] tokens and has n = starts[b + 1] - starts[b] queries: query i is the request's token
  * length - n + i and sees the tokens 0 .. length - n + i (its own was appended before). A query that sees nothing (an empty
  * request; more queries than tokens) has zeros as its output and -infinity as its log-sum-exp. Tokens whose table entry names
- * no page of the pool are not seen. What a page holds behind a request's last token is never used, whatever its bytes are.
+ * no page of the pool are not seen. What a page holds behind a request's last token is never used, whatever its bytes are. A token
+ * whose K holds NaN makes the KV head's rows that see it NaN, one whose V does the 16 channels of the NaN block in those rows;
+ * rows that do not see it are as if it were not there.
  *
  * All functions enqueue on `stream`, allocate nothing and do not synchronise; lengths, tables and slots live on the device, so
  * a captured call follows them. Status codes as in mlops_fbla.h; mlops_paged_last_error() is the calling thread's message. */

@@ -231,18 +231,34 @@ template <int TYPE, int NT> __device__ __forceinline__ void scores(const uint8_t
       }
     }
 }
-// O^T += V^T P^T of a block; of its tokens only the first `tokens` count (EDGE: they may be fewer than 16)
-template <int NT, bool EDGE> __device__ __forceinline__ void values(const uint8_t *block, const uint32_t (&p)[NT][2], Sums<NT> &s, int tokens, int lane) {
+// O^T += V^T P^T of a block whose first token is `token`; of its tokens only the first `tokens` count (EDGE: they may be fewer than 16, and columns may see fewer).
+// A weight of 0 times NaN is NaN: at an edge NaN scales are taken as 0, and NaN goes into the sums of the columns that see such a token. The lane's sixteen
+// channels have one scale per token, and a column sees all tokens up to its limit, so that the first such token decides.
+template <int NT, bool EDGE>
+__device__ __forceinline__ void values(const uint8_t *block, const uint32_t (&p)[NT][2], const int (&limit)[NT][2], Sums<NT> &s, int token, int tokens, int lane) {
   const int g = lane >> 2, t = lane & 3;
   // rows 2 t, 2 t + 1 (and + 8) of the K extent are tokens t, (t ^ 1) + 4 (and + 8)
   const int at[4] = {t, (t ^ 1) + 4, t + 8, (t ^ 1) + 12};
   uint2 v[4];
   uint32_t sv[4];
+  int nan = BT;  // the block's first token with a NaN scale
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     v[i] = fbla::lds64(block + V_CODES + at[i] * CODE_BYTES + 8 * g);
     sv[i] = block[V_SCALES + at[i] * SCALE_BYTES + g];
     if (EDGE && at[i] >= tokens) sv[i] = 0;  // (what is stored behind the last token may be anything, NaN too)
+    if (EDGE && (sv[i] & 0x7f) == 0x7f) sv[i] = 0, nan = min(nan, at[i]);
+  }
+  if (EDGE && __any_sync(FULL, nan < BT)) {
+    nan = min(nan, __shfl_xor_sync(FULL, nan, 1));
+    nan = min(nan, __shfl_xor_sync(FULL, nan, 2));
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (nan < BT && token + nan <= limit[j][i])
+#pragma unroll
+          for (int n = 0; n < 8; ++n) s.o[j][n][i] = s.o[j][n][2 + i] = __int_as_float(0x7fc00000);
   }
   const uint32_t s01 = scales_to_half2(sv[0] | sv[1] << 8), s23 = scales_to_half2(sv[2] | sv[3] << 8);
 #pragma unroll
@@ -319,7 +335,7 @@ __device__ __forceinline__ void take_unit(const uint8_t (&block)[2][BLOCK_BYTES]
       p[j][0] = transpose8(from_floats<MLOPS_PAGED_FP16>(x[n][j][0], x[n][j][1]));
       p[j][1] = transpose8(from_floats<MLOPS_PAGED_FP16>(x[n][j][2], x[n][j][3]));
     }
-    values<NT, EDGE>(block[n], p, s, there >> n & 1 ? tokens - token - 16 * n : 0, lane);
+    values<NT, EDGE>(block[n], p, Q.limit, s, token + 16 * n, there >> n & 1 ? tokens - token - 16 * n : 0, lane);
   }
 }
 

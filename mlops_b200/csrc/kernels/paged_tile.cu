@@ -24,6 +24,7 @@
 #include "fbla_launch.h"
 #include "fbla_tc.cuh"
 #include "paged_attend.cuh"
+#include <climits>
 
 namespace paged {
 namespace {
@@ -61,6 +62,7 @@ struct __align__(1024) Smem {
   uint8_t there[4][8];  // [tile of tokens % 4][block]: 1 where the table names a page
   float down[2][ROWS];      // the rows' factors
   float exchange[2][ROWS];  // between the two threads of a row
+  int v_nan, nan_from[8];   // some V of the run has a NaN scale; [16 channels] of a row of work: the first token with one
   uint8_t over[2][2][4];    // [turn % 2][half of the tokens][quarter of the rows]: a score passes 2^15
   Row begin, row[8];    // the run's first row of work; the softmax warps' rows
   long long warp_sum[THREADS / 32];
@@ -197,6 +199,9 @@ __device__ __forceinline__ void store_operand(uint8_t *tile, const Raw &x, int r
   }
 }
 
+// bit 7 of every byte of four scales that is NaN (0x7f, 0xff)
+__device__ __forceinline__ uint32_t nan_scales(uint32_t scales) { return ((scales & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
 // Where the run's blocks lie, two lanes per tile, up to 32 tiles ahead of the producers, NO_TILE behind the last one: by one warp.
 __device__ __forceinline__ void look_up(const Call &k, Smem &sm, long long hi, int lane) {
   const int per_page = k.c.page_size / BT, half = lane & 1;
@@ -287,6 +292,13 @@ __device__ __forceinline__ void produce(Smem &sm, int warp, int lane) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         if (8 * i + (lane & 7) >= now.left) rv.scales[i] = 0;
+    }
+    // (0 times NaN is NaN, for rows too that do not see the token: such scales are taken as 0, and spoil_rows puts NaN into the rows that see them)
+    if (const uint32_t nan = nan_scales(rv.scales[0] | rv.scales[1] << 16)) {
+      const uint32_t keep = ~((nan >> 7) * 255u);
+      rv.scales[0] &= keep;
+      rv.scales[1] &= keep >> 16;
+      sm.v_nan = 1;
     }
     if (at >= STAGES) ok = ok && wait(sm, &sm.v_empty[at % STAGES], (at / STAGES & 1) ^ 1);
     ok = __all_sync(FULL, ok);
@@ -698,6 +710,42 @@ template <int TYPE> __device__ __forceinline__ void join_row(const Call &k, Smem
   __syncthreads();
 }
 
+// NaN into what the CTA has stored of its rows, 16 channels at a time, where a token that the row sees has a NaN scale of V: by all threads, from the pages, only
+// where a producer has met such a token. A row sees all tokens up to its limit, so that the first such token of a row of work's tiles decides.
+__device__ __forceinline__ void spoil_rows(const Call &k, Smem &sm, long long hi, int tid) {
+  Row w = sm.begin;
+  do {
+    if (tid < 8) sm.nan_from[tid] = INT_MAX;
+    __syncthreads();
+    const int end = min(w.n1 * TOKENS, w.r.tokens);
+    for (int t = w.n0 * TOKENS + tid; t < end; t += THREADS) {
+      const int column = t / k.c.page_size, at = t - column * k.c.page_size, page = __ldg(k.a.table + (size_t)w.b * k.a.table_stride + column);
+      if ((unsigned)page >= (unsigned)k.c.pages) continue;
+      const uint2 scales = __ldg(reinterpret_cast<const uint2 *>(k.c.units + (size_t)page * k.c.page_stride + (size_t)w.head * k.c.head_stride + (size_t)(at / BT) * BLOCK_BYTES +
+                                                                 V_SCALES + at % BT * SCALE_BYTES));
+      for (int j = 0; j < 8; ++j)
+        if (nan_scales(j < 4 ? scales.x : scales.y) >> (8 * (j & 3) + 7) & 1) atomicMin(&sm.nan_from[j], t);
+    }
+    __syncthreads();
+    const bool whole = w.n0 == 0 && w.n1 == w.tiles;
+    for (int e = tid; e < w.rows(k) * 8; e += THREADS) {
+      const int c = e >> 3, j = e & 7;
+      int query, head;
+      split_column(k, 2 * ROWS * w.pair + c, query, head);
+      if (w.r.length - w.r.n + query < sm.nan_from[j]) continue;
+      if (whole) {
+        uint4 *const dst = reinterpret_cast<uint4 *>(out_row(k, w.r.start + query, w.head * k.group + head)) + 2 * j;
+        dst[0] = dst[1] = make_uint4(0x7fff7fff, 0x7fff7fff, 0x7fff7fff, 0x7fff7fff);
+      } else {
+        float4 *const dst = reinterpret_cast<float4 *>(k.tile_part + (((size_t)blockIdx.x * 2 + (w.n0 ? 0 : 1)) * 2 * ROWS + c) * PSTRIDE) + 4 * j;
+        const float x = __int_as_float(0x7fc00000);
+        for (int i = 0; i < 4; ++i) __stcg(dst + i, make_float4(x, x, x, x));
+      }
+    }
+    __syncthreads();
+  } while (next_row(k, sm.before, hi, w));
+}
+
 template <int TYPE> __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const Call k) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Smem &sm = *reinterpret_cast<Smem *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -715,7 +763,7 @@ template <int TYPE> __global__ void __launch_bounds__(THREADS, 1) tile_kernel(co
       fbla::mbar_init(&sm.places_full[i], 1);
       fbla::mbar_init(&sm.places_empty[i], PRODUCERS);
     }
-    sm.abort = 0;
+    sm.abort = sm.v_nan = 0;
     fbla::mbar_init_fence();
   }
   fbla::wait_previous_pass();
@@ -788,6 +836,7 @@ template <int TYPE> __global__ void __launch_bounds__(THREADS, 1) tile_kernel(co
   __syncthreads();
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(sm.tmem) : "memory");
   if (!tiles) return;
+  if (sm.v_nan) spoil_rows(k, sm, hi, tid);
 
   // the run's first and last rows of work, where they are cut
   const Row w = sm.begin;

@@ -59,3 +59,62 @@ def test_rows_before_a_first_request_behind_the_last_row(paged):
     q = torch.randn((8, 4, 128), generator=gen, device="cuda").to(torch.float16)
     out, lse = attend_into_marked(paged, q[:5], cache, table, ints([50]), ints([1000, 1001]))
     assert bool((out == 0).all()) and bool(torch.isneginf(lse).all())
+
+
+def with_bad_values(cache, table, b, bad):
+    """NaN scales of V at (position, KV head, block of 16 channels, byte) of request b; a copy of the pool in which these blocks are zeros"""
+    zeroed, P = cache.units.clone(), cache.page_size
+    for position, head, block, byte in bad:
+        page, at = int(table[b, position // P]), position % P
+        for units, value in ((cache.units, byte), (zeroed, 0)):
+            pu.fields(units)[3][page, head, at // 16, at % 16, block] = value
+    return zeroed
+
+
+def check_bad_values(paged, name, q, cache, table, lengths, counts, b, bad, starts):
+    """NaN in the 16 channels of the rows that see them, all else as if these blocks were zeros"""
+    zeroed = with_bad_values(cache, table, b, bad)
+    heads, group = zeroed.shape[1], q.shape[1] // zeroed.shape[1]
+    first = sum(counts[:b])
+    limit = torch.arange(lengths[b] - counts[b], lengths[b], device="cuda")
+    nan = torch.zeros(q.shape, dtype=torch.bool, device="cuda")
+    for position, head, block, _ in bad:
+        if int(table[b, position // cache.page_size]) in range(cache.pages):
+            nan[first : first + counts[b], head * group : (head + 1) * group, 16 * block : 16 * block + 16] |= (limit >= position)[:, None, None]
+    out, lse = paged.attend(q, cache, table, ints(lengths), starts, return_lse=True)
+    assert torch.equal(out.isnan(), nan)
+    value, weight, log = pu.attend(q, zeroed, cache.k_scale, cache.v_scale, table, lengths, counts)
+    agree(torch.where(nan, value.to(out.dtype), out), lse, (value, weight, log), name)
+
+
+@pytest.mark.parametrize("name", ["bf16", "fp16"])
+@pytest.mark.parametrize("group, length, n", [(4, 200, 1), (4, 200, 2), (1, 200, 30), (4, 200, 8), (3, 77, 5), (4, 200, 20), (2, 200, 64), (4, 200, 60), (4, 333, 333), (8, 3000, 700), (1, 260, 260)])
+def test_not_a_number_in_v_stays_behind_the_causal_limit(paged, name, group, length, n):
+    """both kernels, rows of work of all widths; tokens that no row, some rows and all rows see, and the request beside it"""
+    lengths, counts, heads = [150, length, 90], [min(n, 3), n, 2 if n > 1 else 1], 2
+    gen, table, cache = paged_case(paged, length + n, lengths, heads, 64)
+    q = torch.randn((sum(counts), heads * group, 128), generator=gen, device="cuda").to(TYPES[name][0])
+    bad = [(length - 1, 1, 4, 0x7F), (length - 1 - n // 2, 0, 0, 0xFF), (length - 1 - n // 3, 1, 7, 0x7F), (length - max(n - 1, 1), 1, 5, 0xFF)]
+    if n < length:
+        bad.append((3, 0, 6, 0x7F))
+    check_bad_values(paged, name, q, cache, table, lengths, counts, 1, bad, starts_of(counts) if max(counts) > 1 else None)
+
+
+@pytest.mark.parametrize("n", [2, 7, 30, 100])
+def test_rows_that_see_nothing_beside_not_a_number_in_v(paged, n):
+    """more queries than tokens: the first rows see nothing and are zeros, whatever the tokens hold"""
+    lengths, counts = [1 + n // 3], [n]
+    gen, table, cache = paged_case(paged, n, lengths, 2, 16)
+    q = torch.randn((n, 8, 128), generator=gen, device="cuda").to(torch.bfloat16)
+    check_bad_values(paged, "bf16", q, cache, table, lengths, counts, 0, [(p, h, (3 * p + h) % 8, 0x7F) for p in range(lengths[0]) for h in range(2)], starts_of(counts))
+
+
+@pytest.mark.parametrize("n", [3, 20, 90])
+def test_not_a_number_in_v_of_a_page_that_is_not_there(paged, n):
+    lengths, counts = [300], [n]
+    gen, table, cache = paged_case(paged, n, lengths, 2, 32)
+    q = torch.randn((n, 8, 128), generator=gen, device="cuda").to(torch.bfloat16)
+    whole = table.clone()
+    table[0, 4] = -1
+    with_bad_values(cache, whole, 0, [(4 * 32 + 5, 0, 2, 0x7F)])
+    check_bad_values(paged, "bf16", q, cache, table, lengths, counts, 0, [(299, 0, 3, 0x7F)], starts_of(counts))
