@@ -71,7 +71,9 @@ typedef struct mlops_paged_assign_args {
 mlops_fbla_status mlops_paged_assign(const mlops_paged_assign_args *args, cudaStream_t stream);
 
 /* Quantises K and V of `tokens` tokens, [tokens][kv_heads][128] with strides in elements (multiples of 8, 16-byte aligned rows),
- * into their slots; tokens whose slot is not one of the pool's are left out. Where two tokens have one slot, one of them stays. */
+ * into their slots; tokens whose slot is not one of the pool's are left out. The slots of the pool are distinct: nothing orders two tokens of one
+ * slot, which may end with one's codes and the other's scales, other from run to run; no other slot is touched. (Those that
+ * mlops_paged_assign gives are, where no page is in two places of the ring and the table's rows.) */
 mlops_fbla_status mlops_paged_append(const mlops_paged_cache *cache, int tokens, int type, const void *k, int64_t k_token_stride, int64_t k_head_stride,
                                      const void *v, int64_t v_token_stride, int64_t v_head_stride, const int *slots, cudaStream_t stream);
 

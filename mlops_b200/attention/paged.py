@@ -191,7 +191,8 @@ def assign(table: torch.Tensor, held: torch.Tensor, added: torch.Tensor, free: t
 
 def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> PagedCache:
     """Quantise ``k, v [tokens, kv_heads, 128]`` (BF16 or FP16, slices of a fused projection as they are) into the pool's ``slots`` (int32 [tokens]; a
-    slot outside the pool, -1 for instance: the token is left out). In place; the cache is also returned."""
+    slot outside the pool, -1 for instance: the token is left out). The slots of the pool have to be distinct: what two tokens of one slot leave there may be
+    a mixture of both. In place; the cache is also returned."""
     pool, heads, index = _pool(cache)
     if not _on(index):
         with torch.cuda.device(index):
