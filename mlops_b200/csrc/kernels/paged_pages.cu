@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(THREADS) assign_kernel(const mlops_paged_assig
   if (tid == 0) starts[a.batch] = (int)min(all_new, (long long)INT_MAX), before[a.batch] = all_pages;
   __syncthreads();
   const int64_t head = __ldg(reinterpret_cast<const long long *>(a.cursor)), tail = __ldg(reinterpret_cast<const long long *>(a.cursor) + 1);
-  const int64_t left = max((long long)(tail - head), 0ll);
+  const int64_t left = min(max((long long)(tail - head), 0ll), (long long)a.ring_size);  // (never more than the ring holds)
   if (blockIdx.x == 0) {
     for (int b = tid; b <= a.batch; b += THREADS) {
       a.starts[b] = starts[b];
@@ -105,7 +105,10 @@ __global__ void __launch_bounds__(THREADS) assign_kernel(const mlops_paged_assig
         page = __ldg(entry);
       } else if (column < a.width) {
         const int64_t nth = before[lo] + column - have;
-        if (nth < left) page = __ldg(a.ring + (head + nth) % a.ring_size);
+        if (nth < left) {
+          const int64_t at = (head + nth) % a.ring_size;
+          page = __ldg(a.ring + (at < 0 ? at + a.ring_size : at));
+        }
         if (position % P == 0) *entry = page;
       }
       if (page >= 0) slot = page * P + position % P;

@@ -118,3 +118,18 @@ def test_not_a_number_in_v_of_a_page_that_is_not_there(paged, n):
     table[0, 4] = -1
     with_bad_values(cache, whole, 0, [(4 * 32 + 5, 0, 2, 0x7F)])
     check_bad_values(paged, "bf16", q, cache, table, lengths, counts, 0, [(299, 0, 3, 0x7F)], starts_of(counts))
+
+
+@pytest.mark.parametrize("size, head, tail", [(0, 0, 3), (0, 5, 1 << 40), (4, 0, 100), (4, 3, 8), (7, -5, 2), (7, -20, -9), (3, 9, 9), (3, 9, 4), (5, (1 << 62) + 1, (1 << 62) + 4)])
+def test_rings_of_every_size_and_cursor(paged, size, head, tail):
+    """a ring holds at most its size, none where it has no places or its ends are crossed; cursors are taken modulo the size, negative ones too"""
+    P, held, added = 16, [0, 10, 40], [20, 30, 16]  # two, two and one new pages
+    table, ring = [[-1] * 5, [90] + [-1] * 4, [91, 92, 93, -1, -1]], [10 + i for i in range(size)]
+    left = min(max(tail - head, 0), size)
+    want = [ring[(head + i) % size] if i < left else -1 for i in range(5)]
+    device_table = ints(table)
+    step = paged.assign(device_table, ints(held), ints(added), ints(ring), torch.tensor([head, tail], dtype=torch.int64, device="cuda"), P, sum(added))
+    table[0][:2], table[1][1:3], table[2][3] = want[:2], want[2:4], want[4]
+    assert device_table.tolist() == table and step.cursor.tolist() == [head + min(left, 5), tail, 5 - min(left, 5)]
+    slots = [table[b][p // P] * P + p % P if table[b][p // P] >= 0 else -1 for b, (h, n) in enumerate(zip(held, added)) for p in range(h, h + n)]
+    assert step.slots.tolist() == slots
