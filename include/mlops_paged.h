@@ -56,8 +56,10 @@ typedef struct mlops_paged_cache {
  * Outputs: starts[batch + 1] (exclusive sums of added), lengths[batch] = held + added, and for token i < `tokens` of the call
  * (request by request) its slot and its position in its request; tokens behind starts[batch] have slot and position -1.
  * moved = {cursor[0] + pages taken, cursor[1], pages that were missing}: where the ring runs out or a request outgrows the
- * table's width, entries and slots are -1. The ring holds cursor[1] - cursor[0] pages, at least none and at most ring_size (which may be 0). It is not written: pages go back to it by storing their numbers at
- * ring[cursor[1] % ring_size ...] and advancing cursor[1]. Negative counts are taken as 0. No output may overlap an input. */
+ * table's width, entries and slots are -1. The ring holds cursor[1] - cursor[0] pages, at least none and at most ring_size
+ * (which may be 0). It is not written: pages go back to it by storing their numbers at ring[cursor[1] % ring_size ...] and
+ * advancing cursor[1]. Negative counts are taken as 0, lengths end at 2^31 - 1, a position or slot behind that is -1. No
+ * output may overlap an input. */
 typedef struct mlops_paged_assign_args {
   int batch, tokens, page_size, width; /* width: entries of a table row that may be used; batch at most 16384 */
   int64_t table_stride;                /* entries between rows of the table */

@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(THREADS) assign_kernel(const mlops_paged_assig
   if (blockIdx.x == 0) {
     for (int b = tid; b <= a.batch; b += THREADS) {
       a.starts[b] = starts[b];
-      if (b < a.batch) a.lengths[b] = max(__ldg(a.held + b), 0) + max(__ldg(a.added + b), 0);
+      if (b < a.batch) a.lengths[b] = (int)min((long long)max(__ldg(a.held + b), 0) + max(__ldg(a.added + b), 0), (long long)INT_MAX);
     }
     if (tid == 0) {
       const int64_t taken = min((long long)all_pages, (long long)left);
@@ -96,22 +96,26 @@ __global__ void __launch_bounds__(THREADS) assign_kernel(const mlops_paged_assig
         const int mid = (lo + hi) >> 1;
         if (starts[mid] <= i) lo = mid; else hi = mid;
       }
-      const int held = max(__ldg(a.held + lo), 0), P = a.page_size;
-      position = held + i - starts[lo];
-      const int column = position / P, have = columns(held, P, a.width);
-      int *const entry = a.table + (size_t)lo * a.table_stride + column;
-      int page = -1;
-      if (column < have) {
-        page = __ldg(entry);
-      } else if (column < a.width) {
-        const int64_t nth = before[lo] + column - have;
-        if (nth < left) {
-          const int64_t at = (head + nth) % a.ring_size;
-          page = __ldg(a.ring + (at < 0 ? at + a.ring_size : at));
+      const int P = a.page_size;
+      const uint32_t held = max(__ldg(a.held + lo), 0), p = held + (uint32_t)(i - starts[lo]);
+      if (p <= INT_MAX) {  // (a position behind that is in no table)
+        position = (int)p;
+        const int column = position / P, have = columns(held, P, a.width);
+        int *const entry = a.table + (size_t)lo * a.table_stride + column;
+        int page = -1;
+        if (column < have) {
+          page = __ldg(entry);
+        } else if (column < a.width) {
+          const int64_t nth = before[lo] + column - have;
+          if (nth < left) {
+            const int64_t at = (head + nth) % a.ring_size;
+            page = __ldg(a.ring + (at < 0 ? at + a.ring_size : at));
+          }
+          if (position % P == 0) *entry = page;
         }
-        if (position % P == 0) *entry = page;
+        const int64_t in_pool = (int64_t)page * P + position % P;
+        if (page >= 0 && in_pool <= INT_MAX) slot = (int)in_pool;  // (a pool has fewer than 2^31 slots)
       }
-      if (page >= 0) slot = page * P + position % P;
     }
     a.slots[i] = slot;
     a.positions[i] = position;

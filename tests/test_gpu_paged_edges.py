@@ -133,3 +133,17 @@ def test_rings_of_every_size_and_cursor(paged, size, head, tail):
     assert device_table.tolist() == table and step.cursor.tolist() == [head + min(left, 5), tail, 5 - min(left, 5)]
     slots = [table[b][p // P] * P + p % P if table[b][p // P] >= 0 else -1 for b, (h, n) in enumerate(zip(held, added)) for p in range(h, h + n)]
     assert step.slots.tolist() == slots
+
+
+def test_pages_and_positions_that_pass_31_bits(paged):
+    """a page number whose slots lie behind 2^31 gives no slot (not another page's, modulo 2^32); positions and lengths end at 2^31 - 1"""
+    P, last = 64, 2 ** 31 - 1
+    table = ints([[1 << 27, -1, -1], [(1 << 25) - 1, -1, -1], [7, 8, 9], [1 << 25, -1, -1]])
+    held, added = [3, 60, last - 4, 64], [2, 3, 8, 1]
+    ring = ints([1 << 26])
+    step = paged.assign(table, ints(held), ints(added), ring, torch.tensor([0, 1], dtype=torch.int64, device="cuda"), P, sum(added))
+    positions = [3, 4, 60, 61, 62] + [last - 4 + i for i in range(5)] + [-1, -1, -1] + [64]
+    assert step.positions.tolist() == positions
+    assert step.slots.tolist() == [-1, -1] + [((1 << 25) - 1) * P + i for i in (60, 61, 62)] + [-1] * 8 + [-1]
+    assert step.lengths.tolist() == [5, 63, last, 65] and step.starts.tolist() == [0, 2, 5, 13, 14]
+    assert table[3].tolist() == [1 << 25, 1 << 26, -1] and step.cursor.tolist() == [1, 1, 1]
