@@ -54,7 +54,9 @@ typedef struct mlops_paged_cache {
 /* Pages for `added[b]` new tokens of each request b, which holds held[b]: taken from the ring of free pages
  * ring[cursor[0] % ring_size] .. ring[(cursor[1] - 1) % ring_size], in the order of the requests, and entered into the table.
  * Outputs: starts[batch + 1] (exclusive sums of added), lengths[batch] = held + added, and for token i < `tokens` of the call
- * (request by request) its slot and its position in its request; tokens behind starts[batch] have slot and position -1.
+ * (request by request) its slot and its position in its request; tokens behind starts[batch] have slot and position -1. Where
+ * more than `tokens` are added in all, those behind are left out of everything (starts[batch] = tokens, lengths without them,
+ * no page taken for them); the pages that they would have needed count as missing.
  * moved = {cursor[0] + pages taken, cursor[1], pages that were missing}: where the ring runs out or a request outgrows the
  * table's width, entries and slots are -1. The ring holds cursor[1] - cursor[0] pages, at least none and at most ring_size
  * (which may be 0). It is not written: pages go back to it by storing their numbers at ring[cursor[1] % ring_size ...] and

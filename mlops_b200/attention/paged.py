@@ -163,7 +163,8 @@ def assign(table: torch.Tensor, held: torch.Tensor, added: torch.Tensor, free: t
 
     New pages are taken from the ring ``free`` (int32, from ``cursor[0]`` up to ``cursor[1]``, both counted without end and taken modulo the ring's
     size), in the order of the requests, and entered into ``table`` (int32 [batch, width], in place). ``tokens``: rows of the step, at least the sum of
-    ``added``; rows behind it get slot and position -1. Where the ring runs out or a request outgrows its row, entries and slots are -1 and
+    ``added``; rows behind it get slot and position -1. (Where it is less, the tokens behind it are not added: ``Step.starts`` ends at ``tokens``, ``Step.lengths``
+    are without them, and the pages that they would have needed count as missing.) Where the ring runs out or a request outgrows its row, entries and slots are -1 and
     ``Step.cursor[2]`` counts the pages that were missing. A request's pages are given back by ``free[tail % size ...] = table[b, :n]`` and advancing
     the tail, ``cursor[1]``."""
     index = table.get_device()

@@ -3,7 +3,8 @@
 // Two exclusive sums over the requests give everything: starts (of the new tokens) and before (of the new pages). Token i belongs to the request
 // b with starts[b] <= i < starts[b + 1], is its token p = held[b] + i - starts[b], and lies in column p / P of its table row: in the page that is
 // there, where the column was in use before, else in page ring[head + before[b] + column - columns in use]. The token that opens a page enters
-// it into the table. Nothing that is read is written in the same call, so no CTA waits for another: every CTA forms both sums for itself (8 bytes
+// it into the table. Tokens without a row of the step (it has fewer than are added) are not added: starts end at `tokens`, and what follows from them -- lengths,
+// pages that are taken -- leaves them out, so that every page that is taken is in the table. Nothing that is read is written in the same call, so no CTA waits for another: every CTA forms both sums for itself (8 bytes
 // per request from L2) and serves a share of the tokens. Bound by latency, launch and two passes over the requests: 64 requests of one new token each 3.6 us on the
 // device, 500 with some 40 000 new tokens 8.1.
 #include "fbla_launch.h"
@@ -20,6 +21,16 @@ constexpr int THREADS = 256;
 __device__ __forceinline__ int columns(long long tokens, int page_size, int width) {
   const long long n = (tokens + page_size - 1) / page_size;
   return (int)(n < width ? n : width);
+}
+
+// the request of token i: starts[b] <= i < starts[b + 1]
+__device__ __forceinline__ int request_of(const int *starts, int batch, int i) {
+  int lo = 0, hi = batch;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (starts[mid] <= i) lo = mid; else hi = mid;
+  }
+  return lo;
 }
 
 __global__ void __launch_bounds__(THREADS) assign_kernel(const mlops_paged_assign_args a) {
@@ -66,23 +77,28 @@ __global__ void __launch_bounds__(THREADS) assign_kernel(const mlops_paged_assig
       all_pages += warp_pages[w];
     }
     if (b < a.batch) {
-      starts[b] = (int)min(n_base + n_sum - n, (long long)INT_MAX);
+      starts[b] = (int)min(n_base + n_sum - n, (long long)a.tokens);
       before[b] = p_base + p_sum - pages;
     }
     __syncthreads();
   }
   if (over) atomicAdd(&over_all, over);
-  if (tid == 0) starts[a.batch] = (int)min(all_new, (long long)INT_MAX), before[a.batch] = all_pages;
+  if (tid == 0) starts[a.batch] = (int)min(all_new, (long long)a.tokens), before[a.batch] = all_pages;
   __syncthreads();
   const int64_t head = __ldg(reinterpret_cast<const long long *>(a.cursor)), tail = __ldg(reinterpret_cast<const long long *>(a.cursor) + 1);
   const int64_t left = min(max((long long)(tail - head), 0ll), (long long)a.ring_size);  // (never more than the ring holds)
   if (blockIdx.x == 0) {
     for (int b = tid; b <= a.batch; b += THREADS) {
       a.starts[b] = starts[b];
-      if (b < a.batch) a.lengths[b] = (int)min((long long)max(__ldg(a.held + b), 0) + max(__ldg(a.added + b), 0), (long long)INT_MAX);
+      if (b < a.batch) a.lengths[b] = (int)min((long long)max(__ldg(a.held + b), 0) + (starts[b + 1] - starts[b]), (long long)INT_MAX);
     }
     if (tid == 0) {
-      const int64_t taken = min((long long)all_pages, (long long)left);
+      int pages = all_pages;
+      if (all_new > a.tokens) {  // cut: the pages of the requests before the last one that has rows, and those of its rows
+        const int b = a.tokens ? request_of(starts, a.batch, a.tokens - 1) : 0, held = max(__ldg(a.held + b), 0);
+        pages = before[b] + columns((long long)held + (starts[b + 1] - starts[b]), a.page_size, a.width) - columns(held, a.page_size, a.width);
+      }
+      const int64_t taken = min((long long)pages, (long long)left);
       a.moved[0] = head + taken;
       a.moved[1] = tail;
       a.moved[2] = all_pages - taken + over_all;
@@ -91,11 +107,7 @@ __global__ void __launch_bounds__(THREADS) assign_kernel(const mlops_paged_assig
   for (int i = blockIdx.x * THREADS + tid; i < a.tokens; i += gridDim.x * THREADS) {
     int slot = -1, position = -1;
     if (i < starts[a.batch]) {
-      int lo = 0, hi = a.batch;  // starts[lo] <= i < starts[hi]
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (starts[mid] <= i) lo = mid; else hi = mid;
-      }
+      const int lo = request_of(starts, a.batch, i);
       const int P = a.page_size;
       const uint32_t held = max(__ldg(a.held + lo), 0), p = held + (uint32_t)(i - starts[lo]);
       if (p <= INT_MAX) {  // (a position behind that is in no table)

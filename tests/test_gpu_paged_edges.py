@@ -147,3 +147,39 @@ def test_pages_and_positions_that_pass_31_bits(paged):
     assert step.slots.tolist() == [-1, -1] + [((1 << 25) - 1) * P + i for i in (60, 61, 62)] + [-1] * 8 + [-1]
     assert step.lengths.tolist() == [5, 63, last, 65] and step.starts.tolist() == [0, 2, 5, 13, 14]
     assert table[3].tolist() == [1 << 25, 1 << 26, -1] and step.cursor.tolist() == [1, 1, 1]
+
+
+def assign_cut(table, held, added, ring, head, tail, P, tokens):
+    """page assignment by loops for the first `tokens` new tokens; `missing` counts for all of them"""
+    width, need = len(table[0]), sum(-(-(h + n) // P) - -(-h // P) for h, n in zip(held, added))
+    table, slots, positions, starts, lengths, taken = [list(r) for r in table], [], [], [0], [], 0
+    for b, (h, n) in enumerate(zip(held, added)):
+        n = min(n, tokens - starts[-1])
+        for p in range(h, h + n):
+            column = p // P
+            if p % P == 0 and column < width:
+                table[b][column] = ring[(head + taken) % len(ring)] if head + taken < tail else -1
+                taken += head + taken < tail
+            page = table[b][column] if column < width else -1
+            slots.append(page * P + p % P if page >= 0 else -1)
+            positions.append(p)
+        starts.append(starts[-1] + n)
+        lengths.append(h + n)
+    return table, slots, positions, starts, lengths, [head + taken, tail, need - taken]
+
+
+@pytest.mark.parametrize("held, added, tokens, free", [
+    ([5, 16, 0, 30], [40, 1, 100, 3], 100, 40), ([5, 16, 0, 30], [40, 1, 100, 3], 41, 40), ([5, 16, 0, 30], [40, 1, 100, 3], 40, 40), ([5, 16, 0, 30], [40, 1, 100, 3], 0, 40),
+    ([5, 16, 0, 30], [40, 1, 100, 3], 143, 40), ([5, 16, 0, 30], [40, 1, 100, 3], 100, 4), ([0] * 300, [33] * 300, 4321, 2000), ([7], [500], 300, 40), ([16] * 40, [16] * 40, 16 * 20, 100)])
+def test_fewer_rows_than_new_tokens(paged, held, added, tokens, free):
+    """tokens without a row of the step are not added: no page is taken for them, lengths and starts say what was"""
+    P, width, batch = 16, 12, len(held)
+    table, taken = [[-1] * width for _ in held], 0
+    for b in range(batch):
+        for c in range(-(-held[b] // P)):
+            table[b][c], taken = taken, taken + 1
+    ring = [taken + i for i in range(free)]
+    device_table = ints(table)
+    step = paged.assign(device_table, ints(held), ints(added), ints(ring), torch.tensor([0, free], dtype=torch.int64, device="cuda"), P, tokens)
+    for got, want in zip((device_table, *step), assign_cut(table, held, added, ring, 0, free, P, tokens)):
+        assert got.tolist() == want
