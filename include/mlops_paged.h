@@ -101,7 +101,8 @@ typedef struct mlops_paged_attend_args {
 /* Bytes of scratch a call of this shape needs (0: the arguments are refused). Of the pointers only starts is looked at: null or not. */
 size_t mlops_paged_attend_scratch_bytes(const mlops_paged_attend_args *args, int kv_heads);
 /* Rows of q that are no request's, before starts[0] and behind starts[batch], have zeros as their output and -infinity as their log-sum-exp:
- * a slice of a step's requests (table, lengths and starts from request b on) goes with all of the step's rows. The scratch (16-byte aligned) is filled with zeros once, before its first call; what a
+ * a slice of a step's requests (table, lengths and starts from request b on) goes with all of the step's rows. Where starts[batch] is
+ * above `tokens`, the rows that q does not have are left out and the others see what they would beside them. The scratch (16-byte aligned) is filled with zeros once, before its first call; what a
  * call leaves in it serves the next one, of whatever shape. Calls that overlap need scratches of their own. */
 mlops_fbla_status mlops_paged_attend(const mlops_paged_attend_args *args, const mlops_paged_cache *cache, void *scratch, size_t scratch_bytes, cudaStream_t stream);
 

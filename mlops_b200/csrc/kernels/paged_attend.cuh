@@ -28,22 +28,26 @@ __device__ __forceinline__ void split_column(const Call &k, int column, int &que
   head = column - query * k.group;
 }
 
-// request b's queries and tokens, as far as q's rows and the table's width go
+// request b's queries and tokens, as far as q's rows and the table's width go. Rows that q does not have move no other: row i is the request's token
+// lengths[b] - starts[b + 1] + i.
 struct Request {
-  int start, n, length, tokens;  // first row of q, queries, lengths[b], tokens that a table row can name
+  int start, n, at, tokens;  // first row of q, queries, the first one's token (negative: before the request), tokens that a table row can name
 };
 __device__ __forceinline__ Request request(const Call &k, int b) {
   Request r;
+  int e = b + 1;
   if (k.a.starts) {
-    const int s = __ldg(k.a.starts + b), e = __ldg(k.a.starts + b + 1);
+    const int s = __ldg(k.a.starts + b);
+    e = __ldg(k.a.starts + b + 1);
     r.start = min(max(s, 0), k.a.tokens);
     r.n = max(min(e, k.a.tokens) - r.start, 0);
   } else {
     r.start = b;
     r.n = 1;
   }
-  r.length = max(__ldg(k.a.lengths + b), 0);
-  r.tokens = (int)min((long long)r.length, (long long)k.a.width * k.c.page_size);
+  const int length = max(__ldg(k.a.lengths + b), 0);
+  r.at = length - e + r.start;
+  r.tokens = (int)min((long long)length, (long long)k.a.width * k.c.page_size);
   return r;
 }
 

@@ -140,7 +140,7 @@ template <int TYPE, int NT> struct Columns {  // a row's queries, as B fragments
   __device__ __forceinline__ void convert(const Call &k, const Row<NT> &w, int lane) {
     const int t = lane & 3;
     const float base = k.sl * __ldg(k.c.k_scale + w.head);
-    low = w.r.length - w.r.n + query_of(k, w.tile * 8 * NT);
+    low = w.r.at + query_of(k, w.tile * 8 * NT);
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       uint32_t top = 0;
@@ -162,7 +162,7 @@ template <int TYPE, int NT> struct Columns {  // a row's queries, as B fragments
       for (int i = 0; i < 2; ++i) {
         mult[j][i] = fmaxf(base * __shfl_sync(FULL, down, (2 * t + i) * 4), 1e-37f);  // (not 0: masked scores are -infinity)
         const int cc = 8 * j + 2 * t + i;
-        limit[j][i] = cc < w.columns ? w.r.length - w.r.n + query_of(k, w.tile * 8 * NT + cc) : -1;
+        limit[j][i] = cc < w.columns ? w.r.at + query_of(k, w.tile * 8 * NT + cc) : -1;
       }
     }
   }

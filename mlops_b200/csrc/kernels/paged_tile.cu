@@ -89,7 +89,7 @@ __device__ __forceinline__ uint64_t v_desc(const void *tile, uint32_t byte_offse
 
 // tiles of tokens that rows up to 256 (pair + 1) of a request see
 __device__ __forceinline__ int tiles_of(const Call &k, const Request &r, int pair) {
-  const int last = min(2 * ROWS * (pair + 1), rows_of(k, r)) - 1, seen = min(r.length - r.n + query_of(k, last) + 1, r.tokens);
+  const int last = min(2 * ROWS * (pair + 1), rows_of(k, r)) - 1, seen = min(r.at + query_of(k, last) + 1, r.tokens);
   return max((seen + TOKENS - 1) / TOKENS, 1);  // (rows that see nothing have a tile all the same: their zeros are written like the others' sums)
 }
 __device__ __forceinline__ bool taken(const Call &k, const Request &r) { return r.tokens > 0 && r.n * k.group > k.wide; }
@@ -152,7 +152,7 @@ __device__ __forceinline__ bool next_row(const Call &k, const long long *before,
 // whether half X has a part in tile n of w: w's second half in row order, or every second tile where the halves share the rows; a first half
 // whose rows see less than the second one's leaves the last tile out
 __device__ __forceinline__ int tiles_of_half(const Call &k, const Row &w, int x) {
-  const int last = min(2 * ROWS * w.pair + ROWS * (x + 1), rows_of(k, w.r)) - 1, seen = min(w.r.length - w.r.n + query_of(k, last) + 1, w.r.tokens);
+  const int last = min(2 * ROWS * w.pair + ROWS * (x + 1), rows_of(k, w.r)) - 1, seen = min(w.r.at + query_of(k, last) + 1, w.r.tokens);
   return max((seen + TOKENS - 1) / TOKENS, 1);
 }
 struct Part {
@@ -547,8 +547,8 @@ template <int TYPE> __device__ __forceinline__ void soften(const Call &k, Smem &
       const int c = line + (shared ? 0 : ROWS * x), col = 2 * ROWS * w.pair + c;  // of the row of work, of the request
       const bool live = c < w.rows(k);
       warp_live[x] = c - lane < w.rows(k);
-      q[x] = Line{NOTHING, 0.f, fmaxf(base * sm.down[shared ? 0 : x][line], 1e-37f), live ? w.r.length - w.r.n + query_of(k, col) : -1, false};  // (mult is not 0: masked scores are -infinity)
-      low[x] = w.r.length - w.r.n + query_of(k, col - lane);  // the smallest limit of the warp's rows
+      q[x] = Line{NOTHING, 0.f, fmaxf(base * sm.down[shared ? 0 : x][line], 1e-37f), live ? w.r.at + query_of(k, col) : -1, false};  // (mult is not 0: masked scores are -infinity)
+      low[x] = w.r.at + query_of(k, col - lane);  // the smallest limit of the warp's rows
     }
     const int tiles0 = tiles_of_half(k, w, 0), tiles1 = tiles_of_half(k, w, 1), n0 = w.n0, n1 = w.n1;
 #pragma unroll 1
@@ -732,7 +732,7 @@ __device__ __forceinline__ void spoil_rows(const Call &k, Smem &sm, long long hi
       const int c = e >> 3, j = e & 7;
       int query, head;
       split_column(k, 2 * ROWS * w.pair + c, query, head);
-      if (w.r.length - w.r.n + query < sm.nan_from[j]) continue;
+      if (w.r.at + query < sm.nan_from[j]) continue;
       if (whole) {
         uint4 *const dst = reinterpret_cast<uint4 *>(out_row(k, w.r.start + query, w.head * k.group + head)) + 2 * j;
         dst[0] = dst[1] = make_uint4(0x7fff7fff, 0x7fff7fff, 0x7fff7fff, 0x7fff7fff);

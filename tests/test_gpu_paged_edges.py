@@ -183,3 +183,14 @@ def test_fewer_rows_than_new_tokens(paged, held, added, tokens, free):
     step = paged.assign(device_table, ints(held), ints(added), ints(ring), torch.tensor([0, free], dtype=torch.int64, device="cuda"), P, tokens)
     for got, want in zip((device_table, *step), assign_cut(table, held, added, ring, 0, free, P, tokens)):
         assert got.tolist() == want
+
+
+@pytest.mark.parametrize("group, counts, rows", [(4, [3, 6], 5), (4, [1, 1, 8], 3), (2, [10, 90], 60), (8, [200], 33), (1, [5, 5], 4), (4, [300, 7], 150), (4, [2, 3], 2)])
+def test_fewer_rows_than_the_requests_have(paged, group, counts, rows):
+    """rows that are left out at the end move no other row: each sees what it sees in the whole call"""
+    lengths, heads = [500 + 41 * i for i in range(len(counts))], 2
+    gen, table, cache = paged_case(paged, rows, lengths, heads, 32)
+    q = torch.randn((sum(counts), heads * group, 128), generator=gen, device="cuda").to(torch.bfloat16)
+    out, lse = paged.attend(q[:rows], cache, table, ints(lengths), starts_of(counts), return_lse=True)
+    want = pu.attend(q, cache.units, cache.k_scale, cache.v_scale, table, lengths, counts)
+    agree(out, lse, [x[:rows] for x in want], "bf16")
