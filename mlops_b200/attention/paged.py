@@ -145,10 +145,12 @@ def _rows(x, index, what, heads=None):
     if x.get_device() != index or kind is None or len(shape) != 3 or shape[2] != HEAD_DIM or (heads is not None and shape[1] != heads):
         raise ValueError(f"{what}: expected a bfloat16 or float16 [tokens, {'heads' if heads is None else heads}, {HEAD_DIM}] tensor on cuda:{index}; it is {x.dtype} {tuple(shape)} on {x.device}")
     by_token, by_head, by_channel = x.stride()
+    if shape[0] == 1:  # (a stride that nothing is reached by may be any number, and stays what it is in a copy)
+        by_token = 0
+    if shape[1] == 1:
+        by_head = 0
     if by_channel != 1 or by_token % 8 or by_head % 8 or x.data_ptr() % 16:
-        x = x.contiguous()
-        if x.data_ptr() % 16:
-            x = x.clone()
+        x = torch.empty(shape, dtype=x.dtype, device=x.device).copy_(x)
         by_token, by_head, _ = x.stride()
     return x, shape, by_token, by_head, kind
 

@@ -194,3 +194,26 @@ def test_fewer_rows_than_the_requests_have(paged, group, counts, rows):
     out, lse = paged.attend(q[:rows], cache, table, ints(lengths), starts_of(counts), return_lse=True)
     want = pu.attend(q, cache.units, cache.k_scale, cache.v_scale, table, lengths, counts)
     agree(out, lse, [x[:rows] for x in want], "bf16")
+
+
+@pytest.mark.parametrize("which", [slice(0, 1), slice(1, 2)])
+def test_one_token_of_rows_of_any_width(paged, which):
+    """a dimension of one element has no stride that matters: one row of an array whose rows are no multiple of 8 elements apart, one head of it"""
+    heads, group, P = 2, 2, 16
+    gen, table, cache = paged_case(paged, 4, [40], heads, P)
+    rows = torch.randn((3, 1028), generator=gen, device="cuda").to(torch.bfloat16)
+    q, k, v = (rows[:, at : at + n * 128].view(3, n, 128)[which] for at, n in ((0, heads * group), (512, heads), (768, heads)))
+    assert q.stride(0) % 8 and q.is_contiguous()
+    slots = (table[:, 2] * P + 7).to(torch.int32)
+    other = paged.PagedCache(cache.units.clone(), cache.k_scale, cache.v_scale)
+    paged.append(cache, k, v, slots)
+    paged.append(other, *(torch.empty(x.shape, dtype=x.dtype, device="cuda").copy_(x) for x in (k, v)), slots)
+    assert torch.equal(cache.units, other.units)
+    out, lse = paged.attend(q, cache, table, ints([40]), return_lse=True)
+    agree(out, lse, pu.attend(q, cache.units, cache.k_scale, cache.v_scale, table, [40], [1]), "bf16")
+    # (one head: strides of heads that are no multiple of 8)
+    one = rows.as_strided((2, 1, 128), (128, 1028, 1), which.start * 1028)
+    pair = table.repeat(2, 1)
+    single = paged.PagedCache(cache.units[:, :1], cache.k_scale[:1], cache.v_scale[:1])
+    out, lse = paged.attend(one, single, pair, ints([40, 33]), return_lse=True)
+    agree(out, lse, pu.attend(one, single.units, single.k_scale, single.v_scale, pair, [40, 33], [1, 1]), "bf16")
