@@ -32,6 +32,7 @@ template <int NT> constexpr int WARPS = NT == 1 ? 16 : 8;
 template <int NT> constexpr int STAGES = NT == 1 ? 2 : 3;
 constexpr int UNIT = 2 * BT;  // tokens of a unit
 template <int NT> constexpr int THREADS = 32 * WARPS<NT>;
+constexpr uint32_t DRAIN = 1u << 20;  // polls for a copy after a wait that gave up
 constexpr float TOP = 15.f, REST = 9.f;  // log2 of the largest P, and of a column's largest when m' is set
 
 // a row of work
@@ -475,15 +476,16 @@ template <int TYPE, int NT> __global__ void __launch_bounds__(THREADS<NT>, 1) st
 #pragma unroll 1
       for (; i < end; ++i, token += UNIT) {
         const int stage = i % STAGES<NT>, here = (there[0] >> (i & 31) & 1) | (there[1] >> (i & 31) & 1) << 1;
-        if (alive) alive = fbla::mbar_wait_bounded(&sm.full[warp][stage], (i / STAGES<NT>) & 1);
-        if (__all_sync(FULL, alive)) {
+        if (alive && !__all_sync(FULL, fbla::mbar_wait_bounded(&sm.full[warp][stage], (i / STAGES<NT>) & 1))) {
+          alive = false;  // (for the rest of the run, which asks for nothing more; what it has asked for ends, if it does, before its places are used again)
+          for (int n = i; n < min(i + STAGES<NT>, count); ++n) fbla::mbar_wait_bounded(&sm.full[warp][n % STAGES<NT>], (n / STAGES<NT>) & 1, DRAIN);
+        }
+        if (alive) {
           if (token + UNIT - 1 <= Q.low && here == 3) take_unit<TYPE, NT, false>(sm.ring[warp][stage], Q, s, token, w.r.tokens, 3, lane);
           else if (here) take_unit<TYPE, NT, true>(sm.ring[warp][stage], Q, s, token, w.r.tokens, here, lane);
           __syncwarp();
           const int ahead = i + STAGES<NT>;
           if (ahead < count && lane == (ahead & 31)) issue(ahead, (ahead >> 5) == (i >> 5) ? now : next);
-        } else {
-          alive = false;
         }
         if ((i & 31) == 31) {
           now = next;

@@ -58,6 +58,7 @@ struct __align__(1024) Smem {
   const uint8_t *block[2 * WINDOW][8];  // [tile of the run % (2 WINDOW)][block]: where it lies; null: the table names no page, or the request has no such block
   int left[2 * WINDOW];         // tokens of the request from the tile's first on
   uint64_t places_full[2], places_empty[2];  // of WINDOW tiles each
+  uint64_t drained[2];  // the issuing threads' products, after a wait that gave up
   uint64_t q_ready[2], k_full[STAGES], v_full[STAGES], k_empty[STAGES], v_empty[STAGES], s_ready[2], p_ready[2], o_done[2];
   uint8_t there[4][8];  // [tile of tokens % 4][block]: 1 where the table names a page
   float down[2][ROWS];      // the rows' factors
@@ -760,6 +761,7 @@ template <int TYPE> __global__ void __launch_bounds__(THREADS, 1) tile_kernel(co
       fbla::mbar_init(&sm.v_full[i], PRODUCERS);
       fbla::mbar_init(&sm.k_empty[i], 2);
       fbla::mbar_init(&sm.v_empty[i], 2);
+      fbla::mbar_init(&sm.drained[i], 1);
       fbla::mbar_init(&sm.places_full[i], 1);
       fbla::mbar_init(&sm.places_empty[i], PRODUCERS);
     }
@@ -833,6 +835,11 @@ template <int TYPE> __global__ void __launch_bounds__(THREADS, 1) tile_kernel(co
   tc::tc_fence_after();
   if (warp < PRODUCER0) asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
   else asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
+  if (sm.abort && warp >= ISSUER0 && warp < FINDER && lane == 0) {  // (nobody has waited for these products: they end, if they do, before what they use is given back)
+    tc::mma_commit(&sm.drained[warp - ISSUER0]);
+    fbla::mbar_wait_bounded(&sm.drained[warp - ISSUER0], 0, 1u << 20);
+  }
+  __syncwarp();
   __syncthreads();
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(sm.tmem) : "memory");
   if (!tiles) return;
