@@ -217,3 +217,26 @@ def test_one_token_of_rows_of_any_width(paged, which):
     single = paged.PagedCache(cache.units[:, :1], cache.k_scale[:1], cache.v_scale[:1])
     out, lse = paged.attend(one, single, pair, ints([40, 33]), return_lse=True)
     agree(out, lse, pu.attend(one, single.units, single.k_scale, single.v_scale, pair, [40, 33], [1, 1]), "bf16")
+
+
+@pytest.mark.parametrize("counts", [[1], [6], [200]])
+@pytest.mark.parametrize("at", [5, 39000])
+def test_one_score_far_above_a_long_context(paged, counts, at):
+    """Weights 2^-32 to 2^-24 of the largest, over 40 000 tokens, with V that is 0 in half of the channels of the loud token: these hold what the small weights leave.
+    A weight P is held with its largest at 2^9 or more; in FP16 it is off by 2^-11 of itself, below 2^-14 by 2^-25, which is 2^-34 of the largest. So an element is off by
+    at most 2^-10 sum p |v| / sum p (the bound of the other tests) and 2^-34 max |v| per token that is seen."""
+    length, heads, group, P = 40000, 2, 4, 64
+    gen, table, cache = paged_case(paged, 17, [length], heads, P)
+    height = 6.0 * torch.rand((length, heads), generator=gen, device="cuda")
+    height[at] = 24.0
+    k = (height[..., None] * torch.ones(128, device="cuda")).to(torch.bfloat16)
+    v = (1.0 + torch.rand((length, heads, 128), generator=gen, device="cuda")).to(torch.bfloat16)
+    v[at, :, :64] = 0.0
+    position = torch.arange(length, device="cuda")
+    paged.append(cache, k, v, (table[0, position // P].long() * P + position % P).to(torch.int32))
+    q = torch.ones((counts[0], heads * group, 128), dtype=torch.bfloat16, device="cuda")
+    scale = 32.0 * math.log(2.0) / (24.0 * 128.0)
+    out, lse = paged.attend(q, cache, table, ints([length]), starts_of(counts), scale=scale, return_lse=True)
+    want, weight, want_lse = pu.attend(q, cache.units, cache.k_scale, cache.v_scale, table, [length], counts, scale)
+    assert bool(((out.double() - want).abs() <= 2.0 ** -10 * weight + length * 2.0 ** -34 * 2.5 + TYPES["bf16"][1] * want.abs()).all())
+    assert float(want[..., :64].min()) > 2.0 ** -16 and bool(((lse.double() - want_lse).abs() <= 2.0 ** -12 * (1 + want_lse.abs() / 8)).all())
