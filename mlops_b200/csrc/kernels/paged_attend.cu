@@ -4,8 +4,9 @@
 namespace paged {
 namespace {
 
-// Columns of a request that is streamed, at most. us for 16 requests of 5 000 to 16 000 tokens with 32 columns (8 queries, 32 / 8 heads): streamed 152, tiles 170; with
-// 12 to 24 columns a limit of 16 takes 161, 24 and 32 take 128. A further tile of 16 columns costs the stream some 50, so that 40 columns are the tiles'.
+// Columns of a request that is streamed, at most. us on the device (a graph of calls with a scratch of their own), 16 requests of 5 000 to 16 000 tokens, 32 / 8 heads: 3
+// to 6 queries (12 to 24 columns) take 103 with a limit of 24 or 32 and 156 with 16; 8 queries (32 columns) 125 streamed and 148 as tiles; 10 queries (40 columns), a
+// third tile of the stream, 174 and 152.
 constexpr int WIDE = 32;
 
 struct Scratch {  // offsets: the counters of both kernels (zeros at first), their partial rows
@@ -23,8 +24,8 @@ Scratch scratch_of(int sms, bool tiles) {
 // whether some request may have more than WIDE columns
 bool may_be_wide(const mlops_paged_attend_args *a, int kv_heads) { return a->starts || a->q_heads / kv_heads > WIDE; }
 
-// Streamed in tiles of 8 columns where a request has no more on average, else of 16: 64 requests of 1K-64K tokens and 4 columns each take 183 us in tiles of 8 and 258 in
-// tiles of 16, 16 requests of 5 000 to 16 000 tokens and 12 to 24 columns 120 and 114. The host knows the average only.
+// Streamed in tiles of 8 columns where a request has no more on average, else of 16; us on the device: 64 requests of 1K-64K tokens and 4 columns each take 176 in tiles
+// of 8 and 254 in tiles of 16, 16 requests of 5 000 to 16 000 tokens with 12 to 24 columns 105 and 103, with 32 columns 153 and 125. The host knows the average only.
 template <int TYPE> cudaError_t attend(const Call &k, bool tiles, int sms, cudaStream_t stream) {
   const bool narrow = (int64_t)k.a.tokens * k.group <= (int64_t)8 * k.a.batch;
   const cudaError_t e = narrow ? launch_stream<TYPE, 1>(k, sms, stream) : launch_stream<TYPE, 2>(k, sms, stream);

@@ -5,8 +5,8 @@
 // there, where the column was in use before, else in page ring[head + before[b] + column - columns in use]. The token that opens a page enters
 // it into the table. Tokens without a row of the step (it has fewer than are added) are not added: starts end at `tokens`, and what follows from them -- lengths,
 // pages that are taken -- leaves them out, so that every page that is taken is in the table. Nothing that is read is written in the same call, so no CTA waits for another: every CTA forms both sums for itself (8 bytes
-// per request from L2) and serves a share of the tokens. Bound by latency, launch and two passes over the requests: 64 requests of one new token each 3.6 us on the
-// device, 500 with some 40 000 new tokens 8.1.
+// per request from L2) and serves a share of the tokens. Bound by latency, launch and two passes over the requests: 64 requests of one new token each 3.3 us on the
+// device, 500 with some 40 000 new tokens 7.6.
 #include "fbla_launch.h"
 #include "paged_kernels.h"
 #include "fbla_device.cuh"

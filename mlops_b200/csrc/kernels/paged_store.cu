@@ -1,6 +1,6 @@
 // Quantise-on-write and read-back of the paged cache (mlops_paged_append, mlops_paged_read): a thread has 16 channels of a token and head, of K and of V, so
 // that 64 bytes of a thread's are on their way at once and a slot is looked up once for both. Bound by memory: 65 536 tokens of 8 heads are read back in 56 us =
-// 6.1 TB/s (0.94 of the copy rate), 32 768 appended in 37 us = 4.7 TB/s (0.71; the codes leave in pieces of 8 bytes). With a thread per tensor and two 16-byte
+// 6.1 TB/s (0.94 of the copy rate), 32 768 appended in 37 to 39 us = 4.4 to 4.7 TB/s (0.68 to 0.71; the codes leave in pieces of 8 bytes). With a thread per tensor and two 16-byte
 // accesses for 32 bytes 70 and 50 us.
 #include "fbla_launch.h"
 #include "paged_format.cuh"
@@ -51,7 +51,8 @@ template <bool WIDE> __device__ __forceinline__ void store_channels(uint16_t *p,
 }
 
 // fl(x / s) from r = fl(1 / s): one Newton step on the product is the rounded quotient wherever nothing under- or overflows (the residual of a
-// product within an ulp of it is exact in an FMA), and a code only asks on which side of a halfway case the quotient lies. (The step would take -0 to +0.)
+// product within an ulp of it is exact in an FMA: P. Markstein, Computation of elementary functions on the IBM RISC System/6000 processor, 1990), and a
+// code only asks on which side of a halfway case the quotient lies. (The step would take -0 to +0.)
 __device__ __forceinline__ float quotient(float x, float s, float r) {
   const float q = __fmul_rn(x, r);
   return copysignf(fmaf(fmaf(-q, s, x), r, q), x);

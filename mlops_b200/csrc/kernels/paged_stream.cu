@@ -6,8 +6,9 @@
 //
 // Per block, tokens on the M axis: S^T[16 tokens x 8] = K Q^T and O^T[128 channels x 8] += V^T P^T with mma.sync m16n8k16, FP16 operands, FP32 sums.
 // K and V: code * scale is exact in FP16. Q: FP16 after a power of two per column (q_factor). P: 2^(s - m') with m' between 9 and 15 below the column's
-// largest score so far, rounded to FP16 (relative 2^-11, the only rounding of the operands); m' moves, and O and l are rescaled, only where a score would
-// pass 2^15. l sums the unrounded P. Weights below 2^-33 of the largest are lost, 2^17 of them are 2^-16 of the sum.
+// largest score so far, rounded to FP16: relative 2^-11 down to 2^-14, which is 2^-23 of the column's largest weight or less, and absolute 2^-25 (2^-34 of the largest)
+// below, where weights are lost from 2^-34 of the largest on; 2^17 tokens of such weights are 2^-17 of the sum. m' moves, and O and l are rescaled, only where a score
+// would pass 2^15. l sums the unrounded P.
 //
 // Channels and tokens are dealt to the fragments so that a lane's operands are whole words: for K lane (g, t) takes channels 32 t .. 32 t + 31 of its two
 // tokens (the order of the K extent of a product is free as long as Q has the same); for V it takes channels 16 g .. 16 g + 15 of four tokens, and two
@@ -16,18 +17,19 @@
 // Rows that several warps share are joined in shared memory, those that several CTAs share by the CTA that comes last (a counter per CTA), always in the
 // order of the tokens: the result does not depend on who that is.
 //
-// Bound by instructions beside the bytes: some 290 per block and tile of columns, of which a conversion and a scaling of every pair of codes are 128. Measured, 32 / 8 heads:
-// 64 requests of 1K-64K tokens 200 us = 4.6 TB/s (its loop alone 5.7, 0.87 of the copy rate; without the products and conversions 165 us); 131 072 tokens 42.7 us,
-// of which 28 are the loop, 6.5 what comes before (lengths, table, queries: five dependent reads) and 8 the joining; 4096 tokens 11 us on the device. Units of one block
-// instead of two: 227 us, 384 instructions per block. Twelve warps instead of sixteen: the same.
+// Bound by instructions beside the bytes: some 290 per block and tile of columns, of which a conversion and a scaling of every pair of codes are 128; no pipe is full
+// (issue 0.60 per cycle and scheduler, the ALU pipe 57 % active, shared memory 25 %), warps wait for results of a fixed time and for one another. On the device (a graph of
+// calls with a scratch of their own), 32 / 8 heads: 64 requests of 1K-64K tokens 176 us = 5.2 TB/s, 0.79 of the copy rate; 131 072 tokens 41 us, of which 28 are the
+// loop, 6.5 what comes before (lengths, table, queries: five dependent reads) and some 7 the joining; 4096 tokens 12 us. Without the products and conversions the 64
+// requests took 0.83 of the time, with units of one block instead of two (and rows shared out by 64-bit products) 1.18 times; twelve warps instead of sixteen: the same.
 #include "fbla_launch.h"
 #include "paged_attend.cuh"
 
 namespace paged {
 namespace {
 
-// One tile of columns: sixteen warps of 128 registers. Two: eight of 255; with twelve of 168 the registers do not hold a block's words (106 us for drafted tokens of 16
-// requests, against 102). Three do not pay: requests of 24 columns 123 us instead of 145, but of 16 columns 108 instead of 95 and of 32 168 instead of 146.
+// One tile of columns: sixteen warps of 128 registers (12 bytes of them spilled). Two: eight of 243; with twelve of 168 the registers do not hold a block's words (1.04 times
+// the time of drafted tokens of 16 requests). Three do not pay: requests of 24 columns take 0.85 of the time, but those of 16 columns 1.14 and of 32 1.15.
 template <int NT> constexpr int WARPS = NT == 1 ? 16 : 8;
 template <int NT> constexpr int STAGES = NT == 1 ? 2 : 3;
 constexpr int UNIT = 2 * BT;  // tokens of a unit

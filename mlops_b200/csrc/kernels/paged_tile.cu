@@ -8,15 +8,16 @@
 // Per tile of tokens and half X of the rows (128 each), with FP32 accumulators in tensor memory:
 //   S_X[128 x 128] = Q_X K^T,   O_X[128 x 128] += P_X V
 // K and V are code * scale, exact in FP16; Q is FP16 after a power of two per row (paged_attend.cuh); P = 2^(s - m') in FP16 takes S_X's place in tensor
-// memory. m' moves only where a score would pass 2^15, then O and l are rescaled; l sums the unrounded P. Rows of at most 128 use both halves too: the
-// even tiles of tokens go to X = 0, the odd ones to X = 1, with the same queries, and the halves are joined at the end.
+// memory, rounded as in paged_stream.cu. m' moves only where a score would pass 2^15, then O and l are rescaled; l sums the unrounded P. Rows of at most
+// 128 use both halves too: the even tiles of tokens go to X = 0, the odd ones to X = 1, with the same queries, and the halves are joined at the end.
 //
 // The exponentials of a tile take as long as its two products: 16 per cycle and SM, 2048 cycles for both X. Eight warps do those of X = 0 and then those of X = 1, so that
 // the tensor cores work for one X while the other one's softmax runs. A tile then takes the softmax of one X (1800 cycles, of which the exponentials are 1024) and the way
 // of the other from P to its next scores (2500: two products of 512 among the other X's, three hand-overs through barriers): 4300 cycles where the products alone are
-// 2048. Two prompts of 8192 tokens, 32 / 8 heads: 1.39 ms = 793 TFLOP/s, 0.49 of the measured burst rate. Tried: a thread per row and both X's softmax at once
+// 2048. Two prompts of 8192 tokens, 32 / 8 heads: 1.40 ms = 785 TFLOP/s, 0.48 of the measured burst rate. Tried: a thread per row and both X's softmax at once
 // (7600 cycles: both wait for the tensor cores together); a third of the exponentials as polynomials on the FMA units (1.07 times the time: packed FP32, maxima and
-// conversions share their issue slots); operand warps that look up their blocks themselves (the registers spill, and every load is waited for at once).
+// conversions share their issue slots); operand warps that look up their blocks themselves (the registers spill, and every load is waited for at once). The kernel
+// stores 56 bytes of registers per thread to local memory and loads 200.
 //
 // Warps 0-7 (two threads per row): softmax. Warps 8-15: operands, from packed pages to two stages each of K and V in shared
 // memory, token rows of 128 bytes (64 channels) with 16-byte chunk c of row r at c ^ (r % 8): for S that is K-major, for O V's MN-major. Warps 16, 17: one thread
