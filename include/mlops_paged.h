@@ -1,5 +1,6 @@
 /* A paged cache of K and V in 4 bits for NVIDIA B200 (sm_100a): pages and slots assigned on the device, quantise-on-write,
- * read-back, and attention over the pages. An addition of this library; the reference has no paged cache.
+ * also with a position's rotation on the way, read-back, and attention over the pages: causal, to states of another length, and of requests that begin alike. An addition of this
+ * library; the reference has no paged cache.
  *
  * Pool. Head dimension 128. A page holds page_size tokens (a multiple of 16) of every KV head; slot s of the pool is token
  * s % page_size of page s / page_size. The unit of (page, KV head) is page_size / 16 blocks of 2304 bytes, one after the
@@ -81,6 +82,27 @@ mlops_fbla_status mlops_paged_assign(const mlops_paged_assign_args *args, cudaSt
 mlops_fbla_status mlops_paged_append(const mlops_paged_cache *cache, int tokens, int type, const void *k, int64_t k_token_stride, int64_t k_head_stride,
                                      const void *v, int64_t v_token_stride, int64_t v_head_stride, const int *slots, cudaStream_t stream);
 
+/* A step's tokens as the projection leaves them: q and k rotated by the tokens' positions, q stored, k and v quantised into the slots as
+ * mlops_paged_append does. Rotation of a pair (x, y) of channels by position p: (x c - y s, y c + x s) with c = angles[p][i], s = angles[p][rotated / 2 + i]
+ * for pair i: channels (i, i + rotated / 2), or (2 i, 2 i + 1) where `interleaved`; channels from `rotated` on stay as they are. Rotated q is rounded once to the
+ * type (FP32 arithmetic); rotated k is the exact rotation rounded once to the type, so that the cache's bytes are those that mlops_paged_append stores of it.
+ * A token without a slot of the pool has its q rotated and is not stored. A token of a negative position (a row that is no request's) has zeros as its
+ * q and is not stored; one whose position is behind the table has NaN as its q, and its K is stored as NaN. q_out may be q with the same strides, and overlaps no other input
+ * or q. */
+typedef struct mlops_paged_rotate_args {
+  int tokens, q_heads, type;                /* q_heads: any number, 0 too */
+  int rotated, interleaved;                 /* rotated: 32, 64, 96 or 128; interleaved: 0 or 1 */
+  int reach;                                /* positions of the table */
+  const float *angles;                      /* [reach][rotated], angle_stride floats between rows (a multiple of 4), 16-byte aligned */
+  int64_t angle_stride;
+  const void *q, *k, *v;                    /* [tokens][heads][128], strides in elements: multiples of 8 */
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  void *q_out;
+  int64_t out_token_stride, out_head_stride;
+  const int *slots, *positions;             /* [tokens]; the slots of the pool are distinct */
+} mlops_paged_rotate_args;
+mlops_fbla_status mlops_paged_append_rotated(const mlops_paged_cache *cache, const mlops_paged_rotate_args *args, cudaStream_t stream);
+
 /* The values of `tokens` slots as [tokens][kv_heads][128], rounded once to `type`; zeros for a slot that is not one of the pool's. */
 mlops_fbla_status mlops_paged_read(const mlops_paged_cache *cache, int tokens, int type, const int *slots, void *k, void *v, cudaStream_t stream);
 
@@ -102,9 +124,29 @@ typedef struct mlops_paged_attend_args {
 size_t mlops_paged_attend_scratch_bytes(const mlops_paged_attend_args *args, int kv_heads);
 /* Rows of q that are no request's, before starts[0] and behind starts[batch], have zeros as their output and -infinity as their log-sum-exp:
  * a slice of a step's requests (table, lengths and starts from request b on) goes with all of the step's rows. Where starts[batch] is
- * above `tokens`, the rows that q does not have are left out and the others see what they would beside them. The scratch (16-byte aligned) is filled with zeros once, before its first call; what a
- * call leaves in it serves the next one, of whatever shape. Calls that overlap need scratches of their own. */
+ * above `tokens`, the rows that q does not have are left out and the others see what they would beside them. The first MLOPS_PAGED_SCRATCH_ZEROS bytes of the scratch (16-byte aligned; all of
+ * it where it is smaller) are filled with zeros once, before its first call; what a call leaves in it serves the next one, of whatever shape. Calls that overlap need scratches of
+ * their own. */
+#define MLOPS_PAGED_SCRATCH_ZEROS 8192
 mlops_fbla_status mlops_paged_attend(const mlops_paged_attend_args *args, const mlops_paged_cache *cache, void *scratch, size_t scratch_bytes, cudaStream_t stream);
+
+/* Cross attention: as mlops_paged_attend, but every query of a request sees all of the request's lengths[b] tokens (the states of an encoder; queries may outnumber them, as those of
+ * several beams do). Scratch: mlops_paged_attend_scratch_bytes; one that serves mlops_paged_attend serves this too. */
+mlops_fbla_status mlops_paged_cross_attend(const mlops_paged_attend_args *args, const mlops_paged_cache *cache, void *scratch, size_t scratch_bytes, cudaStream_t stream);
+
+/* Requests that begin with the same tokens: group g is the requests starts[g] .. starts[g + 1] - 1 (ascending; requests of no group share nothing), whose first tokens[g] tokens
+ * are the same. Of these whole pages count, and these pages' entries in the table's rows of the group's requests are the same (those of any one of them may be read for all).
+ * Both arrays live on the device. */
+typedef struct mlops_paged_common {
+  int groups;                          /* batch + groups at most 2048 */
+  const int *starts;                   /* [groups + 1], or null: all requests are one group (groups 1) */
+  const int *tokens;                   /* [groups] */
+} mlops_paged_common;
+/* What mlops_paged_attend gives, within rounding; the pages that a group's requests have in common are read once for all of them. A request whose first query does not see all of the
+ * common tokens is attended by itself. The scratch is mlops_paged_attend's with 1056 bytes more per row of q and query head. */
+size_t mlops_paged_attend_shared_scratch_bytes(const mlops_paged_attend_args *args, const mlops_paged_common *common, int kv_heads);
+mlops_fbla_status mlops_paged_attend_shared(const mlops_paged_attend_args *args, const mlops_paged_common *common, const mlops_paged_cache *cache, void *scratch, size_t scratch_bytes,
+                                            cudaStream_t stream);
 
 const char *mlops_paged_last_error(void);
 

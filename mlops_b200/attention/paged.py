@@ -1,5 +1,6 @@
 """A paged cache of K and V in 4 bits (C interface: include/mlops_paged.h): pages and slots for a step's new tokens (`assign`), quantise-on-write
-(`append`), read-back (`read`) and attention over the pages (`attend`).
+(`append`; `append_rotated` with the positions' rotation on the way), read-back (`read`) and attention over the pages: causal (`attend`), of requests that begin with the same tokens
+(`attend_shared`), and to states of another length, an encoder's for instance (`cross_attend`).
 
 An engine keeps, on the GPU, one pool per layer (`empty`), one block table ``int32 [batch, width]`` for all layers, the requests' lengths, and a ring
 of free page numbers with its two ends. A step of one layer:
@@ -48,6 +49,20 @@ class _Attend(ctypes.Structure):
                 ("width", ctypes.c_int), ("lengths", ctypes.c_void_p), ("starts", ctypes.c_void_p), ("scale", ctypes.c_float)]
 
 
+class _Rotate(ctypes.Structure):
+    """mlops_paged_rotate_args"""
+    _fields_ = [("tokens", ctypes.c_int), ("q_heads", ctypes.c_int), ("type", ctypes.c_int), ("rotated", ctypes.c_int), ("interleaved", ctypes.c_int), ("reach", ctypes.c_int),
+                ("angles", ctypes.c_void_p), ("angle_stride", ctypes.c_int64), ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("q_token_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64), ("k_token_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64),
+                ("v_token_stride", ctypes.c_int64), ("v_head_stride", ctypes.c_int64), ("q_out", ctypes.c_void_p), ("out_token_stride", ctypes.c_int64),
+                ("out_head_stride", ctypes.c_int64), ("slots", ctypes.c_void_p), ("positions", ctypes.c_void_p)]
+
+
+class _Common(ctypes.Structure):
+    """mlops_paged_common"""
+    _fields_ = [("groups", ctypes.c_int), ("starts", ctypes.c_void_p), ("tokens", ctypes.c_void_p)]
+
+
 _lib, _vp, _int, _i64 = _C._lib, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64
 _lib.mlops_paged_assign.argtypes = [_vp, _vp]
 _lib.mlops_paged_append.argtypes = [_vp, _int, _int, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp]
@@ -55,12 +70,26 @@ _lib.mlops_paged_read.argtypes = [_vp, _int, _int, _vp, _vp, _vp, _vp]
 _lib.mlops_paged_attend.argtypes = [_vp, _vp, _vp, ctypes.c_size_t, _vp]
 _lib.mlops_paged_attend_scratch_bytes.argtypes = [_vp, _int]
 _lib.mlops_paged_attend_scratch_bytes.restype = ctypes.c_size_t
+_lib.mlops_paged_append_rotated.argtypes = [_vp, _vp, _vp]
+_lib.mlops_paged_cross_attend.argtypes = [_vp, _vp, _vp, ctypes.c_size_t, _vp]
+_lib.mlops_paged_attend_shared.argtypes = [_vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]
+_lib.mlops_paged_attend_shared_scratch_bytes.argtypes = [_vp, _vp, _int]
+_lib.mlops_paged_attend_shared_scratch_bytes.restype = ctypes.c_size_t
 _lib.mlops_paged_last_error.restype = ctypes.c_char_p
 # the structures as the calls below pass them: their bytes (a third of the host's time that ctypes takes to fill one; addresses of 0 are null)
 _CACHE, _ASSIGN, _ATTEND = struct.Struct("@PPPqqiii4x"), struct.Struct("@iiiiqPPPPiPPPPPP"), struct.Struct("@iiiiPqqPqqPPqiPPf4x")
-assert (_CACHE.size, _ASSIGN.size, _ATTEND.size) == (ctypes.sizeof(_Cache), ctypes.sizeof(_Assign), ctypes.sizeof(_Attend))
+_ROTATE, _COMMON = struct.Struct("@iiiiiiPqPPPqqqqqqPqqPP"), struct.Struct("@i4xPP")
+assert [x.size for x in (_CACHE, _ASSIGN, _ATTEND, _ROTATE, _COMMON)] == [ctypes.sizeof(x) for x in (_Cache, _Assign, _Attend, _Rotate, _Common)]
 
-_scratch = _C._ScratchPool(torch.zeros)  # (zeros at first; every call leaves its counters as it found them)
+
+def _with_zeros(shape, **kind):
+    """a scratch: MLOPS_PAGED_SCRATCH_ZEROS zeros in front (every call leaves its counters as it found them)"""
+    buffer = torch.empty(shape, **kind)
+    buffer[:8192].zero_()
+    return buffer
+
+
+_scratch = _C._ScratchPool(_with_zeros)
 
 
 def _raise(status, what):
@@ -212,6 +241,36 @@ def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Ten
     return cache
 
 
+def append_rotated(cache: PagedCache, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, *,
+                   interleaved: bool = False) -> torch.Tensor:
+    """Rotate ``q [tokens, q_heads, 128]`` and ``k [tokens, kv_heads, 128]`` by the tokens' ``positions`` (int32 [tokens]) and quantise k and ``v`` into the pool's ``slots`` as `append`
+    does; returns the rotated q, ``[tokens, q_heads, 128]`` of q's type.
+
+    ``cos_sin``: float32 [n, R], row p the R / 2 cosines and then the R / 2 sines of position p, R one of 32, 64, 96, 128. Pair i of the first R channels (x, y) becomes
+    (x cos - y sin, y cos + x sin); pairs are (i, i + R / 2), with ``interleaved`` (2 i, 2 i + 1); the channels behind R stay as they are. Rotated k is rounded once to its type before
+    it is quantised. A token without a slot of the pool has its q rotated and is not stored; one of a negative position (`assign`'s rows of no request) has zeros as its q and is not
+    stored; one whose position is not below n has NaN as its q and as the K that is stored."""
+    pool, heads, index = _pool(cache)
+    if not _on(index):
+        with torch.cuda.device(index):
+            return append_rotated(cache, q, k, v, slots, positions, cos_sin, interleaved=interleaved)
+    q, (tokens, q_heads, _), q_by_token, q_by_head, kind = _rows(q, index, "q")
+    k, k_shape, k_by_token, k_by_head, k_kind = _rows(k, index, "k", heads)
+    v, v_shape, v_by_token, v_by_head, v_kind = _rows(v, index, "v", heads)
+    if not (k_shape[0] == v_shape[0] == tokens and k_kind == v_kind == kind):
+        raise ValueError(f"q, k and v have to be alike; q is {q.dtype} {tuple(q.shape)}, k is {k.dtype} {tuple(k.shape)}, v is {v.dtype} {tuple(v.shape)}")
+    shape, strides = cos_sin.shape, cos_sin.stride()
+    if cos_sin.get_device() != index or cos_sin.dtype is not _F32 or len(shape) != 2 or strides[1] != 1 or (strides[0] % 4 and shape[0] > 1) or cos_sin.data_ptr() % 16:
+        raise ValueError(f"cos_sin: expected a float32 [positions, rotated] tensor with dense rows on 16-byte boundaries on cuda:{index}; it is {cos_sin.dtype} {tuple(shape)}, strides {strides}, on {cos_sin.device}")
+    out = torch.empty((tokens, q_heads, HEAD_DIM), dtype=q.dtype, device=q.device)
+    status = _lib.mlops_paged_append_rotated(pool, _ROTATE.pack(tokens, q_heads, kind, shape[1], 1 if interleaved else 0, shape[0], cos_sin.data_ptr(), strides[0] if shape[0] > 1 else shape[1], q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                                                q_by_token, q_by_head, k_by_token, k_by_head, v_by_token, v_by_head, out.data_ptr(), q_heads * HEAD_DIM, HEAD_DIM,
+                                                                _ints(slots, index, "slots", tokens), _ints(positions, index, "positions", tokens)), _C._raw_stream(index))
+    if status:
+        _raise(status, "mlops_paged_append_rotated")
+    return out
+
+
 def read(cache: PagedCache, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
     """What the pool holds in ``slots`` (int32 [tokens]): K and V as ``[tokens, kv_heads, 128]``, rounded once to ``dtype`` (BF16 or FP16). Zeros for a
     slot outside the pool."""
@@ -240,10 +299,31 @@ def attend(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, lengths: tor
     query per request. Row i of n sees the request's tokens up to ``lengths[b] - n + i``. Returns ``[tokens, q_heads, 128]`` of q's type, zeros for a
     row that sees nothing and for rows of no request, before ``starts[0]`` and behind ``starts[batch]``; with ``return_lse`` also the natural log-sum-exp of the rows' scaled scores, float32
     [tokens, q_heads] (-inf for such rows). ``scale`` 0 selects 1/sqrt(128)."""
+    return _attention("mlops_paged_attend", q, cache, table, lengths, starts, scale, return_lse)
+
+
+def cross_attend(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor] = None, *, scale: float = 0.0,
+                 return_lse: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """Cross attention: as `attend`, but every query of request b sees all ``lengths[b]`` tokens that the request has in the pool, for instance the states of its encoder, which
+    `append` has stored. The queries' own tokens are elsewhere; there may be more of them than states (several beams of a request are rows of one request)."""
+    return _attention("mlops_paged_cross_attend", q, cache, table, lengths, starts, scale, return_lse)
+
+
+def attend_shared(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor], groups: Optional[torch.Tensor], shared: torch.Tensor, *,
+                  scale: float = 0.0, return_lse: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """What `attend` gives, for requests that begin with the same tokens: the pages that they have in common are read once for all of them.
+
+    Group g is the requests ``groups[g] .. groups[g + 1] - 1`` (``groups`` int32 [n + 1], ascending; None: all requests are one group); their first ``shared[g]`` tokens are the same
+    (``shared`` int32 [n]). Of these whole pages count, and the requests' rows of ``table`` name the same pages for them; ``lengths`` and positions count the common tokens like
+    the others. A request whose first query does not see all of the common tokens is attended by itself, as are requests of no group."""
+    return _attention("mlops_paged_attend_shared", q, cache, table, lengths, starts, scale, return_lse, groups, shared)
+
+
+def _attention(name, q, cache, table, lengths, starts, scale, return_lse, groups=None, shared=None):
     pool, kv_heads, index = _pool(cache)
     if not _on(index):
         with torch.cuda.device(index):
-            return attend(q, cache, table, lengths, starts, scale=scale, return_lse=return_lse)
+            return _attention(name, q, cache, table, lengths, starts, scale, return_lse, groups, shared)
     q, (tokens, heads, _), by_token, by_head, kind = _rows(q, index, "q")
     entries, stride, batch, width = _table(table, index)
     where = _ints(lengths, index, "lengths", batch)
@@ -253,9 +333,15 @@ def attend(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, lengths: tor
     call = _ATTEND.pack(batch, tokens, heads, kind, q.data_ptr(), by_token, by_head, out.data_ptr(), heads * HEAD_DIM, HEAD_DIM, lse.data_ptr() if return_lse else 0,
                         entries, stride, width, where, begins, scale)
     stream = _C._raw_stream(index)
-    scratch = _scratch.get(q.device, stream, max(16, _lib.mlops_paged_attend_scratch_bytes(call, kv_heads)))
-    with scratch.lock:
-        status = _lib.mlops_paged_attend(call, pool, scratch.pointer, scratch.bytes, stream)
+    if shared is None:
+        scratch = _scratch.get(q.device, stream, max(16, _lib.mlops_paged_attend_scratch_bytes(call, kv_heads)))
+        with scratch.lock:
+            status = getattr(_lib, name)(call, pool, scratch.pointer, scratch.bytes, stream)
+    else:
+        common = _COMMON.pack(shared.size(0), 0 if groups is None else _ints(groups, index, "groups", shared.size(0) + 1), _ints(shared, index, "shared", 1 if groups is None else None))
+        scratch = _scratch.get(q.device, stream, max(16, _lib.mlops_paged_attend_shared_scratch_bytes(call, common, kv_heads)))
+        with scratch.lock:
+            status = _lib.mlops_paged_attend_shared(call, common, pool, scratch.pointer, scratch.bytes, stream)
     if status:
-        _raise(status, "mlops_paged_attend")
+        _raise(status, name)
     return (out, lse) if return_lse else out

@@ -65,8 +65,43 @@ cudaError_t processors(int *sms) {
     return cudaSuccess;
   }
   e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e == cudaSuccess && *sms > PAGED_K_MAX_SMS) *sms = PAGED_K_MAX_SMS;  // (a grid is as many CTAs; their counters fit what is zeros)
   if (e == cudaSuccess && dev < 64) known[dev] = *sms;
   return e;
+}
+
+bool common_acceptable(const mlops_paged_attend_args *a, const mlops_paged_common *common) {
+  return common->groups >= 1 && (common->starts || common->groups == 1) && common->groups <= PAGED_K_MAX_ATTENDED - a->batch;
+}
+
+// checks and enqueues one of the three attentions; common: mlops_paged_attend_shared's
+mlops_fbla_status attention(const char *fn, const mlops_paged_attend_args *a, const mlops_paged_common *common, bool whole, const mlops_paged_cache *c, void *scratch, size_t scratch_bytes,
+                            cudaStream_t stream) {
+  if (const char *why = cache_fault(c)) return refuse(fn, "%s", why);
+  if (!attend_shape_acceptable(a, c->kv_heads))
+    return refuse(fn, "needs batch in 0..%d, tokens >= 0, q_heads that kv_heads divides and fewer than 2^31 rows", PAGED_K_MAX_ATTENDED);
+  if (common && !common_acceptable(a, common)) return refuse(fn, "needs groups >= 1, one without group starts, and batch + groups up to %d", PAGED_K_MAX_ATTENDED);
+  if (!known_type(a->type)) return refuse(fn, "type %d is neither MLOPS_PAGED_BF16 nor MLOPS_PAGED_FP16", a->type);
+  if (!(a->scale >= 0.f) || std::isinf(a->scale)) return refuse(fn, "scale has to be a number that is not negative");
+  if (!a->starts && a->tokens != a->batch) return refuse(fn, "without starts there is one query per request, but there are %d for %d", a->tokens, a->batch);
+  if (a->tokens == 0) return nothing_to_do();
+  if (a->width < 0 || a->table_stride < a->width) return refuse(fn, "the table's stride has to be at least its width, and that not negative");
+  if (a->width > 0 && ((int64_t)a->batch + (common ? common->groups : 0)) * c->kv_heads > INT32_MAX / (4 * (((int64_t)a->width * c->page_size + 31) / 32)))
+    return refuse(fn, "batch * kv_heads * width * page_size is more than a call takes: split the batch");
+  if (!a->q || !a->out || !scratch || (a->batch > 0 && !a->lengths) || (a->batch > 0 && a->width > 0 && !a->table) || (common && !common->tokens)) return refuse(fn, "a required pointer is null");
+  if (!rows_usable(a->q, a->q_token_stride, a->q_head_stride) || !rows_usable(a->out, a->out_token_stride, a->out_head_stride) || !aligned(scratch, 16))
+    return refuse(fn, "q, out and scratch have to start on 16-byte boundaries, q and out with strides that are multiples of 8 elements");
+  if (!aligned(a->lengths, 4) || !aligned(a->starts, 4) || !aligned(a->table, 4) || !aligned(a->lse, 4) || (common && (!aligned(common->starts, 4) || !aligned(common->tokens, 4))))
+    return refuse(fn, "arrays of int and float have to start on 4-byte boundaries");
+  int sms = 0;
+  const cudaError_t e = scratch_bytes < 16 ? cudaSuccess : processors(&sms);
+  if (e != cudaSuccess) return ended(fn, e);
+  if (scratch_bytes < 16 || scratch_bytes < paged_k_attend_scratch(a, c->kv_heads, common != nullptr, sms))
+    return refuse(fn, "the scratch is %zu bytes, which are too few for this call", scratch_bytes);
+  mlops_paged_attend_args call = *a;
+  if (call.scale == 0.f) call.scale = 1.f / std::sqrt((float)MLOPS_PAGED_HEAD_DIM);
+  return ended(fn, common ? paged_k_attend_shared_launch(&call, common, c, scratch, sms, stream)
+                          : whole ? paged_k_cross_attend_launch(&call, c, scratch, sms, stream) : paged_k_attend_launch(&call, c, scratch, sms, stream));
 }
 
 }  // namespace
@@ -105,6 +140,26 @@ mlops_fbla_status mlops_paged_append(const mlops_paged_cache *c, int tokens, int
   return ended(fn, e != cudaSuccess ? e : paged_k_append_launch(c, tokens, type, k, k_ts, k_hs, v, v_ts, v_hs, slots, sms, stream));
 }
 
+mlops_fbla_status mlops_paged_append_rotated(const mlops_paged_cache *c, const mlops_paged_rotate_args *a, cudaStream_t stream) {
+  const char *const fn = "mlops_paged_append_rotated";
+  if (const char *why = cache_fault(c)) return refuse(fn, "%s", why);
+  if (!a || a->tokens < 0 || a->q_heads < 0 || a->reach < 0 || !known_type(a->type)) return refuse(fn, "needs tokens, q_heads, reach >= 0 and a type of MLOPS_PAGED_BF16 or MLOPS_PAGED_FP16");
+  if (a->rotated <= 0 || a->rotated > MLOPS_PAGED_HEAD_DIM || a->rotated % 32 || a->interleaved < 0 || a->interleaved > 1)
+    return refuse(fn, "%d channels can not be rotated: 32, 64, 96 or 128 can, in halves (interleaved 0) or as neighbours (1)", a->rotated);
+  if ((int64_t)a->tokens * ((int64_t)a->q_heads + c->kv_heads) > INT32_MAX) return refuse(fn, "tokens * heads has to be below 2^31: split the tokens");
+  if (a->tokens == 0) return nothing_to_do();
+  if (!a->k || !a->v || !a->slots || !a->positions || (a->reach > 0 && !a->angles) || (a->q_heads > 0 && (!a->q || !a->q_out))) return refuse(fn, "a required pointer is null");
+  if ((a->q_heads > 0 && (!rows_usable(a->q, a->q_token_stride, a->q_head_stride) || !rows_usable(a->q_out, a->out_token_stride, a->out_head_stride))) ||
+      !rows_usable(a->k, a->k_token_stride, a->k_head_stride) || !rows_usable(a->v, a->v_token_stride, a->v_head_stride))
+    return refuse(fn, "q, k, v and q_out have to start on 16-byte boundaries and have strides that are multiples of 8 elements");
+  if (!aligned(a->angles, 16) || a->angle_stride % 4 || (a->reach > 1 && a->angle_stride < a->rotated))
+    return refuse(fn, "angles has to start on a 16-byte boundary, with a stride that is a multiple of 4 and at least the channels that are rotated");
+  if (!aligned(a->slots, 4) || !aligned(a->positions, 4)) return refuse(fn, "arrays of int have to start on 4-byte boundaries");
+  int sms = 0;
+  const cudaError_t e = processors(&sms);
+  return ended(fn, e != cudaSuccess ? e : paged_k_append_rotated_launch(c, a, sms, stream));
+}
+
 mlops_fbla_status mlops_paged_read(const mlops_paged_cache *c, int tokens, int type, const int *slots, void *k, void *v, cudaStream_t stream) {
   const char *const fn = "mlops_paged_read";
   if (const char *why = cache_fault(c)) return refuse(fn, "%s", why);
@@ -120,32 +175,27 @@ mlops_fbla_status mlops_paged_read(const mlops_paged_cache *c, int tokens, int t
 
 size_t mlops_paged_attend_scratch_bytes(const mlops_paged_attend_args *a, int kv_heads) {
   int sms = 0;
-  return attend_shape_acceptable(a, kv_heads) && processors(&sms) == cudaSuccess ? paged_k_attend_scratch(a, kv_heads, sms) : 0;
+  return attend_shape_acceptable(a, kv_heads) && processors(&sms) == cudaSuccess ? paged_k_attend_scratch(a, kv_heads, 0, sms) : 0;
 }
 
 mlops_fbla_status mlops_paged_attend(const mlops_paged_attend_args *a, const mlops_paged_cache *c, void *scratch, size_t scratch_bytes, cudaStream_t stream) {
-  const char *const fn = "mlops_paged_attend";
-  if (const char *why = cache_fault(c)) return refuse(fn, "%s", why);
-  if (!attend_shape_acceptable(a, c->kv_heads))
-    return refuse(fn, "needs batch in 0..%d, tokens >= 0, q_heads that kv_heads divides and fewer than 2^31 rows", PAGED_K_MAX_ATTENDED);
-  if (!known_type(a->type)) return refuse(fn, "type %d is neither MLOPS_PAGED_BF16 nor MLOPS_PAGED_FP16", a->type);
-  if (!(a->scale >= 0.f) || std::isinf(a->scale)) return refuse(fn, "scale has to be a number that is not negative");
-  if (!a->starts && a->tokens != a->batch) return refuse(fn, "without starts there is one query per request, but there are %d for %d", a->tokens, a->batch);
-  if (a->tokens == 0) return nothing_to_do();
-  if (a->width < 0 || a->table_stride < a->width) return refuse(fn, "the table's stride has to be at least its width, and that not negative");
-  if (a->width > 0 && (int64_t)a->batch * c->kv_heads > INT32_MAX / (4 * (((int64_t)a->width * c->page_size + 31) / 32)))
-    return refuse(fn, "batch * kv_heads * width * page_size is more than a call takes: split the batch");
-  if (!a->q || !a->out || !scratch || (a->batch > 0 && !a->lengths) || (a->batch > 0 && a->width > 0 && !a->table)) return refuse(fn, "a required pointer is null");
-  if (!rows_usable(a->q, a->q_token_stride, a->q_head_stride) || !rows_usable(a->out, a->out_token_stride, a->out_head_stride) || !aligned(scratch, 16))
-    return refuse(fn, "q, out and scratch have to start on 16-byte boundaries, q and out with strides that are multiples of 8 elements");
-  if (!aligned(a->lengths, 4) || !aligned(a->starts, 4) || !aligned(a->table, 4) || !aligned(a->lse, 4)) return refuse(fn, "arrays of int and float have to start on 4-byte boundaries");
+  return attention("mlops_paged_attend", a, nullptr, false, c, scratch, scratch_bytes, stream);
+}
+
+mlops_fbla_status mlops_paged_cross_attend(const mlops_paged_attend_args *a, const mlops_paged_cache *c, void *scratch, size_t scratch_bytes, cudaStream_t stream) {
+  return attention("mlops_paged_cross_attend", a, nullptr, true, c, scratch, scratch_bytes, stream);
+}
+
+size_t mlops_paged_attend_shared_scratch_bytes(const mlops_paged_attend_args *a, const mlops_paged_common *common, int kv_heads) {
   int sms = 0;
-  const cudaError_t e = scratch_bytes < 16 ? cudaSuccess : processors(&sms);
-  if (e != cudaSuccess) return ended(fn, e);
-  if (scratch_bytes < 16 || scratch_bytes < paged_k_attend_scratch(a, c->kv_heads, sms)) return refuse(fn, "the scratch is %zu bytes, which are too few for this call", scratch_bytes);
-  mlops_paged_attend_args call = *a;
-  if (call.scale == 0.f) call.scale = 1.f / std::sqrt((float)MLOPS_PAGED_HEAD_DIM);
-  return ended(fn, paged_k_attend_launch(&call, c, scratch, sms, stream));
+  return attend_shape_acceptable(a, kv_heads) && common && common_acceptable(a, common) && processors(&sms) == cudaSuccess ? paged_k_attend_scratch(a, kv_heads, 1, sms) : 0;
+}
+
+mlops_fbla_status mlops_paged_attend_shared(const mlops_paged_attend_args *a, const mlops_paged_common *common, const mlops_paged_cache *c, void *scratch, size_t scratch_bytes,
+                                            cudaStream_t stream) {
+  const char *const fn = "mlops_paged_attend_shared";
+  if (!common) return refuse(fn, "the groups are null");
+  return attention(fn, a, common, false, c, scratch, scratch_bytes, stream);
 }
 
 const char *mlops_paged_last_error(void) { return g_message; }

@@ -10,6 +10,10 @@ constexpr int PSTRIDE = 132;           // floats of a partial row: o[128], m, l,
 constexpr float NOTHING = -3e38f;      // the running maximum before the first score: finite, so that no difference of maxima is NaN
 constexpr float LN2 = 0.6931471805599453f;
 
+// What a query sees: its request's tokens up to its own (mlops_paged_attend), all of its request's (mlops_paged_cross_attend), or as the first with the tokens that
+// groups of requests have in common taken apart (mlops_paged_attend_shared)
+enum { CAUSAL, WHOLE, SHARED };
+
 struct Call {
   mlops_paged_attend_args a;
   mlops_paged_cache c;
@@ -19,6 +23,9 @@ struct Call {
   int wide;        // requests with more than so many columns (queries times group) are the tile kernel's
   float *stream_part, *tile_part;          // partial rows, see the kernels
   int *stream_counters, *tile_counters;    // one per CTA, zeros before and after every call
+  // SHARED: the groups, and the sums (o[128], m, l, whether the common row counts) of every row of q and head over common and own tokens
+  mlops_paged_common common;
+  float *common_rows, *own_rows;
 };
 
 // a column's query and its query head among the KV head's: column / group, column % group
@@ -28,13 +35,26 @@ __device__ __forceinline__ void split_column(const Call &k, int column, int &que
   head = column - query * k.group;
 }
 
-// request b's queries and tokens, as far as q's rows and the table's width go. Rows that q does not have move no other: row i is the request's token
+// An item of a call is a request; SHARED: a group's common tokens (items 0 .. groups - 1), then the requests with their own.
+template <int MODE> __device__ __forceinline__ int items_of(const Call &k) { return MODE == SHARED ? k.common.groups + k.a.batch : k.a.batch; }
+
+// an item's queries and tokens, as far as q's rows and the table's width go. Rows that q does not have move no other: row i of request b is its token
 // lengths[b] - starts[b + 1] + i.
-struct Request {
-  int start, n, at, tokens;  // first row of q, queries, the first one's token (negative: before the request), tokens that a table row can name
+struct Plain {
+  int start, n, at, tokens;  // first row of q, queries, the first one's token (negative: before the item's), tokens that a table row can name
 };
-__device__ __forceinline__ Request request(const Call &k, int b) {
-  Request r;
+struct Apart {
+  int start, n, at, tokens;
+  int row, skip;  // row of the table; the item's first token in it
+  bool common;    // a group's: all of them are seen by all
+  __device__ __forceinline__ operator Plain() const { return Plain{start, n, at, tokens}; }
+};
+template <int MODE> struct RequestOf { using type = Plain; };
+template <> struct RequestOf<SHARED> { using type = Apart; };
+template <int MODE> using Request = typename RequestOf<MODE>::type;
+
+__device__ __forceinline__ Plain plain_request(const Call &k, int b) {
+  Plain r;
   int e = b + 1;
   if (k.a.starts) {
     const int s = __ldg(k.a.starts + b);
@@ -50,6 +70,84 @@ __device__ __forceinline__ Request request(const Call &k, int b) {
   r.tokens = (int)min((long long)length, (long long)k.a.width * k.c.page_size);
   return r;
 }
+// group g's requests, and their common tokens: whole pages of the table, none for a single request. (Whether a request's first query sees them all, so that it takes
+// part, is asked for each.)
+struct Group {
+  int first, end, tokens;
+};
+__device__ __forceinline__ Group group_at(const Call &k, int g) {
+  Group x{0, k.a.batch, 0};
+  if (k.common.starts) {
+    x.first = min(max(__ldg(k.common.starts + g), 0), k.a.batch);
+    x.end = min(max(__ldg(k.common.starts + g + 1), x.first), k.a.batch);
+  }
+  if (x.end - x.first > 1) {
+    const int pages = max(__ldg(k.common.tokens + g), 0) / k.c.page_size;
+    if (pages <= k.a.width) x.tokens = pages * k.c.page_size;  // (no request has more than its row of the table can name)
+  }
+  return x;
+}
+__device__ __forceinline__ bool takes_part(const Plain &r, int tokens) { return r.n > 0 && tokens > 0 && r.at >= tokens - 1; }
+
+template <int MODE> __device__ __forceinline__ Request<MODE> request(const Call &k, int item) {
+  Request<MODE> r;
+  if constexpr (MODE != SHARED) {
+    r = plain_request(k, item);
+    if (MODE == WHOLE) r.at = max(__ldg(k.a.lengths + item), 0) - 1;
+  } else if (item < k.common.groups) {
+    const Group x = group_at(k, item);
+    r.row = 0;
+    r.start = r.n = r.skip = r.tokens = 0;
+    r.at = -1;
+    r.common = true;
+    for (int b = x.first; b < x.end && x.tokens > 0; ++b) {
+      if (!takes_part(plain_request(k, b), x.tokens)) continue;
+      // (the rows of requests that do not take part are computed with the others' and not used)
+      r.row = b;
+      r.tokens = x.tokens;
+      r.at = x.tokens - 1;
+      r.start = k.a.starts ? min(max(__ldg(k.a.starts + x.first), 0), k.a.tokens) : x.first;
+      r.n = max((k.a.starts ? min(__ldg(k.a.starts + x.end), k.a.tokens) : x.end) - r.start, 0);
+      break;
+    }
+  } else {
+    const int b = item - k.common.groups;
+    const Plain p = plain_request(k, b);
+    r.start = p.start;
+    r.n = p.n;
+    r.at = p.at;
+    r.tokens = p.tokens;
+    r.row = b;
+    r.skip = 0;
+    r.common = false;
+    int g = 0;
+    if (k.common.starts)
+      for (int e = k.common.groups; e - g > 1;) {
+        const int mid = (g + e) >> 1;
+        if (__ldg(k.common.starts + mid) <= b) g = mid; else e = mid;
+      }
+    const Group x = group_at(k, g);
+    if (b >= x.first && b < x.end && takes_part(r, x.tokens)) {
+      r.skip = x.tokens;
+      r.at -= x.tokens;
+      r.tokens -= x.tokens;
+    }
+  }
+  return r;
+}
+// the last of the item's tokens that its query sees
+template <int MODE> __device__ __forceinline__ int limit_of(const Request<MODE> &r, int query) {
+  if constexpr (MODE == SHARED) return r.common ? r.at : r.at + query;
+  else return MODE == WHOLE ? r.at : r.at + query;
+}
+template <int MODE> __device__ __forceinline__ const int *table_row(const Call &k, const Request<MODE> &r, int item) {
+  if constexpr (MODE == SHARED) return k.a.table + (size_t)r.row * k.a.table_stride;
+  else return k.a.table + (size_t)item * k.a.table_stride;
+}
+template <int MODE> __device__ __forceinline__ int first_token(const Request<MODE> &r) {
+  if constexpr (MODE == SHARED) return r.skip;
+  else return 0;
+}
 
 // a row of the output in 16 bits: eight channels from ch on
 template <int TYPE> __device__ __forceinline__ uint4 pack8(const float4 &x, const float4 &y) {
@@ -61,17 +159,35 @@ __device__ __forceinline__ uint16_t *out_row(const Call &k, int row, int head) {
 // the log-sum-exp of a row with running maximum m (log2 units) and sum l
 __device__ __forceinline__ float lse_of(float m, float l) { return l == 0.f ? -FBLA_INF : (m + lg2(l)) * LN2; }
 
-// zeros (and -infinity) for q's row `row`, by one warp
-__device__ __forceinline__ void clear_row(const Call &k, int row, int lane) {
-  for (int i = lane; i < k.a.q_heads * 16; i += 32) reinterpret_cast<uint4 *>(out_row(k, row, i >> 4))[i & 15] = make_uint4(0, 0, 0, 0);
-  if (k.a.lse)
-    for (int i = lane; i < k.a.q_heads; i += 32) k.a.lse[(size_t)row * k.a.q_heads + i] = -FBLA_INF;
+// SHARED: where the sums of q's row `row` and query head `head` go, by the item
+__device__ __forceinline__ float *sums_row(const Call &k, bool common, int row, int head) {
+  return (common ? k.common_rows : k.own_rows) + ((size_t)row * k.a.q_heads + head) * PSTRIDE;
+}
+// what stands behind them: m (anything where l is 0), l, whether the common row counts too
+__device__ __forceinline__ float4 sums_end(const Apart &r, float m, float l) { return make_float4(m, l, r.skip > 0 ? 1.f : 0.f, 0.f); }
+
+// zeros (and -infinity) for q's row `row`, by one warp; SHARED: no sums, for the item r or for no request (skip 0)
+template <int MODE> __device__ __forceinline__ void clear_row(const Call &k, const Request<MODE> &r, int row, int lane) {
+  if constexpr (MODE == SHARED) {
+    for (int i = lane; i < k.a.q_heads; i += 32) *reinterpret_cast<float4 *>(sums_row(k, false, row, i) + D) = sums_end(r, NOTHING, 0.f);
+  } else {
+    for (int i = lane; i < k.a.q_heads * 16; i += 32) reinterpret_cast<uint4 *>(out_row(k, row, i >> 4))[i & 15] = make_uint4(0, 0, 0, 0);
+    if (k.a.lse)
+      for (int i = lane; i < k.a.q_heads; i += 32) k.a.lse[(size_t)row * k.a.q_heads + i] = -FBLA_INF;
+  }
 }
 
-template <int TYPE> __device__ __forceinline__ void store_joined(const Call &k, int row, int kv_head, int head, int x, const float4 &o, float m, float l) {
-  const float f = l == 0.f ? 0.f : __ldg(k.c.v_scale + kv_head) / l;
-  *reinterpret_cast<uint2 *>(out_row(k, row, head) + 4 * x) = make_uint2(from_floats<TYPE>(o.x * f, o.y * f), from_floats<TYPE>(o.z * f, o.w * f));
-  if (k.a.lse && x == 0) k.a.lse[(size_t)row * k.a.q_heads + head] = lse_of(m, l);
+template <int TYPE, int MODE>
+__device__ __forceinline__ void store_joined(const Call &k, const Request<MODE> &r, int row, int kv_head, int head, int x, const float4 &o, float m, float l) {
+  if constexpr (MODE == SHARED) {
+    float *const to = sums_row(k, r.common, row, head);
+    reinterpret_cast<float4 *>(to)[x] = l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : o;
+    if (x == 0) *reinterpret_cast<float4 *>(to + D) = sums_end(r, m, l);
+  } else {
+    const float f = l == 0.f ? 0.f : __ldg(k.c.v_scale + kv_head) / l;
+    *reinterpret_cast<uint2 *>(out_row(k, row, head) + 4 * x) = make_uint2(from_floats<TYPE>(o.x * f, o.y * f), from_floats<TYPE>(o.z * f, o.w * f));
+    if (k.a.lse && x == 0) k.a.lse[(size_t)row * k.a.q_heads + head] = lse_of(m, l);
+  }
 }
 
 // the power of two that puts a query's largest element (its bits: `top`) into [2^8, 2^9), and its inverse; 1 where that is infinite or NaN. As FP16
@@ -92,7 +208,9 @@ template <class K> cudaError_t allow_shared(K *kernel, bool (&ready)[64]) {
   return e;
 }
 // 8 NT: columns of a row of work
-template <int TYPE, int NT> cudaError_t launch_stream(const Call &k, int sms, cudaStream_t stream);
-template <int TYPE> cudaError_t launch_tile(const Call &k, int sms, cudaStream_t stream);
+template <int TYPE, int NT, int MODE> cudaError_t launch_stream(const Call &k, int sms, cudaStream_t stream);
+template <int TYPE, int MODE> cudaError_t launch_tile(const Call &k, int sms, cudaStream_t stream);
+// SHARED: the outputs from the sums over common and own tokens
+template <int TYPE> cudaError_t launch_merge(const Call &k, int sms, cudaStream_t stream);
 
 }  // namespace paged
