@@ -34,11 +34,17 @@ bool may_be_wide(const mlops_paged_attend_args *a, int kv_heads, bool shared) {
 // of 8 and 254 in tiles of 16, 16 requests of 5 000 to 16 000 tokens with 12 to 24 columns 105 and 103, with 32 columns 153 and 125. The host knows the average only.
 template <int TYPE, int MODE> cudaError_t attend(const Call &k, bool tiles, int sms, cudaStream_t stream) {
   const bool narrow = (int64_t)k.a.tokens * k.group <= (int64_t)8 * k.a.batch;
-  cudaError_t e = narrow ? launch_stream<TYPE, 1, MODE>(k, sms, stream) : launch_stream<TYPE, 2, MODE>(k, sms, stream);
-  if (e == cudaSuccess && tiles) e = launch_tile<TYPE, MODE>(k, sms, stream);
-  if constexpr (MODE == SHARED)
-    if (e == cudaSuccess) e = launch_merge<TYPE>(k, sms, stream);
-  return e;
+  const auto few = [&](const Call &k) { return narrow ? launch_stream<TYPE, 1, MODE>(k, sms, stream) : launch_stream<TYPE, 2, MODE>(k, sms, stream); };
+  if constexpr (MODE == SHARED) {
+    // the stream's CTAs begin where the tile kernel's end: neither reads what the other leaves
+    cudaError_t e = tiles ? launch_tile<TYPE, MODE>(k, sms, stream) : cudaSuccess;
+    Call second = k;
+    second.wait_last = tiles;
+    if (e == cudaSuccess) e = few(second);
+    return e != cudaSuccess ? e : launch_merge<TYPE>(k, sms, stream);
+  }
+  const cudaError_t e = few(k);
+  return e != cudaSuccess || !tiles ? e : launch_tile<TYPE, MODE>(k, sms, stream);
 }
 
 template <int MODE> cudaError_t call(const mlops_paged_attend_args *a, const mlops_paged_common *common, const mlops_paged_cache *c, void *scratch, int sms, cudaStream_t stream) {

@@ -23,9 +23,10 @@ struct Call {
   int wide;        // requests with more than so many columns (queries times group) are the tile kernel's
   float *stream_part, *tile_part;          // partial rows, see the kernels
   int *stream_counters, *tile_counters;    // one per CTA, zeros before and after every call
-  // SHARED: the groups, and the sums (o[128], m, l, whether the common row counts) of every row of q and head over common and own tokens
+  // SHARED: the groups, and the sums of every row of q and head over common and own tokens (RowEnd)
   mlops_paged_common common;
   float *common_rows, *own_rows;
+  bool wait_last;  // the kernel before in the stream is of the same call and leaves nothing that this one reads: waited for at the end
 };
 
 // a column's query and its query head among the KV head's: column / group, column % group
@@ -163,13 +164,19 @@ __device__ __forceinline__ float lse_of(float m, float l) { return l == 0.f ? -F
 __device__ __forceinline__ float *sums_row(const Call &k, bool common, int row, int head) {
   return (common ? k.common_rows : k.own_rows) + ((size_t)row * k.a.q_heads + head) * PSTRIDE;
 }
-// what stands behind them: m (anything where l is 0), l, whether the common row counts too
-__device__ __forceinline__ float4 sums_end(const Apart &r, float m, float l) { return make_float4(m, l, r.skip > 0 ? 1.f : 0.f, 0.f); }
+// What stands behind a row's sums o[128], which merge_kernel joins: m (anything where l is 0), l, whether the common row counts too, 0. Where CTAs share the row: the first of its
+// pieces as a row of stream_part, the rows of a CTA's slot, whether the common row counts too, how many pieces.
+__device__ __forceinline__ float4 row_end(const Apart &r, float m, float l) { return make_float4(m, l, __int_as_float(r.skip > 0), __int_as_float(0)); }
+__device__ __forceinline__ float4 pieces_end(const Apart &r, int first, int rows, int pieces) {
+  return make_float4(__int_as_float(first), __int_as_float(rows), __int_as_float(r.skip > 0), __int_as_float(pieces));
+}
+// CTA c has two slots of `rows` rows: pieces of rows that other CTAs begin, and that it begins. Piece i of a row that CTA c begins, relative to piece 0
+__device__ __forceinline__ int piece_row(int rows, int i) { return i ? (2 * i - 1) * rows : 0; }
 
 // zeros (and -infinity) for q's row `row`, by one warp; SHARED: no sums, for the item r or for no request (skip 0)
 template <int MODE> __device__ __forceinline__ void clear_row(const Call &k, const Request<MODE> &r, int row, int lane) {
   if constexpr (MODE == SHARED) {
-    for (int i = lane; i < k.a.q_heads; i += 32) *reinterpret_cast<float4 *>(sums_row(k, false, row, i) + D) = sums_end(r, NOTHING, 0.f);
+    for (int i = lane; i < k.a.q_heads; i += 32) *reinterpret_cast<float4 *>(sums_row(k, false, row, i) + D) = row_end(r, NOTHING, 0.f);
   } else {
     for (int i = lane; i < k.a.q_heads * 16; i += 32) reinterpret_cast<uint4 *>(out_row(k, row, i >> 4))[i & 15] = make_uint4(0, 0, 0, 0);
     if (k.a.lse)
@@ -182,7 +189,7 @@ __device__ __forceinline__ void store_joined(const Call &k, const Request<MODE> 
   if constexpr (MODE == SHARED) {
     float *const to = sums_row(k, r.common, row, head);
     reinterpret_cast<float4 *>(to)[x] = l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : o;
-    if (x == 0) *reinterpret_cast<float4 *>(to + D) = sums_end(r, m, l);
+    if (x == 0) *reinterpret_cast<float4 *>(to + D) = row_end(r, m, l);
   } else {
     const float f = l == 0.f ? 0.f : __ldg(k.c.v_scale + kv_head) / l;
     *reinterpret_cast<uint2 *>(out_row(k, row, head) + 4 * x) = make_uint2(from_floats<TYPE>(o.x * f, o.y * f), from_floats<TYPE>(o.z * f, o.w * f));

@@ -9,6 +9,48 @@ namespace {
 
 constexpr int WARPS = 8;
 
+struct Part {  // a lane's four channels; m is NOTHING where l is 0
+  float4 o;
+  float m, l;
+};
+__device__ __forceinline__ void add(float4 &o, const float4 &x, float f) { o = make_float4(fmaf(x.x, f, o.x), fmaf(x.y, f, o.y), fmaf(x.z, f, o.z), fmaf(x.w, f, o.w)); }
+__device__ __forceinline__ void join(Part &a, float top, const Part &b) {
+  const float f = a.l == 0.f ? 0.f : ex2(a.m - top), g = b.l == 0.f ? 0.f : ex2(b.m - top);
+  a.o = make_float4(a.o.x * f, a.o.y * f, a.o.z * f, a.o.w * f);
+  if (b.l != 0.f) add(a.o, b.o, g);
+  a.l = a.l * f + (b.l == 0.f ? 0.f : b.l * g);
+  a.m = top;
+}
+// a row's sums, from itself (x: the lane's channels) or from its pieces, in their order
+__device__ __forceinline__ Part part_of(const Call &k, const float4 &x, const float4 &end, int lane) {
+  const int pieces = __float_as_int(end.w), rows = __float_as_int(end.y);
+  if (!pieces) {
+    if (end.y == 0.f) return Part{make_float4(0.f, 0.f, 0.f, 0.f), NOTHING, 0.f};
+    return Part{x, end.x, end.y};
+  }
+  const float *const first = k.stream_part + (size_t)__float_as_int(end.x) * PSTRIDE;
+  Part p{make_float4(0.f, 0.f, 0.f, 0.f), NOTHING, 0.f};
+  for (int i0 = 0; i0 < pieces; i0 += 32) {
+    const int n = min(pieces - i0, 32);
+    float2 z = make_float2(NOTHING, 0.f);
+    if (lane < n) z = __ldcg(reinterpret_cast<const float2 *>(first + (size_t)piece_row(rows, i0 + lane) * PSTRIDE + D));
+    if (z.y == 0.f) z.x = NOTHING;
+    float top = fmaxf(z.x, p.m);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, d));
+    const float weight = z.y == 0.f ? 0.f : ex2(z.x - top), keep = p.l == 0.f ? 0.f : ex2(p.m - top);
+    p.l = p.l * keep + fbla::warp_sum(z.y * weight);
+    p.o = make_float4(p.o.x * keep, p.o.y * keep, p.o.z * keep, p.o.w * keep);
+    p.m = top;
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+      const float4 v = __ldcg(reinterpret_cast<const float4 *>(first + (size_t)piece_row(rows, i0 + i) * PSTRIDE) + lane);
+      add(p.o, v, __shfl_sync(FULL, weight, i));
+    }
+  }
+  return p;
+}
+
 template <int TYPE> __global__ void __launch_bounds__(32 * WARPS) merge_kernel(const Call k, const Divisor by_heads) {
   fbla::wait_previous_pass();
   fbla::allow_next_pass();
@@ -19,15 +61,16 @@ template <int TYPE> __global__ void __launch_bounds__(32 * WARPS) merge_kernel(c
     const float *const own = sums_row(k, false, row, head), *const common = sums_row(k, true, row, head);
     const float4 x = __ldcg(reinterpret_cast<const float4 *>(own) + lane), x_end = __ldcg(reinterpret_cast<const float4 *>(own + D));
     const float4 y = __ldcg(reinterpret_cast<const float4 *>(common) + lane), y_end = __ldcg(reinterpret_cast<const float4 *>(common + D));
-    // (a part without sums holds anything)
-    const float m = x_end.y == 0.f ? NOTHING : x_end.x, n = x_end.z == 0.f || y_end.y == 0.f ? NOTHING : y_end.x, top = fmaxf(m, n);
-    const float f = x_end.y == 0.f ? 0.f : ex2(m - top), g = x_end.z == 0.f || y_end.y == 0.f ? 0.f : ex2(n - top);
-    const float l = (f == 0.f ? 0.f : f * x_end.y) + (g == 0.f ? 0.f : g * y_end.y);
-    float4 o = f == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
-    if (g != 0.f) o = make_float4(fmaf(y.x, g, o.x), fmaf(y.y, g, o.y), fmaf(y.z, g, o.z), fmaf(y.w, g, o.w));
+    Part a = part_of(k, x, x_end, lane);
+    if (__float_as_int(x_end.z)) {
+      const Part b = part_of(k, y, y_end, lane);
+      const float top = fmaxf(a.m, b.m);
+      join(a, top, b);
+    }
+    const float l = a.l;
     const float scale = l == 0.f ? 0.f : __ldg(k.c.v_scale + k.by_group.divide(head)) / l;
-    *reinterpret_cast<uint2 *>(out_row(k, row, head) + 4 * lane) = make_uint2(from_floats<TYPE>(o.x * scale, o.y * scale), from_floats<TYPE>(o.z * scale, o.w * scale));
-    if (k.a.lse && lane == 0) k.a.lse[at] = lse_of(top, l);
+    *reinterpret_cast<uint2 *>(out_row(k, row, head) + 4 * lane) = make_uint2(from_floats<TYPE>(a.o.x * scale, a.o.y * scale), from_floats<TYPE>(a.o.z * scale, a.o.w * scale));
+    if (k.a.lse && lane == 0) k.a.lse[at] = lse_of(a.m, l);
   }
 }
 

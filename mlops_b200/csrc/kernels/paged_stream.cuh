@@ -368,7 +368,7 @@ template <int TYPE, int NT, int MODE> __device__ __forceinline__ void store_row(
         for (int h = 0; h < 4; ++h)
           reinterpret_cast<float4 *>(to + 16 * g)[h] = make_float4(s.o[j][4 * (h & 1)][2 * (h >> 1) + i], s.o[j][4 * (h & 1) + 1][2 * (h >> 1) + i],
                                                                    s.o[j][4 * (h & 1) + 2][2 * (h >> 1) + i], s.o[j][4 * (h & 1) + 3][2 * (h >> 1) + i]);
-        if (g == 0) *reinterpret_cast<float4 *>(to + D) = sums_end(w.r, s.m[j][i], s.l[j][i]);
+        if (g == 0) *reinterpret_cast<float4 *>(to + D) = row_end(w.r, s.m[j][i], s.l[j][i]);
         continue;
       }
       const float f = s.l[j][i] == 0.f ? 0.f : vs / s.l[j][i];
@@ -403,7 +403,7 @@ template <int TYPE, int NT, int MODE> __global__ void __launch_bounds__(THREADS<
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (lane < STAGES<NT>) fbla::mbar_init(&sm.full[warp][lane], 1);
   fbla::mbar_init_fence();
-  fbla::wait_previous_pass();
+  if (MODE != SHARED || !k.wait_last) fbla::wait_previous_pass();
   fbla::allow_next_pass();
 
   // the items' units
@@ -565,13 +565,20 @@ template <int TYPE, int NT, int MODE> __global__ void __launch_bounds__(THREADS<
       float *const slot = k.stream_part + (((size_t)blockIdx.x * 2 + (w.unit0 < cta_lo ? 0 : 1)) * 8 * NT + c) * PSTRIDE;
       __stcg(reinterpret_cast<float4 *>(slot) + lane, o);
       if (lane == 0) __stcg(reinterpret_cast<float2 *>(slot + D), make_float2(m, l));
+      if constexpr (MODE == SHARED)
+        if (lane == 0 && w.unit0 >= cta_lo) {
+          int query, head;
+          split_column(k, w.tile * 8 * NT + c, query, head);
+          const int slots = deal.warp_of(w.unit0 + w.units - 1) / WARPS<NT> - blockIdx.x + 1;
+          *reinterpret_cast<float4 *>(sums_row(k, w.r.common, w.r.start + query, w.head * k.group + head) + D) = pieces_end(w.r, (blockIdx.x * 2 + 1) * 8 * NT + c, 8 * NT, slots);
+        }
     } else {
       store(w, c, o, m, l);
     }
   }
-  // rows that go on in other CTAs, this one's first and last at most: the CTA that comes last joins their slots
+  // rows that go on in other CTAs, this one's first and last at most: the CTA that comes last joins their slots (SHARED: merge_kernel)
   const int ends[2] = {__ffs(leaders) - 1, 31 - __clz(leaders)};
-  if (leaders && (is_cut(sm.row[ends[0]]) || is_cut(sm.row[ends[1]]))) {
+  if (MODE != SHARED && leaders && (is_cut(sm.row[ends[0]]) || is_cut(sm.row[ends[1]]))) {
     __threadfence();
     __syncthreads();
     if (tid < 2) {
@@ -661,6 +668,7 @@ template <int TYPE, int NT, int MODE> __global__ void __launch_bounds__(THREADS<
     const int first = min(max(__ldg(k.a.starts), 0), k.a.tokens), end = min(max(__ldg(k.a.starts + k.a.batch), first), k.a.tokens);
     for (int i = me; i < first + k.a.tokens - end; i += all) clear_row<MODE>(k, Request<MODE>{}, i < first ? i : i - first + end, lane);
   }
+  if (MODE == SHARED && k.wait_last) fbla::wait_previous_pass();
 }
 
 }  // namespace

@@ -523,6 +523,9 @@ __device__ __forceinline__ bool take_tile(Smem<MODE> &sm, Line &q, uint32_t s, u
   return ok;
 }
 
+// CTA of unit u when `ctas` CTAs share `total` units: CTA c has [total c / ctas, total (c + 1) / ctas)
+__device__ __forceinline__ int cta_of(long long u, long long total, int ctas) { return (int)(((u + 1) * ctas - 1) / total); }
+
 template <int TYPE, int MODE> __device__ __forceinline__ void soften(const Call &k, Smem<MODE> &sm, long long hi, int warp, int lane) {
   const int half = warp >> 2, line = 32 * (warp & 3) + lane;
   const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
@@ -632,8 +635,16 @@ template <int TYPE, int MODE> __device__ __forceinline__ void soften(const Call 
       if (half == 0 && c < w.rows(k)) {
         int query, head;
         split_column(k, 2 * ROWS * w.pair + c, query, head);
-        if constexpr (MODE == SHARED) __stcg(reinterpret_cast<float4 *>(slot + D), sums_end(w.r, m, l));
-        else if (!whole) __stcg(reinterpret_cast<float2 *>(slot + D), make_float2(m, l));
+        if constexpr (MODE == SHARED) {
+          if (whole) __stcg(reinterpret_cast<float4 *>(slot + D), row_end(w.r, m, l));
+          else __stcg(reinterpret_cast<float2 *>(slot + D), make_float2(m, l));
+          if (!whole && w.n0 == 0) {
+            const long long total = sm.before[items_of<MODE>(k)];
+            const int pieces = cta_of(w.unit0 + HEAD + w.tiles - 1, total, (int)min(total, (long long)gridDim.x)) - blockIdx.x + 1;
+            __stcg(reinterpret_cast<float4 *>(sums_row(k, w.r.common, w.r.start + query, w.head * k.group + head) + D),
+                   pieces_end(w.r, (int)((k.tile_part - k.stream_part) / PSTRIDE) + (blockIdx.x * 2 + 1) * 2 * ROWS + c, 2 * ROWS, pieces));
+          }
+        } else if (!whole) __stcg(reinterpret_cast<float2 *>(slot + D), make_float2(m, l));
         else if (k.a.lse) k.a.lse[(size_t)(w.r.start + query) * k.a.q_heads + w.head * k.group + head] = lse_of(m, l);
       }
     }
@@ -655,9 +666,6 @@ template <int TYPE, int MODE> __device__ __forceinline__ void soften(const Call 
     more = __shfl_sync(FULL, (int)more, 0);
   } while (more);
 }
-
-// CTA of unit u when `ctas` CTAs share `total` units: CTA c has [total c / ctas, total (c + 1) / ctas)
-__device__ __forceinline__ int cta_of(long long u, long long total, int ctas) { return (int)(((u + 1) * ctas - 1) / total); }
 
 // the partial rows of row of work w, joined by the CTA that comes last
 template <int TYPE, int MODE> __device__ __forceinline__ void join_row(const Call &k, Smem<MODE> &sm, const Row<MODE> &w, long long total, int tid) {
@@ -686,12 +694,11 @@ template <int TYPE, int MODE> __device__ __forceinline__ void join_row(const Cal
       weights[c * pieces + i] = ex2(y.x - m);
       l += y.y * ex2(y.x - m);
     }
-    const float f = MODE == SHARED ? 1.f : l == 0.f ? 0.f : v_scale / l;
+    const float f = l == 0.f ? 0.f : v_scale / l;
     for (int i = 0; i < pieces; ++i) weights[c * pieces + i] *= f;
     int query, head;
     split_column(k, 2 * ROWS * w.pair + c, query, head);
-    if constexpr (MODE == SHARED) *reinterpret_cast<float4 *>(sums_row(k, w.r.common, w.r.start + query, w.head * k.group + head) + D) = sums_end(w.r, m, l);
-    else if (k.a.lse) k.a.lse[(size_t)(w.r.start + query) * k.a.q_heads + w.head * k.group + head] = lse_of(m, l);
+    if (k.a.lse) k.a.lse[(size_t)(w.r.start + query) * k.a.q_heads + w.head * k.group + head] = lse_of(m, l);
   }
   __syncthreads();
   constexpr int AHEAD = 8;  // float4 of a thread that are on their way at once
@@ -717,8 +724,7 @@ template <int TYPE, int MODE> __device__ __forceinline__ void join_row(const Cal
       if (e >= rows * 32) break;
       int query, head;
       split_column(k, 2 * ROWS * w.pair + (e >> 5), query, head);
-      if constexpr (MODE == SHARED) reinterpret_cast<float4 *>(sums_row(k, w.r.common, w.r.start + query, w.head * k.group + head))[e & 31] = o[j];
-      else reinterpret_cast<uint2 *>(out_row(k, w.r.start + query, w.head * k.group + head))[e & 31] = make_uint2(from_floats<TYPE>(o[j].x, o[j].y), from_floats<TYPE>(o[j].z, o[j].w));
+      reinterpret_cast<uint2 *>(out_row(k, w.r.start + query, w.head * k.group + head))[e & 31] = make_uint2(from_floats<TYPE>(o[j].x, o[j].y), from_floats<TYPE>(o[j].z, o[j].w));
     }
   }
   __syncthreads();
@@ -862,7 +868,8 @@ template <int TYPE, int MODE> __global__ void __launch_bounds__(THREADS, 1) tile
   if (!tiles) return;
   if (sm.v_nan) spoil_rows(k, sm, hi, tid);
 
-  // the run's first and last rows of work, where they are cut
+  // the run's first and last rows of work, where they are cut (SHARED: merge_kernel joins them)
+  if constexpr (MODE == SHARED) return;
   const Row<MODE> w = sm.begin;
   if (w.n0 > 0 || w.n1 < w.tiles) join_row<TYPE, MODE>(k, sm, w, total, tid);
   const Row<MODE> end = sm.row[0];
