@@ -33,8 +33,7 @@ bool may_be_wide(const mlops_paged_attend_args *a, int kv_heads, bool shared) {
 // Streamed in tiles of 8 columns where a request has no more on average, else of 16; us on the device: 64 requests of 1K-64K tokens and 4 columns each take 176 in tiles
 // of 8 and 254 in tiles of 16, 16 requests of 5 000 to 16 000 tokens with 12 to 24 columns 105 and 103, with 32 columns 153 and 125. The host knows the average only.
 template <int TYPE, int MODE> cudaError_t attend(const Call &k, bool tiles, int sms, cudaStream_t stream) {
-  const bool narrow = (int64_t)k.a.tokens * k.group <= (int64_t)8 * k.a.batch;
-  const auto few = [&](const Call &k) { return narrow ? launch_stream<TYPE, 1, MODE>(k, sms, stream) : launch_stream<TYPE, 2, MODE>(k, sms, stream); };
+  const auto few = [&](const Call &k) { return k.narrow == 8 ? launch_stream<TYPE, 1, MODE>(k, sms, stream) : launch_stream<TYPE, 2, MODE>(k, sms, stream); };
   if constexpr (MODE == SHARED) {
     // the stream's CTAs begin where the tile kernel's end: neither reads what the other leaves
     cudaError_t e = tiles ? launch_tile<TYPE, MODE>(k, sms, stream) : cudaSuccess;
@@ -58,6 +57,7 @@ template <int MODE> cudaError_t call(const mlops_paged_attend_args *a, const mlo
   k.group = a->q_heads / c->kv_heads;
   k.by_group = Divisor(k.group);
   k.wide = WIDE;
+  k.narrow = (int64_t)a->tokens * k.group <= (int64_t)8 * a->batch ? 8 : 16;
   k.stream_counters = reinterpret_cast<int *>(base + s.stream_counters);
   k.tile_counters = reinterpret_cast<int *>(base + s.tile_counters);
   k.stream_part = reinterpret_cast<float *>(base + s.stream_part);

@@ -21,6 +21,7 @@ struct Call {
   int group;       // query heads per KV head
   Divisor by_group;
   int wide;        // requests with more than so many columns (queries times group) are the tile kernel's
+  int narrow;      // columns of the stream's rows of work
   float *stream_part, *tile_part;          // partial rows, see the kernels
   int *stream_counters, *tile_counters;    // one per CTA, zeros before and after every call
   // SHARED: the groups, and the sums of every row of q and head over common and own tokens (RowEnd)
@@ -172,6 +173,44 @@ __device__ __forceinline__ float4 pieces_end(const Apart &r, int first, int rows
 }
 // CTA c has two slots of `rows` rows: pieces of rows that other CTAs begin, and that it begins. Piece i of a row that CTA c begins, relative to piece 0
 __device__ __forceinline__ int piece_row(int rows, int i) { return i ? (2 * i - 1) * rows : 0; }
+
+// Units of work. The stream's: two blocks of a row of work of `narrow` columns. The tile kernel's: a tile of 128 tokens of a row of work of 256 rows, and HEAD for the row.
+constexpr int UNIT = 2 * BT, TILE_ROWS = 256, TOKENS = 128;
+constexpr int HEAD = 4;  // what loading Q, the first tile and storing O cost (17 000 cycles beside 4 300 per tile; us for two prompts of 8192 with 0, 2, 4, 6, 8: 2006, 1833, 1732, 1757, 1754
+                         // when they were 26 000 and 5 300)
+__device__ __forceinline__ int units_of(const Plain &r) { return (r.tokens + UNIT - 1) / UNIT; }  // of each of the item's rows of work
+__device__ __forceinline__ int stream_units(const Call &k, const Plain &r, int columns) {
+  return r.n * k.group > k.wide ? 0 : k.c.kv_heads * ((r.n * k.group + columns - 1) / columns) * units_of(r);
+}
+__device__ __forceinline__ int rows_of(const Call &k, const Plain &r) { return r.n * k.group; }
+// tiles of tokens that rows up to 256 (pair + 1) of an item see
+template <int MODE> __device__ __forceinline__ int tiles_of(const Call &k, const Request<MODE> &r, int pair) {
+  const int last = min(TILE_ROWS * (pair + 1), rows_of(k, r)) - 1, seen = min(limit_of<MODE>(r, query_of(k, last)) + 1, r.tokens);
+  return max((seen + TOKENS - 1) / TOKENS, 1);  // (rows that see nothing have a tile all the same: their zeros are written like the others' sums)
+}
+template <int MODE> __device__ __forceinline__ long long tile_units(const Call &k, const Request<MODE> &r) {
+  long long n = 0;
+  if (r.tokens > 0 && r.n * k.group > k.wide) {
+    for (int p = 0; TILE_ROWS * p < rows_of(k, r); ++p) n += HEAD + tiles_of<MODE>(k, r, p);
+    n *= k.c.kv_heads;
+  }
+  return n;
+}
+
+// SHARED: both kernels have work that does not wait for the other's, one bound by its products, the other by memory, on multiprocessors of their own: how many of `sms` are the tile
+// kernel's, so that both end together. Cycles of a unit and beside the units, as measured: 4 400 and 36 000; 250 or 360 (tiles of 8 or 16 columns) and 40 000, with the start behind the tile
+// kernel's CTAs that have nothing to do. In pairs: both kernels are launched in clusters of two, which lie on two multiprocessors of a kind of their own (TPC); one of each kernel there slow
+// each other down, the tile kernel's to 0.78 and the stream's to 0.7 of their rate (256 requests behind 32 768 common tokens, us: 306, in pairs 220). By one warp; any number is right.
+constexpr int PAIR = 2;
+__device__ __forceinline__ int tile_share(const Call &k, long long tiles, int units, int sms, int lane) {
+  if (tiles == 0 || units == 0 || sms < 2 * PAIR) return tiles ? sms : 0;
+  uint32_t best = ~0u;
+  for (int n = PAIR * (1 + lane); n < sms; n += 32 * PAIR) {
+    const float a = 36e3f + 4400.f * ceilf((float)tiles / n), b = 40e3f + (k.narrow == 8 ? 250.f : 360.f) * (float)units / (sms - n);
+    best = min(best, (uint32_t)fminf(fmaxf(a, b) * 0.0625f, 2097151.f) << 11 | n);
+  }
+  return __reduce_min_sync(FULL, best) & 2047;
+}
 
 // zeros (and -infinity) for q's row `row`, by one warp; SHARED: no sums, for the item r or for no request (skip 0)
 template <int MODE> __device__ __forceinline__ void clear_row(const Call &k, const Request<MODE> &r, int row, int lane) {

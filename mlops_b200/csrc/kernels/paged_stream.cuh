@@ -33,7 +33,6 @@ namespace {
 // the time of drafted tokens of 16 requests). Three do not pay: requests of 24 columns take 0.85 of the time, but those of 16 columns 1.14 and of 32 1.15.
 template <int NT> constexpr int WARPS = NT == 1 ? 16 : 8;
 template <int NT> constexpr int STAGES = NT == 1 ? 2 : 3;
-constexpr int UNIT = 2 * BT;  // tokens of a unit
 template <int NT> constexpr int THREADS = 32 * WARPS<NT>;
 constexpr uint32_t DRAIN = 1u << 20;  // polls for a copy after a wait that gave up
 constexpr float TOP = 15.f, REST = 9.f;  // log2 of the largest P, and of a column's largest when m' is set
@@ -55,7 +54,8 @@ template <int NT, int MODE> struct __align__(128) Smem {
   int tag[32];                     // pieces in the order of the tokens, two per warp: the first unit of the piece's row, -1: none
   Row<NT, MODE> row[32];           // the pieces' rows
   float2 total[8 * NT];            // (m', l) of a row that CTAs share
-  int warp_sum[WARPS<NT>];
+  int warp_sum[WARPS<NT>], share;
+  long long tiles;  // SHARED: units of the tile kernel
   int last[2];
   int before[];                    // [items + 1]: the items' first units
 };
@@ -93,12 +93,7 @@ struct Deal {
   __device__ __forceinline__ int warp_of(int u) const { return u < more * (whole + 1) ? u / (whole + 1) : (u - more) / whole; }
 };
 
-__device__ __forceinline__ int units_of(const Plain &r) { return (r.tokens + UNIT - 1) / UNIT; }  // of each of a request's rows of work
 template <int NT> __device__ __forceinline__ int tiles_of(const Call &k, const Plain &r) { return (r.n * k.group + 8 * NT - 1) / (8 * NT); }
-template <int NT> __device__ __forceinline__ int all_units_of(const Call &k, const Plain &r) {
-  return r.n * k.group > k.wide ? 0 : k.c.kv_heads * tiles_of<NT>(k, r) * units_of(r);
-}
-
 // the item that unit u belongs to: before[b] <= u < before[b + 1]
 __device__ __forceinline__ int item_at(const int *before, int items, int u) {
   int a = 0;
@@ -409,8 +404,15 @@ template <int TYPE, int NT, int MODE> __global__ void __launch_bounds__(THREADS<
   // the items' units
   const int items = items_of<MODE>(k);
   int total = 0;
+  long long tiles = 0;
   for (int b0 = 0; b0 < items; b0 += THREADS<NT>) {
-    const int b = b0 + tid, n = b < items ? all_units_of<NT>(k, request<MODE>(k, b)) : 0;
+    const int b = b0 + tid;
+    int n = 0;
+    if (b < items) {
+      const Request<MODE> r = request<MODE>(k, b);
+      n = stream_units(k, r, 8 * NT);
+      if (MODE == SHARED && k.wait_last) tiles += tile_units<MODE>(k, r);
+    }
     int sum = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -430,9 +432,23 @@ template <int TYPE, int NT, int MODE> __global__ void __launch_bounds__(THREADS<
   }
   if (tid == 0) sm.before[items] = total;
   if (tid < 32) sm.tag[tid] = -1;
+  int ctas = gridDim.x;  // that have units
+  if (MODE == SHARED && k.wait_last && total) {
+    if (tid == 0) sm.tiles = 0;
+    __syncthreads();
+    if (tiles) atomicAdd(reinterpret_cast<unsigned long long *>(&sm.tiles), (unsigned long long)tiles);
+    __syncthreads();
+    if (warp == 0) {
+      const int share = tile_share(k, sm.tiles, total, gridDim.x, lane);
+      if (lane == 0) sm.share = share;
+    }
+    __syncthreads();
+    ctas -= sm.share;
+    if (blockIdx.x >= ctas) return;  // (they begin when the tile kernel's CTAs are through; those with units wait for all of them)
+  }
   __syncthreads();
 
-  const int me = blockIdx.x * WARPS<NT> + warp, all = gridDim.x * WARPS<NT>;
+  const int me = blockIdx.x * WARPS<NT> + warp, all = ctas * WARPS<NT>;
   const Deal deal(total, all);
   const int lo = deal.first(me), hi = deal.first(me + 1), count = hi - lo;
   if (count > 0) {
@@ -678,7 +694,8 @@ template <int TYPE, int NT, int MODE> cudaError_t launch_stream(const Call &k, i
   const cudaError_t e = allow_shared(stream_kernel<TYPE, NT, MODE>, ready);
   if (e != cudaSuccess) return e;
   const size_t items = (size_t)k.a.batch + (MODE == SHARED ? k.common.groups : 0);
-  return fbla::launch(true, 1, stream_kernel<TYPE, NT, MODE>, dim3(sms), THREADS<NT>, shared_bytes<NT, MODE>(items), stream, k);
+  const int pair = MODE == SHARED && k.wait_last && sms > 1 ? PAIR : 1;
+  return fbla::launch(true, pair, stream_kernel<TYPE, NT, MODE>, dim3(sms / pair * pair), THREADS<NT>, shared_bytes<NT, MODE>(items), stream, k);
 }
 template <int NT, int MODE> constexpr bool holds = shared_bytes<NT, MODE>(PAGED_K_MAX_ATTENDED) <= 232448;
 #define PAGED_STREAM(mode)                                                                                   \

@@ -33,18 +33,14 @@ namespace {
 
 namespace tc = fbla::tc;
 
-constexpr int ROWS = 128, TOKENS = 128;     // of a product
+constexpr int ROWS = 128;  // of a product, with 128 tokens
 constexpr int SLAB = 128 * 128, TILE = 2 * SLAB;  // bytes of a slab (128 rows of 64 channels) and of an operand
 constexpr int STAGES = 2, PRODUCER0 = 8, PRODUCERS = 8, ISSUER0 = 16, FINDER = 18, THREADS = 20 * 32;  // (four warps share a register count: 19 idles)
-constexpr int HEAD = 4;  // units of a row of work beside its tiles: what loading Q, the first tile and storing O cost (17 000 cycles beside 4 300 per
-                         // tile; us for two prompts of 8192 with 0, 2, 4, 6, 8: 2006, 1833, 1732, 1757, 1754 when they were 26 000 and 5 300)
 constexpr int WINDOW = 16;  // tiles whose blocks are looked up at a time
 constexpr int NO_TILE = -0x7fffffff;
 constexpr float TOP = 15.f, REST = 9.f;
 constexpr long long WAIT_CYCLES = 2000000000;
 constexpr uint32_t IDESC_S = tc::IDESC_F16, IDESC_O = tc::IDESC_F16 | (1u << 16);  // V: MN-major
-
-__device__ __forceinline__ int rows_of(const Call &k, const Plain &r) { return r.n * k.group; }
 
 // a row of work and its part in this CTA's run: tiles of tokens n0 .. n1 - 1 of `tiles`
 template <int MODE> struct Row {
@@ -71,6 +67,7 @@ template <int MODE> struct __align__(1024) Smem {
   long long warp_sum[THREADS / 32];
   uint32_t tmem;
   int abort, last;
+  int others, share;  // SHARED: the stream's units, the CTAs that have tiles
   long long before[];   // [items + 1]: the items' first units
 };
 
@@ -89,13 +86,6 @@ template <int MODE> __device__ __forceinline__ bool wait(Smem<MODE> &sm, uint64_
 __device__ __forceinline__ uint64_t v_desc(const void *tile, uint32_t byte_offset) {
   return tc::smem_desc_at(tile, byte_offset) | ((uint64_t)(SLAB >> 4) << 16);
 }
-
-// tiles of tokens that rows up to 256 (pair + 1) of a request see
-template <int MODE> __device__ __forceinline__ int tiles_of(const Call &k, const Request<MODE> &r, int pair) {
-  const int last = min(2 * ROWS * (pair + 1), rows_of(k, r)) - 1, seen = min(limit_of<MODE>(r, query_of(k, last)) + 1, r.tokens);
-  return max((seen + TOKENS - 1) / TOKENS, 1);  // (rows that see nothing have a tile all the same: their zeros are written like the others' sums)
-}
-__device__ __forceinline__ bool taken(const Call &k, const Plain &r) { return r.tokens > 0 && r.n * k.group > k.wide; }
 
 // the first row of work of the run [lo, hi), found by a warp
 template <int MODE> __device__ __forceinline__ Row<MODE> first_row(const Call &k, const long long *before, long long lo, long long hi, int lane) {
@@ -640,7 +630,7 @@ template <int TYPE, int MODE> __device__ __forceinline__ void soften(const Call 
           else __stcg(reinterpret_cast<float2 *>(slot + D), make_float2(m, l));
           if (!whole && w.n0 == 0) {
             const long long total = sm.before[items_of<MODE>(k)];
-            const int pieces = cta_of(w.unit0 + HEAD + w.tiles - 1, total, (int)min(total, (long long)gridDim.x)) - blockIdx.x + 1;
+            const int pieces = cta_of(w.unit0 + HEAD + w.tiles - 1, total, (int)min(total, (long long)sm.share)) - blockIdx.x + 1;
             __stcg(reinterpret_cast<float4 *>(sums_row(k, w.r.common, w.r.start + query, w.head * k.group + head) + D),
                    pieces_end(w.r, (int)((k.tile_part - k.stream_part) / PSTRIDE) + (blockIdx.x * 2 + 1) * 2 * ROWS + c, 2 * ROWS, pieces));
           }
@@ -787,7 +777,7 @@ template <int TYPE, int MODE> __global__ void __launch_bounds__(THREADS, 1) tile
       fbla::mbar_init(&sm.places_full[i], 1);
       fbla::mbar_init(&sm.places_empty[i], PRODUCERS);
     }
-    sm.abort = sm.v_nan = 0;
+    sm.abort = sm.v_nan = sm.others = 0;
     fbla::mbar_init_fence();
   }
   fbla::wait_previous_pass();
@@ -795,15 +785,14 @@ template <int TYPE, int MODE> __global__ void __launch_bounds__(THREADS, 1) tile
 
   const int items = items_of<MODE>(k);
   long long total = 0;
+  int others = 0;
   for (int b0 = 0; b0 < items; b0 += THREADS) {
     const int b = b0 + tid;
     long long n = 0;
     if (b < items) {
       const Request<MODE> r = request<MODE>(k, b);
-      if (taken(k, r)) {
-        for (int p = 0; 2 * ROWS * p < rows_of(k, r); ++p) n += HEAD + tiles_of<MODE>(k, r, p);
-        n *= k.c.kv_heads;
-      }
+      n = tile_units<MODE>(k, r);
+      if (MODE == SHARED) others += stream_units(k, r, k.narrow);
     }
     long long sum = n;
 #pragma unroll
@@ -823,8 +812,16 @@ template <int TYPE, int MODE> __global__ void __launch_bounds__(THREADS, 1) tile
     __syncthreads();
   }
   if (tid == 0) sm.before[items] = total;
+  if (MODE == SHARED) {
+    if (others) atomicAdd(&sm.others, others);
+    __syncthreads();
+    if (warp == 0) {
+      const int share = tile_share(k, total, sm.others, gridDim.x, lane);
+      if (lane == 0) sm.share = share;
+    }
+  }
   __syncthreads();
-  const int ctas = (int)min(total, (long long)gridDim.x);  // (each has a unit at least: a row's CTAs are consecutive)
+  const int ctas = (int)min(total, (long long)(MODE == SHARED ? sm.share : gridDim.x));  // (each has a unit at least: a row's CTAs are consecutive)
   if ((int)blockIdx.x >= ctas) return;
   const long long lo = total * blockIdx.x / ctas, hi = total * (blockIdx.x + 1) / ctas;
   if (warp == 0) {
@@ -886,7 +883,8 @@ template <int TYPE, int MODE> cudaError_t launch_tile(const Call &k, int sms, cu
   static thread_local bool ready[64] = {false};
   const cudaError_t e = allow_shared(tile_kernel<TYPE, MODE>, ready);
   if (e != cudaSuccess) return e;
-  return fbla::launch(true, 1, tile_kernel<TYPE, MODE>, dim3(sms), THREADS, tile_shared_bytes<MODE>((size_t)k.a.batch + (MODE == SHARED ? k.common.groups : 0)), stream, k);
+  const int pair = MODE == SHARED && sms > 1 ? PAIR : 1;
+  return fbla::launch(true, pair, tile_kernel<TYPE, MODE>, dim3(sms / pair * pair), THREADS, tile_shared_bytes<MODE>((size_t)k.a.batch + (MODE == SHARED ? k.common.groups : 0)), stream, k);
 }
 #define PAGED_TILE(mode)                                                                                             \
   static_assert(tile_shared_bytes<mode>(PAGED_K_MAX_ATTENDED) <= 232448, "the operands and the largest batch fit"); \
