@@ -574,68 +574,82 @@ template <int TYPE, int MODE> __device__ __forceinline__ void soften(const Call 
     const float v_scale = __ldg(k.c.v_scale + w.head);
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      if (!warp_live[x] || (x == 1 && shared)) continue;
-      float m = q[x].m, l = q[x].l, keep = q[x].started ? 1.f : 0.f, other = 0.f;
-      if (shared) {  // both halves' sums are of these rows
-        m = fmaxf(q[0].m, q[1].m);
-        l = q[0].l * ex2(q[0].m - m) + q[1].l * ex2(q[1].m - m);
-        keep = q[0].started ? ex2(q[0].m - m) : 0.f;
-        other = q[1].started ? ex2(q[1].m - m) : 0.f;
-      }
-      pair_meet(line >> 5);
-      sm.exchange[half][line] = l;
-      pair_meet(line >> 5);
-      l = half ? sm.exchange[0][line] + l : l + sm.exchange[1][line];
-      if (!ok) l = __int_as_float(0x7fc00000);  // (a wait that gave up: the rows are NaN)
-      const int c = line + ROWS * x;
-      const float f = l == 0.f ? 0.f : v_scale / l;
-      float *slot = k.tile_part + (((size_t)blockIdx.x * 2 + (w.n0 ? 0 : 1)) * 2 * ROWS + c) * PSTRIDE;
-      if constexpr (MODE == SHARED)
-        if (whole) {
+      if (x == 1 && shared) break;
+      const bool sums = MODE == SHARED || !whole;  // (else outputs)
+      auto slot = [&](int c) {  // where row c's sums go
+        if (MODE == SHARED && whole) {
           int query, head;
-          split_column(k, 2 * ROWS * w.pair + min(c, w.rows(k) - 1), query, head);
-          slot = sums_row(k, w.r.common, w.r.start + query, w.head * k.group + head);
+          split_column(k, 2 * ROWS * w.pair + c, query, head);
+          return sums_row(k, w.r.common, w.r.start + query, w.head * k.group + head);
         }
+        return k.tile_part + (((size_t)blockIdx.x * 2 + (w.n0 ? 0 : 1)) * 2 * ROWS + c) * PSTRIDE;
+      };
+      if (warp_live[x]) {
+        float m = q[x].m, l = q[x].l, keep = q[x].started ? 1.f : 0.f, other = 0.f;
+        if (shared) {  // both halves' sums are of these rows
+          m = fmaxf(q[0].m, q[1].m);
+          l = q[0].l * ex2(q[0].m - m) + q[1].l * ex2(q[1].m - m);
+          keep = q[0].started ? ex2(q[0].m - m) : 0.f;
+          other = q[1].started ? ex2(q[1].m - m) : 0.f;
+        }
+        pair_meet(line >> 5);
+        sm.exchange[half][line] = l;
+        pair_meet(line >> 5);
+        l = half ? sm.exchange[0][line] + l : l + sm.exchange[1][line];
+        if (!ok) l = __int_as_float(0x7fc00000);  // (a wait that gave up: the rows are NaN)
+        const int c = line + ROWS * x;
+        const float f = l == 0.f ? 0.f : v_scale / l;
 #pragma unroll 1
-      for (int i = 0; i < 4; ++i) {
-        const int ch = 64 * half + 16 * i;
-        uint32_t r[16], y[16];
-        tc::tmem_ld16(sm.tmem + 256 + 128 * x + lanes + ch, r);
-        tc::tmem_ld_wait(r);
-        float o[16];
+        for (int i = 0; i < 4; ++i) {
+          const int ch = 64 * half + 16 * i;
+          uint32_t r[16], y[16];
+          tc::tmem_ld16(sm.tmem + 256 + 128 * x + lanes + ch, r);
+          tc::tmem_ld_wait(r);
+          float o[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[e] = keep == 0.f ? 0.f : __uint_as_float(r[e]) * keep;  // (a half without tiles has nothing in its accumulator)
-        if (shared) {
-          tc::tmem_ld16(sm.tmem + 256 + 128 + lanes + ch, y);
-          tc::tmem_ld_wait(y);
+          for (int e = 0; e < 16; ++e) o[e] = keep == 0.f ? 0.f : __uint_as_float(r[e]) * keep;  // (a half without tiles has nothing in its accumulator)
+          if (shared) {
+            tc::tmem_ld16(sm.tmem + 256 + 128 + lanes + ch, y);
+            tc::tmem_ld_wait(y);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] = other == 0.f ? o[e] : fmaf(__uint_as_float(y[e]), other, o[e]);
+            for (int e = 0; e < 16; ++e) o[e] = other == 0.f ? o[e] : fmaf(__uint_as_float(y[e]), other, o[e]);
+          }
+          // through Q's place, from where rows are stored as a whole: in 16 bits both X's, sums one X after the other (16-byte piece i of a row at i ^ row % 32)
+          if (sums) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              *reinterpret_cast<float4 *>(sm.q[0] + line * 512 + ((((ch >> 2) + e) ^ lane) << 4)) = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              *reinterpret_cast<uint4 *>(sm.q[x] + half * SLAB + line * 128 + (((2 * i + e) ^ (line & 7)) << 4)) =
+                  pack8<TYPE>(make_float4(o[8 * e] * f, o[8 * e + 1] * f, o[8 * e + 2] * f, o[8 * e + 3] * f),
+                              make_float4(o[8 * e + 4] * f, o[8 * e + 5] * f, o[8 * e + 6] * f, o[8 * e + 7] * f));
+          }
         }
-        if (MODE != SHARED && whole) {  // through Q's place, from where whole rows are stored
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            *reinterpret_cast<uint4 *>(sm.q[x] + half * SLAB + line * 128 + (((2 * i + e) ^ (line & 7)) << 4)) =
-                pack8<TYPE>(make_float4(o[8 * e] * f, o[8 * e + 1] * f, o[8 * e + 2] * f, o[8 * e + 3] * f),
-                            make_float4(o[8 * e + 4] * f, o[8 * e + 5] * f, o[8 * e + 6] * f, o[8 * e + 7] * f));
-        } else if (c < w.rows(k)) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) __stcg(reinterpret_cast<float4 *>(slot + ch) + e, make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]));
+        if (half == 0 && c < w.rows(k)) {
+          int query, head;
+          split_column(k, 2 * ROWS * w.pair + c, query, head);
+          if constexpr (MODE == SHARED) {
+            if (whole) __stcg(reinterpret_cast<float4 *>(slot(c) + D), row_end(w.r, m, l));
+            else __stcg(reinterpret_cast<float2 *>(slot(c) + D), make_float2(m, l));
+            if (!whole && w.n0 == 0) {
+              const long long total = sm.before[items_of<MODE>(k)];
+              const int pieces = cta_of(w.unit0 + HEAD + w.tiles - 1, total, (int)min(total, (long long)sm.share)) - blockIdx.x + 1;
+              __stcg(reinterpret_cast<float4 *>(sums_row(k, w.r.common, w.r.start + query, w.head * k.group + head) + D),
+                     pieces_end(w.r, (int)((k.tile_part - k.stream_part) / PSTRIDE) + (blockIdx.x * 2 + 1) * 2 * ROWS + c, 2 * ROWS, pieces));
+            }
+          } else if (!whole) __stcg(reinterpret_cast<float2 *>(slot(c) + D), make_float2(m, l));
+          else if (k.a.lse) k.a.lse[(size_t)(w.r.start + query) * k.a.q_heads + w.head * k.group + head] = lse_of(m, l);
         }
       }
-      if (half == 0 && c < w.rows(k)) {
-        int query, head;
-        split_column(k, 2 * ROWS * w.pair + c, query, head);
-        if constexpr (MODE == SHARED) {
-          if (whole) __stcg(reinterpret_cast<float4 *>(slot + D), row_end(w.r, m, l));
-          else __stcg(reinterpret_cast<float2 *>(slot + D), make_float2(m, l));
-          if (!whole && w.n0 == 0) {
-            const long long total = sm.before[items_of<MODE>(k)];
-            const int pieces = cta_of(w.unit0 + HEAD + w.tiles - 1, total, (int)min(total, (long long)sm.share)) - blockIdx.x + 1;
-            __stcg(reinterpret_cast<float4 *>(sums_row(k, w.r.common, w.r.start + query, w.head * k.group + head) + D),
-                   pieces_end(w.r, (int)((k.tile_part - k.stream_part) / PSTRIDE) + (blockIdx.x * 2 + 1) * 2 * ROWS + c, 2 * ROWS, pieces));
-          }
-        } else if (!whole) __stcg(reinterpret_cast<float2 *>(slot + D), make_float2(m, l));
-        else if (k.a.lse) k.a.lse[(size_t)(w.r.start + query) * k.a.q_heads + w.head * k.group + head] = lse_of(m, l);
+      if (sums) {
+        asm volatile("bar.sync 5, 256;" ::: "memory");
+        const int rows = min(w.rows(k) - ROWS * x, ROWS);
+#pragma unroll 4
+        for (int c = warp; c < rows; c += 8)
+          __stcg(reinterpret_cast<float4 *>(slot(c + ROWS * x)) + lane, *reinterpret_cast<const float4 *>(sm.q[0] + c * 512 + ((lane ^ (c & 31)) << 4)));
+        asm volatile("bar.sync 5, 256;" ::: "memory");
       }
     }
     if (MODE != SHARED && whole) {
