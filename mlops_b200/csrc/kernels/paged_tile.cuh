@@ -577,11 +577,12 @@ template <int TYPE, int MODE> __device__ __forceinline__ void soften(const Call 
       if (x == 1 && shared) break;
       const bool sums = MODE == SHARED || !whole;  // (else outputs)
       auto slot = [&](int c) {  // where row c's sums go
-        if (MODE == SHARED && whole) {
-          int query, head;
-          split_column(k, 2 * ROWS * w.pair + c, query, head);
-          return sums_row(k, w.r.common, w.r.start + query, w.head * k.group + head);
-        }
+        if constexpr (MODE == SHARED)
+          if (whole) {
+            int query, head;
+            split_column(k, 2 * ROWS * w.pair + c, query, head);
+            return sums_row(k, w.r.common, w.r.start + query, w.head * k.group + head);
+          }
         return k.tile_part + (((size_t)blockIdx.x * 2 + (w.n0 ? 0 : 1)) * 2 * ROWS + c) * PSTRIDE;
       };
       if (warp_live[x]) {
