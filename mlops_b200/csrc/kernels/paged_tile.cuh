@@ -40,7 +40,8 @@ constexpr int WINDOW = 16;  // tiles whose blocks are looked up at a time
 constexpr int NO_TILE = -0x7fffffff;
 constexpr float TOP = 15.f, REST = 9.f;
 constexpr long long WAIT_CYCLES = 2000000000;
-constexpr uint32_t IDESC_S = tc::IDESC_F16, IDESC_O = tc::IDESC_F16 | (1u << 16);  // V: MN-major
+constexpr uint32_t IDESC_S = (1u << 4) | ((64u >> 3) << 17) | ((128u >> 4) << 24),  // N 64: the scores of half of a tile
+                    IDESC_O = tc::IDESC_F16 | (1u << 16);  // V: MN-major
 
 // a row of work and its part in this CTA's run: tiles of tokens n0 .. n1 - 1 of `tiles`
 template <int MODE> struct Row {
@@ -57,12 +58,11 @@ template <int MODE> struct __align__(1024) Smem {
   int left[2 * WINDOW];         // tokens of the request from the tile's first on
   uint64_t places_full[2], places_empty[2];  // of WINDOW tiles each
   uint64_t drained[2];  // the issuing threads' products, after a wait that gave up
-  uint64_t q_ready[2], k_full[STAGES], v_full[STAGES], k_empty[STAGES], v_empty[STAGES], s_ready[2], p_ready[2], o_done[2];
+  uint64_t q_ready[2], k_full[STAGES], v_full[STAGES], k_empty[STAGES], v_empty[STAGES], s_ready[2][2], p_ready[2][2], o_done[2][2];  // [X], [X][half of the tokens]
   uint8_t there[4][8];  // [tile of tokens % 4][block]: 1 where the table names a page
   float down[2][ROWS];      // the rows' factors
-  float exchange[2][ROWS];  // between the two threads of a row
+  float2 exchange[2][ROWS];  // (m, l) between the two threads of a row that both X have, l -1 where one has seen no tile
   int v_nan, nan_from[8];   // some V of the run has a NaN scale; [16 channels] of a row of work: the first token with one
-  uint8_t over[2][2][4];    // [turn % 2][half of the tokens][quarter of the rows]: a score passes 2^15
   Row<MODE> begin, row[8];  // the run's first row of work; the softmax warps' rows
   long long warp_sum[THREADS / 32];
   uint32_t tmem;
@@ -317,40 +317,44 @@ template <int MODE> __device__ __forceinline__ void issue(const Call &k, Smem<MO
     const uint8_t *const q = sm.q[shared ? 0 : x];
     int n = w.n0 + (shared && (w.n0 & 1) != x);
     auto at = [&](int n) { return row_at + (n - w.n0); };
-    auto scores = [&]() {
+    auto scores = [&](int h) {
       const int stage = at(n) % STAGES;
       tc::tc_fence_after();
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const uint32_t offset = (i >> 2) * SLAB + (i & 3) * 32;
-        tc::mma_f16(s_at, tc::smem_desc_at(q, offset), tc::smem_desc_at(sm.k[stage], offset), IDESC_S, i > 0);
+        tc::mma_f16(s_at + 64 * h, tc::smem_desc_at(q, offset), tc::smem_desc_at(sm.k[stage], offset + 64 * 128 * h), IDESC_S, i > 0);
       }
-      tc::mma_commit(&sm.s_ready[x]);
+      tc::mma_commit(&sm.s_ready[x][h]);
+      if (h == 0) return;
       tc::mma_commit(&sm.k_empty[stage]);
       if (n >= both) tc::mbar_arrive(&sm.k_empty[stage]);
     };
     ok = ok && wait(sm, &sm.q_ready[x], items++ & 1);
     if (n < end) {
       ok = ok && wait(sm, &sm.k_full[at(n) % STAGES], at(n) / STAGES & 1);
-      if (ok) scores();
+      if (ok) scores(0), scores(1);
     }
     for (bool first = true; n < end && ok; first = false) {
-      const int stage = at(n) % STAGES, alone = n >= both;
-      ok = wait(sm, &sm.v_full[stage], at(n) / STAGES & 1) && wait(sm, &sm.p_ready[x], mine & 1);
-      if (!ok) break;
-      tc::tc_fence_after();
+      const int stage = at(n) % STAGES, alone = n >= both, here = n;
+      ok = wait(sm, &sm.v_full[stage], at(n) / STAGES & 1);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) tc::mma_f16_ts(o_at, s_at + 64 * (i >> 2) + 8 * (i & 3), v_desc(sm.v[stage], i * 2048), IDESC_O, !first || i > 0);
-      tc::mma_commit(&sm.o_done[x]);
-      n += step;
-      if (n < end) {
-        // (P is in S's place: its product has to be through before the next scores)
-        ok = wait(sm, &sm.k_full[at(n) % STAGES], at(n) / STAGES & 1) && wait(sm, &sm.o_done[x], mine & 1);
-        if (ok) scores();
-        tc::mbar_arrive(&sm.v_empty[stage]);
-      } else {
-        tc::mma_commit(&sm.v_empty[stage]);
+      for (int h = 0; h < 2; ++h) {
+        ok = ok && wait(sm, &sm.p_ready[x][h], mine & 1);
+        if (!ok) break;
+        tc::tc_fence_after();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tc::mma_f16_ts(o_at, s_at + 64 * h + 8 * i, v_desc(sm.v[stage], (4 * h + i) * 2048), IDESC_O, !first || h > 0 || i > 0);
+        tc::mma_commit(&sm.o_done[x][h]);
+        n = here + step;
+        if (n < end) {  // the next tile's scores of this half (P is in their place: its products have to be through)
+          ok = (h || wait(sm, &sm.k_full[at(n) % STAGES], at(n) / STAGES & 1)) && wait(sm, &sm.o_done[x][h], mine & 1);
+          if (ok) scores(h);
+        }
       }
+      if (!ok) break;
+      if (n < end) tc::mbar_arrive(&sm.v_empty[stage]);
+      else tc::mma_commit(&sm.v_empty[stage]);
       if (alone) tc::mbar_arrive(&sm.v_empty[stage]);
       ++mine;
     }
@@ -359,17 +363,16 @@ template <int MODE> __device__ __forceinline__ void issue(const Call &k, Smem<MO
 }
 
 // ---- softmax --------------------------------------------------------------------------------------------------------------------
-// Two threads have a row: warps w and w + 4 share 32 rows, warp w the first 64 tokens of a tile (and channels of O), w + 4 the others.
+// Warps 0-3 have the rows of X = 0, a thread each, warps 4-7 those of X = 1. Where both X have the same rows, warps w and w + 4 join their sums, each for half of the channels.
 __device__ __forceinline__ void pair_meet(int quarter) { asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory"); }
 
-// Q's rows first .. first + 127 of the row of work as FP16 in `tile`, each times a power of two (q_factor) whose inverse goes to `down`; by eight warps, a
-// half-warp per row
-template <int TYPE, int MODE> __device__ __forceinline__ void load_q(const Call &k, const Row<MODE> &w, int first, uint8_t *tile, float *down, int warp, int lane) {
-  const int c = lane & 15, rows = w.rows(k);
-  uint4 raw[8];
+// Q's rows first + 32 quarter .. of the row of work as FP16 in `tile`, each times a power of two (q_factor) whose inverse goes to `down`; by a warp, a half-warp per row
+template <int TYPE, int MODE> __device__ __forceinline__ void load_q(const Call &k, const Row<MODE> &w, int first, uint8_t *tile, float *down, int quarter, int lane) {
+  const int c = lane & 15, rows = w.rows(k), line0 = 32 * quarter + (lane >> 4);
+  uint4 raw[16];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int line = 16 * warp + 2 * i + (lane >> 4);
+  for (int i = 0; i < 16; ++i) {
+    const int line = line0 + 2 * i;
     int query, head;
     split_column(k, 2 * ROWS * w.pair + first + line, query, head);
     raw[i] = make_uint4(0, 0, 0, 0);
@@ -378,22 +381,22 @@ template <int TYPE, int MODE> __device__ __forceinline__ void load_q(const Call 
                                                      (int64_t)(w.head * k.group + head) * k.a.q_head_stride) + c);
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int line = 16 * warp + 2 * i + (lane >> 4);
+  for (int i = 0; i < 16; ++i) {
+    const int line = line0 + 2 * i;
     const uint32_t word[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-    float2 f[4];
-    uint32_t top = 0, h[4];
+    uint32_t top = 0, h[4];  // two magnitudes' bits: in their order NaN is above infinity, infinity above the numbers
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = __vmaxu2(top, word[e] & 0x7fff7fffu);
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) top = __vmaxu2(top, __shfl_xor_sync(FULL, top, o));
+    const float2 tops = to_floats<TYPE>(top);
+    float inverse;
+    const float up = q_factor(max(__float_as_uint(tops.x), __float_as_uint(tops.y)), inverse);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      f[e] = to_floats<TYPE>(word[e]);
-      top = max(top, max(__float_as_uint(f[e].x) & 0x7fffffffu, __float_as_uint(f[e].y) & 0x7fffffffu));
+      const float2 f = to_floats<TYPE>(word[e]);
+      h[e] = from_floats<MLOPS_PAGED_FP16>(f.x * up, f.y * up);
     }
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(FULL, top, o));
-    float inverse;
-    const float up = q_factor(top, inverse);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) h[e] = from_floats<MLOPS_PAGED_FP16>(f[e].x * up, f[e].y * up);
     *reinterpret_cast<uint4 *>(tile + (c >> 3) * SLAB + line * 128 + (((c & 7) ^ (line & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
     if (c == 0) down[line] = inverse;
   }
@@ -409,7 +412,7 @@ template <int TYPE, int MODE> __device__ __forceinline__ void load_q(const Call 
   asm volatile("" : "+r"((r)[0]), "+r"((r)[1]), "+r"((r)[2]), "+r"((r)[3]), "+r"((r)[4]), "+r"((r)[5]), "+r"((r)[6]), "+r"((r)[7]), "+r"((r)[8]), "+r"((r)[9]), "+r"((r)[10]), "+r"((r)[11]), \
                     "+r"((r)[12]), "+r"((r)[13]), "+r"((r)[14]), "+r"((r)[15]), "+r"((r)[16]), "+r"((r)[17]), "+r"((r)[18]), "+r"((r)[19]), "+r"((r)[20]), "+r"((r)[21]), "+r"((r)[22]), \
                     "+r"((r)[23]), "+r"((r)[24]), "+r"((r)[25]), "+r"((r)[26]), "+r"((r)[27]), "+r"((r)[28]), "+r"((r)[29]), "+r"((r)[30]), "+r"((r)[31]))
-struct Half {  // of a row of scores
+struct Half {  // 64 of a row's scores
   uint32_t r[2][32];
   __device__ __forceinline__ void load(uint32_t at) {
     PAGED_LD32(at, r[0]);
@@ -448,42 +451,32 @@ struct Half {  // of a row of scores
   }
 };
 
-// a thread's part of a row of queries
+// a thread's row
 struct Line {
   float m, l, mult;
   int limit;     // the last token that the row sees
-  bool started;  // O holds sums
+  bool started;  // O holds sums, or will
 };
 
-// one tile of half X: scores in tensor memory at s become P there
+// 64 tokens of a tile, from first_token on: scores in tensor memory at s become P there. o_done: of the products with the 64 tokens before.
 template <int MODE>
-__device__ __forceinline__ bool take_tile(Smem<MODE> &sm, Line &q, uint32_t s, uint32_t o, int first_token, int low, uint2 there, uint64_t *o_done, uint32_t o_parity,
-                                          int line, int half, int turn) {
-  const int quarter = line >> 5, in_half = q.limit - first_token - 64 * half;
-  const bool mask = first_token + TOKENS - 1 > low || (there.x & there.y) != 0x01010101u;  // some row does not see all of the tile
-  const uint32_t blocks = half ? there.y : there.x;
+__device__ __forceinline__ bool take_half(Smem<MODE> &sm, Line &q, uint32_t s, uint32_t o, int first_token, int low, uint32_t blocks, uint64_t *o_done, uint32_t o_parity) {
+  const bool mask = first_token + 63 > low || blocks != 0x01010101u;  // some row does not see all of them
   Half x;
-  bool ok = true;
+  bool ok = true, over = true;
   float high, sum = 0.f;
-  bool over = true;
-  x.load(s + 64 * half);
-  if (mask) x.mask(in_half, blocks);
-  if (q.started) {  // as if m' may stay where it is; the pair finds out together whether it may
+  x.load(s);
+  if (mask) x.mask(q.limit - first_token, blocks);
+  if (q.started) {  // as if m' may stay where it is
     sum = x.exponentials(q.mult, q.m, high);
     over = __any_sync(FULL, high > TOP);
-    if ((line & 31) == 0) sm.over[turn & 1][half][quarter] = over;
-    pair_meet(quarter);
-    over |= sm.over[turn & 1][half ^ 1][quarter];
   }
   if (over) {
     if (q.started) {
-      x.load(s + 64 * half);
-      if (mask) x.mask(in_half, blocks);
+      x.load(s);
+      if (mask) x.mask(q.limit - first_token, blocks);
     }
-    const float own = x.largest() * q.mult;  // (mult is positive)
-    sm.exchange[half][line] = own;
-    pair_meet(quarter);
-    high = fmaxf(own, sm.exchange[half ^ 1][line]);
+    high = x.largest() * q.mult;  // (mult is positive)
     float keep = 1.f;
     if (high - q.m > TOP) {
       keep = ex2(q.m - (high - REST));
@@ -494,22 +487,22 @@ __device__ __forceinline__ bool take_tile(Smem<MODE> &sm, Line &q, uint32_t s, u
       ok = __all_sync(FULL, wait(sm, o_done, o_parity));
       tc::tc_fence_after();
 #pragma unroll 1
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 8; ++i) {
         uint32_t y[16];
-        tc::tmem_ld16(o + 64 * half + 16 * i, y);
+        tc::tmem_ld16(o + 16 * i, y);
         tc::tmem_ld_wait(y);
 #pragma unroll
         for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(__uint_as_float(y[e]) * keep);
-        tc::tmem_st8(o + 64 * half + 16 * i, reinterpret_cast<const uint32_t(&)[8]>(y[0]));
-        tc::tmem_st8(o + 64 * half + 16 * i + 8, reinterpret_cast<const uint32_t(&)[8]>(y[8]));
+        tc::tmem_st8(o + 16 * i, reinterpret_cast<const uint32_t(&)[8]>(y[0]));
+        tc::tmem_st8(o + 16 * i + 8, reinterpret_cast<const uint32_t(&)[8]>(y[8]));
       }
       tc::tmem_st_wait();
     }
     sum = x.exponentials(q.mult, q.m, high);
-    pair_meet(quarter);  // (the exchanged maxima have been read)
   }
   q.l += sum;
-  tc::tmem_st32(s + 64 * half, x.r[0]);  // (in the place of the thread's own scores)
+  q.started = true;
+  tc::tmem_st32(s, x.r[0]);  // (in the place of the thread's own scores)
   return ok;
 }
 
@@ -517,9 +510,9 @@ __device__ __forceinline__ bool take_tile(Smem<MODE> &sm, Line &q, uint32_t s, u
 __device__ __forceinline__ int cta_of(long long u, long long total, int ctas) { return (int)(((u + 1) * ctas - 1) / total); }
 
 template <int TYPE, int MODE> __device__ __forceinline__ void soften(const Call &k, Smem<MODE> &sm, long long hi, int warp, int lane) {
-  const int half = warp >> 2, line = 32 * (warp & 3) + lane;
-  const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-  uint32_t mine[2] = {0, 0}, at = 0;
+  const int x = warp >> 2, quarter = warp & 3, line = 32 * quarter + lane;
+  const uint32_t lanes = (uint32_t)(32 * quarter) << 16, s_at = sm.tmem + 128 * x + lanes, o_at = sm.tmem + 256 + lanes;
+  uint32_t mine = 0, at = 0;
   bool ok = true;
   Row<MODE> &w = sm.row[warp];  // (not in registers: they are all needed)
   if (lane == 0) w = sm.begin;
@@ -527,145 +520,138 @@ template <int TYPE, int MODE> __device__ __forceinline__ void soften(const Call 
   bool more;
   do {
     const bool shared = w.halves(k);
-    asm volatile("bar.sync 5, 256;" ::: "memory");  // (the last row of work's outputs have left Q's place)
-    load_q<TYPE, MODE>(k, w, 0, sm.q[0], sm.down[0], warp, lane);
-    if (!shared) load_q<TYPE, MODE>(k, w, ROWS, sm.q[1], sm.down[1], warp, lane);
-    fbla::fence_async_smem();
-    asm volatile("bar.sync 5, 256;" ::: "memory");
-    if (lane == 0) {
-      tc::mbar_arrive(&sm.q_ready[0]);
-      tc::mbar_arrive(&sm.q_ready[1]);
+    const int row0 = shared ? 0 : ROWS * x, rows = w.rows(k) - row0;  // the X's rows: row0 .. of the row of work
+    if (!shared || x == 0) {  // (the warp's part of Q's place: nobody else writes or, its products being through, reads there)
+      load_q<TYPE, MODE>(k, w, row0, sm.q[x], sm.down[x], quarter, lane);
+      fbla::fence_async_smem();
     }
-    Line q[2];
-    int low[2];
-    bool warp_live[2];
-    const float base = k.sl * __ldg(k.c.k_scale + w.head);
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int c = line + (shared ? 0 : ROWS * x), col = 2 * ROWS * w.pair + c;  // of the row of work, of the request
-      const bool live = c < w.rows(k);
-      warp_live[x] = c - lane < w.rows(k);
-      q[x] = Line{NOTHING, 0.f, fmaxf(base * sm.down[shared ? 0 : x][line], 1e-37f), live ? limit_of<MODE>(w.r, query_of(k, col)) : -1, false};  // (mult is not 0: masked scores are -infinity)
-      low[x] = limit_of<MODE>(w.r, query_of(k, col - lane));  // the smallest limit of the warp's rows
+    __syncwarp();
+    if (shared) pair_meet(quarter);
+    if (lane == 0 && (!shared || x == 0)) {
+      tc::mbar_arrive(&sm.q_ready[x]);
+      if (shared) tc::mbar_arrive(&sm.q_ready[1]);
     }
-    const int tiles0 = tiles_of_half(k, w, 0), tiles1 = tiles_of_half(k, w, 1), n0 = w.n0, n1 = w.n1;
+    const bool warp_live = 32 * quarter < rows;
+    const int col = 2 * ROWS * w.pair + row0 + line;  // of the item
+    Line q{NOTHING, 0.f, fmaxf(k.sl * __ldg(k.c.k_scale + w.head) * sm.down[shared ? 0 : x][line], 1e-37f),  // (mult is not 0: masked scores are -infinity)
+           line < rows ? limit_of<MODE>(w.r, query_of(k, col)) : -1, false};
+    const int low = limit_of<MODE>(w.r, query_of(k, col - lane));  // the smallest limit of the warp's rows
+    const Part part{shared, tiles_of_half(k, w, x)};
+    const int n0 = w.n0, n1 = w.n1;
+    bool any = false;
 #pragma unroll 1
     for (int n = n0; n < n1; ++n, ++at) {
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        if (!Part{shared, x ? tiles1 : tiles0}.has(n, x)) continue;
-        ok = __all_sync(FULL, ok && wait(sm, &sm.s_ready[x], mine[x] & 1));
+      if (!part.has(n, x)) continue;
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        ok = __all_sync(FULL, ok && wait(sm, &sm.s_ready[x][h], mine & 1));
         tc::tc_fence_after();
-        if (warp_live[x])  // (after a wait that gave up too: the warps of a pair meet)
-          ok &= take_tile(sm, q[x], sm.tmem + 128 * x + lanes, sm.tmem + 256 + 128 * x + lanes, TOKENS * n, low[x], *reinterpret_cast<const uint2 *>(sm.there[at & 3]),
-                         &sm.o_done[x], (mine[x] - 1) & 1, line, half, (int)(mine[0] + mine[1]));
+        if (warp_live)
+          ok &= take_half(sm, q, s_at + 64 * h, o_at + 128 * x, TOKENS * n + 64 * h, low, *reinterpret_cast<const uint32_t *>(sm.there[at & 3] + 4 * h), &sm.o_done[x][h ^ 1],
+                          h ? mine & 1 : (mine - 1) & 1);
         tc::tc_fence_before();
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&sm.p_ready[x]);
-        q[x].started = true;
-        ++mine[x];
+        if (lane == 0) tc::mbar_arrive(&sm.p_ready[x][h]);
       }
+      any = true;
+      ++mine;
     }
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-      if (q[x].started) ok = __all_sync(FULL, ok && wait(sm, &sm.o_done[x], (mine[x] - 1) & 1));
+    if (any) ok = __all_sync(FULL, ok && wait(sm, &sm.o_done[x][1], (mine - 1) & 1));
     tc::tc_fence_after();
-    const bool whole = w.n0 == 0 && w.n1 == w.tiles;
-    const float v_scale = __ldg(k.c.v_scale + w.head);
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      if (x == 1 && shared) break;
-      const bool sums = MODE == SHARED || !whole;  // (else outputs)
-      auto slot = [&](int c) {  // where row c's sums go
-        if constexpr (MODE == SHARED)
-          if (whole) {
-            int query, head;
-            split_column(k, 2 * ROWS * w.pair + c, query, head);
-            return sums_row(k, w.r.common, w.r.start + query, w.head * k.group + head);
-          }
-        return k.tile_part + (((size_t)blockIdx.x * 2 + (w.n0 ? 0 : 1)) * 2 * ROWS + c) * PSTRIDE;
-      };
-      if (warp_live[x]) {
-        float m = q[x].m, l = q[x].l, keep = q[x].started ? 1.f : 0.f, other = 0.f;
-        if (shared) {  // both halves' sums are of these rows
-          m = fmaxf(q[0].m, q[1].m);
-          l = q[0].l * ex2(q[0].m - m) + q[1].l * ex2(q[1].m - m);
-          keep = q[0].started ? ex2(q[0].m - m) : 0.f;
-          other = q[1].started ? ex2(q[1].m - m) : 0.f;
+
+    // Outputs of whole rows in 16 bits, or sums: through the warp's part of Q's place, from where a half-warp or less stores a row at a time
+    const bool whole = w.n0 == 0 && w.n1 == w.tiles, sums = MODE == SHARED || !whole;
+    float m = q.m, l = q.l, keep = any ? 1.f : 0.f, other = 0.f;
+    if (!ok) l = __int_as_float(0x7fc00000);  // (a wait that gave up: the rows are NaN)
+    if (shared) {  // both X's sums are of these rows; this thread has 64 of the channels
+      sm.exchange[x][line] = make_float2(m, any ? l : -1.f);
+      tc::tc_fence_before();
+      pair_meet(quarter);
+      tc::tc_fence_after();
+      const float2 y = sm.exchange[x ^ 1][line];
+      const bool both = y.y != -1.f;
+      const float top = both ? fmaxf(m, y.x) : m;
+      keep = any ? ex2(m - top) : 0.f;
+      other = both ? ex2(y.x - top) : 0.f;
+      l = (any ? l * keep : 0.f) + (both ? y.y * other : 0.f);
+      m = top;
+    }
+    const float f = l == 0.f ? 0.f : __ldg(k.c.v_scale + w.head) / l;
+    auto slot = [&](int c) {  // where row c's sums go
+      if constexpr (MODE == SHARED)
+        if (whole) {
+          int query, head;
+          split_column(k, 2 * ROWS * w.pair + c, query, head);
+          return sums_row(k, w.r.common, w.r.start + query, w.head * k.group + head);
         }
-        pair_meet(line >> 5);
-        sm.exchange[half][line] = l;
-        pair_meet(line >> 5);
-        l = half ? sm.exchange[0][line] + l : l + sm.exchange[1][line];
-        if (!ok) l = __int_as_float(0x7fc00000);  // (a wait that gave up: the rows are NaN)
-        const int c = line + ROWS * x;
-        const float f = l == 0.f ? 0.f : v_scale / l;
+      return k.tile_part + (((size_t)blockIdx.x * 2 + (w.n0 ? 0 : 1)) * 2 * ROWS + c) * PSTRIDE;
+    };
+    uint8_t *const place = sm.q[x] + 32 * quarter * 128;  // 16-byte piece i < 8 of the warp's row r at r * 128 + 16 (i ^ r % 8), pieces from 8 on a slab further
+    const int wide = sums ? 4 : 8, pieces = !sums && shared ? 8 : 16, span = wide * pieces;  // channels of a piece, pieces of a row at a time, channels at a time
+    if (warp_live) {
 #pragma unroll 1
-        for (int i = 0; i < 4; ++i) {
-          const int ch = 64 * half + 16 * i;
+      for (int ch0 = shared ? 64 * x : 0; ch0 < (shared ? 64 * x + 64 : D); ch0 += span) {
+#pragma unroll 1
+        for (int i = 0; i < span / 16; ++i) {
           uint32_t r[16], y[16];
-          tc::tmem_ld16(sm.tmem + 256 + 128 * x + lanes + ch, r);
-          tc::tmem_ld_wait(r);
           float o[16];
+          tc::tmem_ld16(o_at + (shared ? 0 : 128 * x) + ch0 + 16 * i, r);
+          tc::tmem_ld_wait(r);
+          const float a = shared && x ? other : keep, b = shared && x ? keep : other;  // of X = 0's sums, of X = 1's where the rows are both's
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] = keep == 0.f ? 0.f : __uint_as_float(r[e]) * keep;  // (a half without tiles has nothing in its accumulator)
+          for (int e = 0; e < 16; ++e) o[e] = a == 0.f ? 0.f : __uint_as_float(r[e]) * a;  // (an X without tiles has nothing in its accumulator)
           if (shared) {
-            tc::tmem_ld16(sm.tmem + 256 + 128 + lanes + ch, y);
+            tc::tmem_ld16(o_at + 128 + ch0 + 16 * i, y);
             tc::tmem_ld_wait(y);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = other == 0.f ? o[e] : fmaf(__uint_as_float(y[e]), other, o[e]);
+            for (int e = 0; e < 16; ++e) o[e] = b == 0.f ? o[e] : fmaf(__uint_as_float(y[e]), b, o[e]);
           }
-          // through Q's place, from where rows are stored as a whole: in 16 bits both X's, sums one X after the other (16-byte piece i of a row at i ^ row % 32)
+          auto piece = [&](int p) { return reinterpret_cast<uint4 *>(place + (p >> 3) * SLAB + lane * 128 + (((p & 7) ^ (lane & 7)) << 4)); };
           if (sums) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              *reinterpret_cast<float4 *>(sm.q[0] + line * 512 + ((((ch >> 2) + e) ^ lane) << 4)) = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            for (int e = 0; e < 4; ++e) *reinterpret_cast<float4 *>(piece(4 * i + e)) = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
           } else {
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-              *reinterpret_cast<uint4 *>(sm.q[x] + half * SLAB + line * 128 + (((2 * i + e) ^ (line & 7)) << 4)) =
-                  pack8<TYPE>(make_float4(o[8 * e] * f, o[8 * e + 1] * f, o[8 * e + 2] * f, o[8 * e + 3] * f),
-                              make_float4(o[8 * e + 4] * f, o[8 * e + 5] * f, o[8 * e + 6] * f, o[8 * e + 7] * f));
+              *piece(2 * i + e) = pack8<TYPE>(make_float4(o[8 * e] * f, o[8 * e + 1] * f, o[8 * e + 2] * f, o[8 * e + 3] * f),
+                                              make_float4(o[8 * e + 4] * f, o[8 * e + 5] * f, o[8 * e + 6] * f, o[8 * e + 7] * f));
           }
         }
-        if (half == 0 && c < w.rows(k)) {
-          int query, head;
-          split_column(k, 2 * ROWS * w.pair + c, query, head);
-          if constexpr (MODE == SHARED) {
-            if (whole) __stcg(reinterpret_cast<float4 *>(slot(c) + D), row_end(w.r, m, l));
-            else __stcg(reinterpret_cast<float2 *>(slot(c) + D), make_float2(m, l));
-            if (!whole && w.n0 == 0) {
-              const long long total = sm.before[items_of<MODE>(k)];
-              const int pieces = cta_of(w.unit0 + HEAD + w.tiles - 1, total, (int)min(total, (long long)sm.share)) - blockIdx.x + 1;
-              __stcg(reinterpret_cast<float4 *>(sums_row(k, w.r.common, w.r.start + query, w.head * k.group + head) + D),
-                     pieces_end(w.r, (int)((k.tile_part - k.stream_part) / PSTRIDE) + (blockIdx.x * 2 + 1) * 2 * ROWS + c, 2 * ROWS, pieces));
-            }
-          } else if (!whole) __stcg(reinterpret_cast<float2 *>(slot(c) + D), make_float2(m, l));
-          else if (k.a.lse) k.a.lse[(size_t)(w.r.start + query) * k.a.q_heads + w.head * k.group + head] = lse_of(m, l);
-        }
-      }
-      if (sums) {
-        asm volatile("bar.sync 5, 256;" ::: "memory");
-        const int rows = min(w.rows(k) - ROWS * x, ROWS);
+        __syncwarp();
+        const int p = lane & (pieces - 1), live = min(rows - 32 * quarter, 32);
 #pragma unroll 4
-        for (int c = warp; c < rows; c += 8)
-          __stcg(reinterpret_cast<float4 *>(slot(c + ROWS * x)) + lane, *reinterpret_cast<const float4 *>(sm.q[0] + c * 512 + ((lane ^ (c & 31)) << 4)));
-        asm volatile("bar.sync 5, 256;" ::: "memory");
+        for (int r = lane / pieces; r < live; r += 32 / pieces) {
+          const uint4 v = *reinterpret_cast<const uint4 *>(place + (p >> 3) * SLAB + r * 128 + (((p & 7) ^ (r & 7)) << 4));
+          const int c = row0 + 32 * quarter + r;
+          if (sums) {
+            __stcg(reinterpret_cast<uint4 *>(slot(c) + ch0) + p, v);
+          } else {
+            int query, head;
+            split_column(k, 2 * ROWS * w.pair + c, query, head);
+            reinterpret_cast<uint4 *>(out_row(k, w.r.start + query, w.head * k.group + head) + ch0)[p] = v;
+          }
+        }
+        __syncwarp();
       }
     }
-    if (MODE != SHARED && whole) {
-      asm volatile("bar.sync 5, 256;" ::: "memory");
-      const int rows = w.rows(k), ch = lane & 15;
-#pragma unroll 4
-      for (int c = 2 * warp + (lane >> 4); c < rows; c += 16) {
-        const int at = c & (ROWS - 1);
-        int query, head;
-        split_column(k, 2 * ROWS * w.pair + c, query, head);
-        reinterpret_cast<uint4 *>(out_row(k, w.r.start + query, w.head * k.group + head))[ch] =
-            *reinterpret_cast<const uint4 *>(sm.q[c >> 7] + (ch >> 3) * SLAB + at * 128 + (((ch & 7) ^ (at & 7)) << 4));
-      }
+    if (line < rows && (!shared || x == 0)) {
+      const int c = row0 + line;
+      int query, head;
+      split_column(k, 2 * ROWS * w.pair + c, query, head);
+      if constexpr (MODE == SHARED) {
+        if (whole) __stcg(reinterpret_cast<float4 *>(slot(c) + D), row_end(w.r, m, l));
+        else __stcg(reinterpret_cast<float2 *>(slot(c) + D), make_float2(m, l));
+        if (!whole && w.n0 == 0) {
+          const long long total = sm.before[items_of<MODE>(k)];
+          const int pieces = cta_of(w.unit0 + HEAD + w.tiles - 1, total, (int)min(total, (long long)sm.share)) - blockIdx.x + 1;
+          __stcg(reinterpret_cast<float4 *>(sums_row(k, w.r.common, w.r.start + query, w.head * k.group + head) + D),
+                 pieces_end(w.r, (int)((k.tile_part - k.stream_part) / PSTRIDE) + (blockIdx.x * 2 + 1) * 2 * ROWS + c, 2 * ROWS, pieces));
+        }
+      } else if (!whole) __stcg(reinterpret_cast<float2 *>(slot(c) + D), make_float2(m, l));
+      else if (k.a.lse) k.a.lse[(size_t)(w.r.start + query) * k.a.q_heads + w.head * k.group + head] = lse_of(m, l);
     }
     tc::tc_fence_before();
+    if (shared) pair_meet(quarter);  // (both have read both X's sums)
     __syncwarp();
     more = lane == 0 && next_row(k, sm.before, hi, w);
     more = __shfl_sync(FULL, (int)more, 0);
@@ -780,10 +766,12 @@ template <int TYPE, int MODE> __global__ void __launch_bounds__(THREADS, 1) tile
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
-      fbla::mbar_init(&sm.q_ready[i], PRODUCER0);
-      fbla::mbar_init(&sm.s_ready[i], 1);
-      fbla::mbar_init(&sm.p_ready[i], PRODUCER0);
-      fbla::mbar_init(&sm.o_done[i], 1);
+      fbla::mbar_init(&sm.q_ready[i], PRODUCER0 / 2);
+      for (int h = 0; h < 2; ++h) {
+        fbla::mbar_init(&sm.s_ready[i][h], 1);
+        fbla::mbar_init(&sm.p_ready[i][h], PRODUCER0 / 2);
+        fbla::mbar_init(&sm.o_done[i][h], 1);
+      }
       fbla::mbar_init(&sm.k_full[i], PRODUCERS);
       fbla::mbar_init(&sm.v_full[i], PRODUCERS);
       fbla::mbar_init(&sm.k_empty[i], 2);
