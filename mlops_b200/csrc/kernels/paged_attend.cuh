@@ -102,19 +102,20 @@ template <int MODE> __device__ __forceinline__ Request<MODE> request(const Call 
     r.start = r.n = r.skip = r.tokens = 0;
     r.at = -1;
     r.common = true;
+    const int start = k.a.starts ? min(max(__ldg(k.a.starts + x.first), 0), k.a.tokens) : x.first, end = k.a.starts ? min(__ldg(k.a.starts + x.end), k.a.tokens) : x.end;
     for (int b = x.first; b < x.end && x.tokens > 0; ++b) {
       if (!takes_part(plain_request(k, b), x.tokens)) continue;
       // (the rows of requests that do not take part are computed with the others' and not used)
       r.row = b;
       r.tokens = x.tokens;
       r.at = x.tokens - 1;
-      r.start = k.a.starts ? min(max(__ldg(k.a.starts + x.first), 0), k.a.tokens) : x.first;
-      r.n = max((k.a.starts ? min(__ldg(k.a.starts + x.end), k.a.tokens) : x.end) - r.start, 0);
+      r.start = start;
+      r.n = max(end - start, 0);
       break;
     }
   } else {
     const int b = item - k.common.groups;
-    const Plain p = plain_request(k, b);
+    const Plain p = plain_request(k, b);  // (its loads beside those of the groups)
     r.start = p.start;
     r.n = p.n;
     r.at = p.at;
@@ -191,7 +192,12 @@ template <int MODE> __device__ __forceinline__ int tiles_of(const Call &k, const
 template <int MODE> __device__ __forceinline__ long long tile_units(const Call &k, const Request<MODE> &r) {
   long long n = 0;
   if (r.tokens > 0 && r.n * k.group > k.wide) {
-    for (int p = 0; TILE_ROWS * p < rows_of(k, r); ++p) n += HEAD + tiles_of<MODE>(k, r, p);
+    const int pairs = (rows_of(k, r) + TILE_ROWS - 1) / TILE_ROWS;
+    bool alike = MODE == WHOLE;  // all of the item's rows see the same tokens
+    if constexpr (MODE == SHARED) alike = r.common;
+    if (alike) n = (long long)pairs * (HEAD + tiles_of<MODE>(k, r, 0));
+    else
+      for (int p = 0; p < pairs; ++p) n += HEAD + tiles_of<MODE>(k, r, p);
     n *= k.c.kv_heads;
   }
   return n;
@@ -206,7 +212,7 @@ __device__ __forceinline__ int tile_share(const Call &k, long long tiles, int un
   if (tiles == 0 || units == 0 || sms < 2 * PAIR) return tiles ? sms : 0;
   uint32_t best = ~0u;
   for (int n = PAIR * (1 + lane); n < sms; n += 32 * PAIR) {
-    const float a = 36e3f + 4400.f * ceilf((float)tiles / n), b = 40e3f + (k.narrow == 8 ? 250.f : 360.f) * (float)units / (sms - n);
+    const float a = 36e3f + 4400.f * ceilf(__fdividef((float)tiles, n)), b = 40e3f + (k.narrow == 8 ? 250.f : 360.f) * __fdividef((float)units, sms - n);
     best = min(best, (uint32_t)fminf(fmaxf(a, b) * 0.0625f, 2097151.f) << 11 | n);
   }
   return __reduce_min_sync(FULL, best) & 2047;

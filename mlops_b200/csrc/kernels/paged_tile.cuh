@@ -87,6 +87,9 @@ __device__ __forceinline__ uint64_t v_desc(const void *tile, uint32_t byte_offse
   return tc::smem_desc_at(tile, byte_offset) | ((uint64_t)(SLAB >> 4) << 16);
 }
 
+// a / b for a >= 0, b > 0: in 32 bits where both have no more
+__device__ __forceinline__ long long divide(long long a, long long b) { return (a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b); }
+
 // the first row of work of the run [lo, hi), found by a warp
 template <int MODE> __device__ __forceinline__ Row<MODE> first_row(const Call &k, const long long *before, long long lo, long long hi, int lane) {
   Row<MODE> w;
@@ -97,8 +100,8 @@ template <int MODE> __device__ __forceinline__ Row<MODE> first_row(const Call &k
   }
   w.b = a;
   w.r = request<MODE>(k, a);
-  const long long per_head = (before[a + 1] - before[a]) / k.c.kv_heads, x = lo - before[a];
-  w.head = (int)(x / per_head);
+  const long long per_head = divide(before[a + 1] - before[a], k.c.kv_heads), x = lo - before[a];
+  w.head = (int)divide(x, per_head);
   long long rest = x - w.head * per_head;
   for (int pair0 = 0;; pair0 += 32) {  // 32 pairs at a time
     const int pair = pair0 + lane, units = 2 * ROWS * pair < rows_of(k, w.r) ? HEAD + tiles_of<MODE>(k, w.r, pair) : 0;
@@ -217,16 +220,16 @@ template <int MODE> __device__ __forceinline__ void look_up(const Call &k, Smem<
       const int number = 8 * n + 4 * half;
       const int in_row = number + first_token<MODE>(w.r) / BT;
       int column = in_row / per_page, at = in_row - column * per_page;
+      int page[4], in_page[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint8_t *block = nullptr;
-        if ((number + j) * BT < w.r.tokens) {
-          const int page = __ldg(entries + column);
-          if ((unsigned)page < (unsigned)k.c.pages) block = head + (size_t)page * k.c.page_stride + (size_t)at * BLOCK_BYTES;
-        }
-        sm.block[tile % (2 * WINDOW)][4 * half + j] = block;
+      for (int j = 0; j < 4; ++j) {  // (all on their way before the first is used)
+        page[j] = (number + j) * BT < w.r.tokens ? __ldg(entries + column) : -1;
+        in_page[j] = at;
         if (++at == per_page) at = 0, ++column;
       }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        sm.block[tile % (2 * WINDOW)][4 * half + j] = (unsigned)page[j] < (unsigned)k.c.pages ? head + (size_t)page[j] * k.c.page_stride + (size_t)in_page[j] * BLOCK_BYTES : nullptr;
     }
     __syncwarp();
     if (lane == 0) tc::mbar_arrive(&sm.places_full[i & 1]);
@@ -366,39 +369,53 @@ template <int MODE> __device__ __forceinline__ void issue(const Call &k, Smem<MO
 // Warps 0-3 have the rows of X = 0, a thread each, warps 4-7 those of X = 1. Where both X have the same rows, warps w and w + 4 join their sums, each for half of the channels.
 __device__ __forceinline__ void pair_meet(int quarter) { asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory"); }
 
-// Q's rows first + 32 quarter .. of the row of work as FP16 in `tile`, each times a power of two (q_factor) whose inverse goes to `down`; by a warp, a half-warp per row
+// the larger magnitudes of two pairs of 16-bit numbers (NaN where both are)
+template <int TYPE> __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+  uint32_t y;
+  if (TYPE == MLOPS_PAGED_BF16) asm("{.reg .b32 x;\n\tabs.bf16x2 x, %2;\n\tmax.bf16x2 %0, %1, x;}" : "=r"(y) : "r"(a), "r"(b));
+  else asm("{.reg .b32 x;\n\tabs.f16x2 x, %2;\n\tmax.f16x2 %0, %1, x;}" : "=r"(y) : "r"(a), "r"(b));
+  return y;
+}
+
+// Q's rows first + 32 quarter .. of the row of work as FP16 in `tile`, each times a power of two (q_factor) whose inverse goes to `down`; by a warp, four lanes of 32 channels each
+// per row, all loads ahead of the arithmetic
 template <int TYPE, int MODE> __device__ __forceinline__ void load_q(const Call &k, const Row<MODE> &w, int first, uint8_t *tile, float *down, int quarter, int lane) {
-  const int c = lane & 15, rows = w.rows(k), line0 = 32 * quarter + (lane >> 4);
-  uint4 raw[16];
+  const int part = lane & 3, rows = w.rows(k) - first - 32 * quarter, line0 = 32 * quarter + (lane >> 2);
+  int query, head;
+  split_column(k, 2 * ROWS * w.pair + first + 32 * quarter + min(lane, max(rows - 1, 0)), query, head);
+  const long long mine = (int64_t)(w.r.start + query) * k.a.q_token_stride + (int64_t)(w.head * k.group + head) * k.a.q_head_stride;  // of the lane's row
+  uint4 raw[4][4];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int line = line0 + 2 * i;
-    int query, head;
-    split_column(k, 2 * ROWS * w.pair + first + line, query, head);
-    raw[i] = make_uint4(0, 0, 0, 0);
-    if (first + line < rows)
-      raw[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(k.a.q) + (int64_t)(w.r.start + query) * k.a.q_token_stride +
-                                                     (int64_t)(w.head * k.group + head) * k.a.q_head_stride) + c);
+  for (int i = 0; i < 4; ++i) {
+    const int row = 8 * i + (lane >> 2);
+    const uint4 *const from = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(k.a.q) + __shfl_sync(FULL, mine, row)) + 4 * part;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) raw[i][e] = row < rows ? __ldg(from + e) : make_uint4(0, 0, 0, 0);
   }
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int line = line0 + 2 * i;
-    const uint32_t word[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-    uint32_t top = 0, h[4];  // two magnitudes' bits: in their order NaN is above infinity, infinity above the numbers
+  for (int i = 0; i < 4; ++i) {
+    const int line = line0 + 8 * i;
+    uint32_t tops = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) top = __vmaxu2(top, word[e] & 0x7fff7fffu);
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) top = __vmaxu2(top, __shfl_xor_sync(FULL, top, o));
-    const float2 tops = to_floats<TYPE>(top);
+    for (int e = 0; e < 4; ++e) tops = larger<TYPE>(larger<TYPE>(larger<TYPE>(larger<TYPE>(tops, raw[i][e].x), raw[i][e].y), raw[i][e].z), raw[i][e].w);
+    const float2 t = to_floats<TYPE>(tops);
+    float top = fmaxf(t.x, t.y);
+    top = fmaxf(top, __shfl_xor_sync(FULL, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(FULL, top, 2));
     float inverse;
-    const float up = q_factor(max(__float_as_uint(tops.x), __float_as_uint(tops.y)), inverse);
+    const float up = q_factor(__float_as_uint(top) & 0x7fffffffu, inverse);
+    if (part == 0) down[line] = inverse;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float2 f = to_floats<TYPE>(word[e]);
-      h[e] = from_floats<MLOPS_PAGED_FP16>(f.x * up, f.y * up);
+      const uint32_t word[4] = {raw[i][e].x, raw[i][e].y, raw[i][e].z, raw[i][e].w};
+      uint32_t h[4];
+#pragma unroll
+      for (int f = 0; f < 4; ++f) {
+        const float2 x = __fmul2_rn(to_floats<TYPE>(word[f]), make_float2(up, up));
+        h[f] = from_floats<MLOPS_PAGED_FP16>(x.x, x.y);
+      }
+      *reinterpret_cast<uint4 *>(tile + (part >> 1) * SLAB + line * 128 + (((4 * (part & 1) + e) ^ (line & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
     }
-    *reinterpret_cast<uint4 *>(tile + (c >> 3) * SLAB + line * 128 + (((c & 7) ^ (line & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-    if (c == 0) down[line] = inverse;
   }
 }
 
@@ -816,7 +833,8 @@ template <int TYPE, int MODE> __global__ void __launch_bounds__(THREADS, 1) tile
   }
   if (tid == 0) sm.before[items] = total;
   if (MODE == SHARED) {
-    if (others) atomicAdd(&sm.others, others);
+    others = (int)__reduce_add_sync(FULL, (unsigned)others);
+    if (others && lane == 0) atomicAdd(&sm.others, others);
     __syncthreads();
     if (warp == 0) {
       const int share = tile_share(k, total, sm.others, gridDim.x, lane);
