@@ -204,15 +204,15 @@ template <int MODE> __device__ __forceinline__ long long tile_units(const Call &
 }
 
 // SHARED: both kernels have work that does not wait for the other's, one bound by its products, the other by memory, on multiprocessors of their own: how many of `sms` are the tile
-// kernel's, so that both end together. Cycles of a unit and beside the units, as measured: 4 400 and 36 000; 250 or 360 (tiles of 8 or 16 columns) and 40 000, with the start behind the tile
-// kernel's CTAs that have nothing to do. In pairs: both kernels are launched in clusters of two, which lie on two multiprocessors of a kind of their own (TPC); one of each kernel there slow
-// each other down, the tile kernel's to 0.78 and the stream's to 0.7 of their rate (256 requests behind 32 768 common tokens, us: 306, in pairs 220). By one warp; any number is right.
+// kernel's, so that both end together. Cycles of a unit and beside the units, as measured: 4 100 and 45 000; 280 or 450 (tiles of 8 or 16 columns) and 32 000, with the start behind the
+// tile kernel's CTAs that have nothing to do. In pairs: both kernels are launched in clusters of two, which lie on two neighbouring multiprocessors; one of each kernel there slow each other
+// down, the tile kernel's to 0.78 and the stream's to 0.7 of their rate (256 requests behind 32 768 common tokens, us: 306, in pairs 230). By one warp; any number is right.
 constexpr int PAIR = 2;
 __device__ __forceinline__ int tile_share(const Call &k, long long tiles, int units, int sms, int lane) {
   if (tiles == 0 || units == 0 || sms < 2 * PAIR) return tiles ? sms : 0;
   uint32_t best = ~0u;
   for (int n = PAIR * (1 + lane); n < sms; n += 32 * PAIR) {
-    const float a = 36e3f + 4400.f * ceilf(__fdividef((float)tiles, n)), b = 40e3f + (k.narrow == 8 ? 250.f : 360.f) * __fdividef((float)units, sms - n);
+    const float a = 45e3f + 4100.f * ceilf(__fdividef((float)tiles, n)), b = 32e3f + (k.narrow == 8 ? 280.f : 450.f) * __fdividef((float)units, sms - n);
     best = min(best, (uint32_t)fminf(fmaxf(a, b) * 0.0625f, 2097151.f) << 11 | n);
   }
   return __reduce_min_sync(FULL, best) & 2047;
