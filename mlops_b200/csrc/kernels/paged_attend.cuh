@@ -72,8 +72,11 @@ __device__ __forceinline__ Plain plain_request(const Call &k, int b) {
   r.tokens = (int)min((long long)length, (long long)k.a.width * k.c.page_size);
   return r;
 }
-// group g's requests, and their common tokens: whole pages of the table, none for a single request. (Whether a request's first query sees them all, so that it takes
+// group g's requests, and their common tokens: whole pages of the table, none for a single request, nor for requests of more than LONE columns on average, which fill rows of work by
+// themselves: they take their tokens in one row instead of two that are joined (16 requests behind 6 000 common tokens, us by themselves and together: 260 columns each 216 and 196, 512 287 and
+// 370; 256 fill rows just so: 165 and 201). (Whether a request's first query sees them all, so that it takes
 // part, is asked for each.)
+constexpr int LONE = 384;
 struct Group {
   int first, end, tokens;
 };
@@ -86,6 +89,7 @@ __device__ __forceinline__ Group group_at(const Call &k, int g) {
   if (x.end - x.first > 1) {
     const int pages = max(__ldg(k.common.tokens + g), 0) / k.c.page_size;
     if (pages <= k.a.width) x.tokens = pages * k.c.page_size;  // (no request has more than its row of the table can name)
+    if (k.a.starts && (long long)(__ldg(k.a.starts + x.end) - __ldg(k.a.starts + x.first)) * k.group > (long long)LONE * (x.end - x.first)) x.tokens = 0;
   }
   return x;
 }
