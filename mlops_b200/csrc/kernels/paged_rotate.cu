@@ -2,9 +2,13 @@
 // quantised into the cache's slots.
 //
 // Rotation of a pair (x, y) by (c, s): (x c - y s, y c + x s). q takes it in FP32, rounded once to its type at the end. A stored code of k asks on which side of a border a value
-// lies, so k's rotation is exact before its one rounding to 16 bits: each product with its error (an FMA gives it), each sum with its (TwoSum: D. Knuth, The Art of Computer
-// Programming 2, 4.2.2), and where the rounded sum is not exact its last bit is set, so that rounding it again to 16 bits never meets a halfway case that is none (rounding to odd: S. Boldo, G.
-// Melquiond, Emulation of FMA and correctly rounded sums, 2008). What is stored is, bit for bit, what mlops_paged_append stores of the correctly rounded rotation.
+// lies, so k's rotation is correctly rounded to 16 bits: r = fl(x c - fl(y s)) is off by at most 2^-24 (|y s| + |r|), and where all numbers so near to r round to the same one, that is it. Where they do not
+// (some 2^-14 of the elements), the thread takes all of its products with their errors (an FMA gives them) and sums with theirs (TwoSum: D. Knuth, The
+// Art of Computer Programming 2, 4.2.2), and sets the last bit of a rounded sum that is not exact, so that rounding it again to 16 bits never meets a halfway case that is none (rounding to odd: S. Boldo,
+// G. Melquiond, Emulation of FMA and correctly rounded sums, 2008). What is stored is, bit for bit, what mlops_paged_append stores of the correctly rounded rotation.
+//
+// Warps have units of two kinds, dealt evenly over each other so that the ones' memory and the others' arithmetic share a multiprocessor: a token's query heads, eight at a time, with the
+// token's angles in registers; eight (token, KV head), four threads each.
 #include "paged_store.cuh"
 #include <type_traits>
 
@@ -13,12 +17,15 @@ namespace {
 
 constexpr int WARPS = 8, THREADS = 32 * WARPS, CTAS = 2;
 constexpr int SLICE = 8;  // heads that a warp has at once: four threads of 32 channels each
+constexpr int AHEAD = 2;  // slices of queries on their way at once
 
 struct Turn {
   mlops_paged_rotate_args a;
   Store s;
   Divisor by_parts;
-  int q_slices, slices, parts, span;  // slices of 8 query heads, of 8 KV heads behind them; a warp's unit is up to `span` slices of a token, which has `parts` units
+  int q_slices, parts, span;   // slices of 8 query heads; a unit is up to `span` slices of a token, which has `parts` units
+  int units;                   // in all
+  uint64_t kv_step;            // 2^32 times the share of (token, KV head) units, rounded up: of the first u units floor(u kv_step / 2^32) are of that kind
 };
 
 // channels of a thread: two blocks of 16, which hold the pairs' two halves or whole pairs
@@ -47,24 +54,63 @@ __device__ __forceinline__ float turned_exactly(float x, float c, float y, float
   if (rest != 0.f && !(bits & 1) && (bits & 0x7f800000u) != 0x7f800000u) bits += (rest > 0.f) == (r > 0.f) ? 1u : ~0u;
   return __uint_as_float(bits);
 }
-template <bool EXACT> __device__ __forceinline__ float2 turn(float x, float y, float c, float s) {
-  if (EXACT) return make_float2(turned_exactly(x, c, y, s), turned_exactly(y, c, x, -s));
-  return make_float2(__fmaf_rn(x, c, -__fmul_rn(y, s)), __fmaf_rn(y, c, __fmul_rn(x, s)));
-}
-template <int TYPE, bool NEIGHBOURS, bool EXACT> __device__ __forceinline__ void rotate(Two &t, const float (&c)[16], const float (&s)[16]) {
+// a thread's angles, of its 16 pairs
+struct Angles {
+  float c[16], s[16];
+  __device__ __forceinline__ void load(const float *row, int half, int t) {
+    const float4 *const from = reinterpret_cast<const float4 *>(row + 16 * t);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 x = __ldg(from + i), y = __ldg(from + 4 * half + i);
+      c[4 * i] = x.x; c[4 * i + 1] = x.y; c[4 * i + 2] = x.z; c[4 * i + 3] = x.w;
+      s[4 * i] = y.x; s[4 * i + 1] = y.y; s[4 * i + 2] = y.z; s[4 * i + 3] = y.w;
+    }
+  }
+};
+// every word from the two pairs that it takes: turn(x, y, c, s of its low half, of its high half)
+template <int TYPE, bool NEIGHBOURS, class F> __device__ __forceinline__ void each_pair(Two &t, const Angles &k, F turn) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float2 a = to_floats<TYPE>(t.x[0].w[i]), b = to_floats<TYPE>(t.x[1].w[i]);
     if (NEIGHBOURS) {
-      const float2 x = turn<EXACT>(a.x, a.y, c[i], s[i]), y = turn<EXACT>(b.x, b.y, c[8 + i], s[8 + i]);
-      t.x[0].w[i] = from_floats<TYPE>(x.x, x.y);
-      t.x[1].w[i] = from_floats<TYPE>(y.x, y.y);
+      t.x[0].w[i] = turn(a.x, a.y, k.c[i], k.s[i], a.y, a.x, k.c[i], -k.s[i]);
+      t.x[1].w[i] = turn(b.x, b.y, k.c[8 + i], k.s[8 + i], b.y, b.x, k.c[8 + i], -k.s[8 + i]);
     } else {
-      const float2 x = turn<EXACT>(a.x, b.x, c[2 * i], s[2 * i]), y = turn<EXACT>(a.y, b.y, c[2 * i + 1], s[2 * i + 1]);
-      t.x[0].w[i] = from_floats<TYPE>(x.x, y.x);
-      t.x[1].w[i] = from_floats<TYPE>(x.y, y.y);
+      t.x[0].w[i] = turn(a.x, b.x, k.c[2 * i], k.s[2 * i], a.y, b.y, k.c[2 * i + 1], k.s[2 * i + 1]);
+      t.x[1].w[i] = turn(b.x, a.x, k.c[2 * i], -k.s[2 * i], b.y, a.y, k.c[2 * i + 1], -k.s[2 * i + 1]);
     }
   }
+}
+// each word is two of x c - y s
+template <int TYPE, bool NEIGHBOURS> __device__ __forceinline__ void rotate(Two &t, const Angles &k) {
+  each_pair<TYPE, NEIGHBOURS>(t, k, [](float x, float y, float c, float s, float u, float v, float d, float r) {
+    return from_floats<TYPE>(__fmaf_rn(x, c, -__fmul_rn(y, s)), __fmaf_rn(u, d, -__fmul_rn(v, r)));
+  });
+}
+// the same, correctly rounded where it returns true
+template <int TYPE, bool NEIGHBOURS> __device__ __forceinline__ bool rotate_surely(Two &t, const Angles &k) {
+  uint32_t unsure = 0;
+  each_pair<TYPE, NEIGHBOURS>(t, k, [&](float x, float y, float c, float s, float u, float v, float d, float r) {
+    constexpr float OFF = 1.5f / (1 << 24);  // (the bounds' own roundings are within the half)
+    const float p = __fmul_rn(y, s), q = __fmul_rn(v, r), a = __fmaf_rn(x, c, -p), b = __fmaf_rn(u, d, -q);
+    const float e = __fmul_rn(__fadd_rn(fabsf(p), fabsf(a)), OFF), f = __fmul_rn(__fadd_rn(fabsf(q), fabsf(b)), OFF);
+    const uint32_t lo = from_floats<TYPE>(__fsub_rn(a, e), __fsub_rn(b, f)), hi = from_floats<TYPE>(__fadd_rn(a, e), __fadd_rn(b, f));
+    unsure |= lo ^ hi;
+    return lo;
+  });
+  return unsure == 0;
+}
+template <bool WIDE> __device__ __forceinline__ Two load_two(const uint16_t *p, int first, int second) { return Two{{load_channels<WIDE>(p + 16 * first), load_channels<WIDE>(p + 16 * second)}}; }
+template <int TYPE, bool NEIGHBOURS> __device__ __forceinline__ void rotate_exactly(Two &t, const Angles &k) {
+  each_pair<TYPE, NEIGHBOURS>(t, k, [](float x, float y, float c, float s, float u, float v, float d, float r) { return from_floats<TYPE>(turned_exactly(x, c, y, s), turned_exactly(u, d, v, r)); });
+}
+// all of it again, correctly rounded
+template <int TYPE, bool WIDE, bool NEIGHBOURS> __device__ __noinline__ Two rotated_exactly(const uint16_t *key, const float *row, int half, int t, int first, int second) {
+  Two x = load_two<WIDE>(key, first, second);
+  Angles k;
+  k.load(row, half, t);
+  rotate_exactly<TYPE, NEIGHBOURS>(x, k);
+  return x;
 }
 
 template <int TYPE, bool WIDE, bool NEIGHBOURS> __global__ void __launch_bounds__(THREADS, CTAS) rotate_kernel(const Turn k) {
@@ -75,58 +121,68 @@ template <int TYPE, bool WIDE, bool NEIGHBOURS> __global__ void __launch_bounds_
   const int half = k.a.rotated / 32;
   const bool turns = t < half;
   const int first = !NEIGHBOURS && turns ? t : 2 * t, second = !NEIGHBOURS && turns ? t + half : 2 * t + 1;
-  for (int64_t unit = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5); unit < (int64_t)k.a.tokens * k.parts; unit += (int64_t)gridDim.x * WARPS) {
-    const int token = k.by_parts.divide((int)unit), slice0 = ((int)unit - token * k.parts) * k.span, slice1 = min(slice0 + k.span, k.slices);
-    const int position = __ldg(k.a.positions + token), slot = __ldg(k.s.slots + token);
-    const bool known = (unsigned)position < (unsigned)k.a.reach;
-    float c[16], s[16];
-    if (turns && known) {
-      const float4 *const row = reinterpret_cast<const float4 *>(k.a.angles + position * k.a.angle_stride + 16 * t);
+  Angles angles;
+  auto row_of = [&](int position) { return k.a.angles + position * k.a.angle_stride; };
+  auto spoil = [&](Two &x, uint32_t bits) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4 x = __ldg(row + i), y = __ldg(row + 4 * half + i);
-        c[4 * i] = x.x; c[4 * i + 1] = x.y; c[4 * i + 2] = x.z; c[4 * i + 3] = x.w;
-        s[4 * i] = y.x; s[4 * i + 1] = y.y; s[4 * i + 2] = y.z; s[4 * i + 3] = y.w;
-      }
-    }
-    auto spoil = [&](Two &x) {  // no position: zeros; one behind the table: NaN
+    for (int i = 0; i < 8; ++i) x.x[0].w[i] = x.x[1].w[i] = bits;
+  };
+  constexpr uint32_t NANS = 0x7fff7fffu;  // (of either type)
+  for (int64_t u = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5); u < k.units; u += (int64_t)gridDim.x * WARPS) {
+    const int before = (int)((uint64_t)u * k.kv_step >> 32), after = (int)((uint64_t)(u + 1) * k.kv_step >> 32);
+    if (after == before) {  // query heads of a token
+      const int unit = (int)u - before, token = k.by_parts.divide(unit), slice0 = (unit - token * k.parts) * k.span, slice1 = min(slice0 + k.span, k.q_slices);
+      const int position = __ldg(k.a.positions + token);
+      const bool known = (unsigned)position < (unsigned)k.a.reach;
+      if (turns && known) angles.load(row_of(position), half, t);
+      for (int slice = slice0; slice < slice1; slice += AHEAD) {
+        Two x[AHEAD];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x.x[0].w[i] = x.x[1].w[i] = position < 0 ? 0u : 0x7fff7fffu;
-    };
-    for (int slice = slice0; slice < slice1; ++slice) {
-      if (slice < k.q_slices) {
-        const int head = SLICE * slice + g;
-        if (head >= k.a.q_heads) continue;
-        const uint16_t *const from = static_cast<const uint16_t *>(k.a.q) + token * k.a.q_token_stride + head * k.a.q_head_stride;
-        Two x{{load_shared<WIDE>(from + 16 * first), load_shared<WIDE>(from + 16 * second)}};
-        if (!known) spoil(x);
-        else if (turns) rotate<TYPE, NEIGHBOURS, false>(x, c, s);
-        uint16_t *const to = static_cast<uint16_t *>(k.a.q_out) + token * k.a.out_token_stride + head * k.a.out_head_stride;
-        store_channels<WIDE>(to + 16 * first, x.x[0]);
-        store_channels<WIDE>(to + 16 * second, x.x[1]);
-      } else {
-        const int head = SLICE * (slice - k.q_slices) + g;
-        if (head >= k.s.c.kv_heads || position < 0 || !is_slot(k.s.c, slot)) continue;
-        const uint16_t *const key = static_cast<const uint16_t *>(k.a.k) + token * k.a.k_token_stride + head * k.a.k_head_stride;
-        const uint16_t *const value = static_cast<const uint16_t *>(k.a.v) + token * k.a.v_token_stride + head * k.a.v_head_stride + 32 * t;
-        Two x{{load_channels<WIDE>(key + 16 * first), load_channels<WIDE>(key + 16 * second)}};
-        const Two y{{load_channels<WIDE>(value), load_channels<WIDE>(value + 16)}};
-        if (!known) spoil(x);
-        else if (turns) rotate<TYPE, NEIGHBOURS, true>(x, c, s);
-        int at;
-        uint8_t *const block = block_of(k.s, slot, head, at);
-        uint8_t *const codes = block + at * CODE_BYTES, *const scales = block + K_SCALES + at * SCALE_BYTES;
-        uint32_t scale[2];
-        const float k_inverse = __fdiv_rn(1.f, __ldg(k.s.c.k_scale + head)), v_inverse = __fdiv_rn(1.f, __ldg(k.s.c.v_scale + head));
-        const uint2 k0 = quantise<TYPE>(x.x[0], k_inverse, scale[0]), k1 = quantise<TYPE>(x.x[1], k_inverse, scale[1]);
-        *reinterpret_cast<uint2 *>(codes + 8 * first) = k0;
-        *reinterpret_cast<uint2 *>(codes + 8 * second) = k1;
-        scales[first] = (uint8_t)scale[0];
-        scales[second] = (uint8_t)scale[1];
-        const uint2 v0 = quantise<TYPE>(y.x[0], v_inverse, scale[0]), v1 = quantise<TYPE>(y.x[1], v_inverse, scale[1]);
-        *reinterpret_cast<uint4 *>(codes + V_CODES + 16 * t) = make_uint4(v0.x, v0.y, v1.x, v1.y);
-        *reinterpret_cast<uint16_t *>(scales + (V_SCALES - K_SCALES) + 2 * t) = (uint16_t)(scale[0] | scale[1] << 8);
+        for (int i = 0; i < AHEAD; ++i) {
+          const int head = SLICE * (slice + i) + g;
+          if (slice + i >= slice1 || head >= k.a.q_heads) continue;
+          const uint16_t *const from = static_cast<const uint16_t *>(k.a.q) + token * k.a.q_token_stride + head * k.a.q_head_stride;
+          x[i] = Two{{load_shared<WIDE>(from + 16 * first), load_shared<WIDE>(from + 16 * second)}};
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+          const int head = SLICE * (slice + i) + g;
+          if (slice + i >= slice1 || head >= k.a.q_heads) continue;
+          if (!known) spoil(x[i], position < 0 ? 0u : NANS);  // no position: zeros; one behind the table: NaN
+          else if (turns) rotate<TYPE, NEIGHBOURS>(x[i], angles);
+          uint16_t *const to = static_cast<uint16_t *>(k.a.q_out) + token * k.a.out_token_stride + head * k.a.out_head_stride;
+          store_channels<WIDE>(to + 16 * first, x[i].x[0]);
+          store_channels<WIDE>(to + 16 * second, x[i].x[1]);
+        }
       }
+    } else {  // eight (token, KV head)
+      const int row = min(SLICE * before + g, k.s.rows - 1), token = k.s.by_heads.divide(row), head = row - token * k.s.c.kv_heads;
+      const int position = __ldg(k.a.positions + token), slot = __ldg(k.s.slots + token);
+      const bool known = (unsigned)position < (unsigned)k.a.reach;
+      const uint16_t *const key = static_cast<const uint16_t *>(k.a.k) + token * k.a.k_token_stride + head * k.a.k_head_stride;
+      Two x = load_two<WIDE>(key, first, second);
+      const Two y = load_two<WIDE>(static_cast<const uint16_t *>(k.a.v) + token * k.a.v_token_stride + head * k.a.v_head_stride, 2 * t, 2 * t + 1);
+      if (!known) {
+        spoil(x, NANS);
+      } else if (turns) {
+        angles.load(row_of(position), half, t);
+        if (TYPE == MLOPS_PAGED_FP16) rotate_exactly<TYPE, NEIGHBOURS>(x, angles);
+        else if (!rotate_surely<TYPE, NEIGHBOURS>(x, angles)) x = rotated_exactly<TYPE, WIDE, NEIGHBOURS>(key, row_of(position), half, t, first, second);
+      }
+      if (position < 0 || !is_slot(k.s.c, slot) || SLICE * before + g >= k.s.rows) continue;
+      int at;
+      uint8_t *const block = block_of(k.s, slot, head, at);
+      uint8_t *const codes = block + at * CODE_BYTES, *const scales = block + K_SCALES + at * SCALE_BYTES;
+      uint32_t scale[2];
+      const float k_inverse = __fdiv_rn(1.f, __ldg(k.s.c.k_scale + head)), v_inverse = __fdiv_rn(1.f, __ldg(k.s.c.v_scale + head));
+      const uint2 k0 = quantise<TYPE>(x.x[0], k_inverse, scale[0]), k1 = quantise<TYPE>(x.x[1], k_inverse, scale[1]);
+      *reinterpret_cast<uint2 *>(codes + 8 * first) = k0;
+      *reinterpret_cast<uint2 *>(codes + 8 * second) = k1;
+      scales[first] = (uint8_t)scale[0];
+      scales[second] = (uint8_t)scale[1];
+      const uint2 v0 = quantise<TYPE>(y.x[0], v_inverse, scale[0]), v1 = quantise<TYPE>(y.x[1], v_inverse, scale[1]);
+      *reinterpret_cast<uint4 *>(codes + V_CODES + 16 * t) = make_uint4(v0.x, v0.y, v1.x, v1.y);
+      *reinterpret_cast<uint16_t *>(scales + (V_SCALES - K_SCALES) + 2 * t) = (uint16_t)(scale[0] | scale[1] << 8);
     }
   }
 }
@@ -139,11 +195,14 @@ extern "C" cudaError_t paged_k_append_rotated_launch(const mlops_paged_cache *c,
   k.a = *a;
   k.s = paged::Store{*c, a->slots, paged::Divisor(c->kv_heads), paged::Divisor(c->page_size), a->tokens * c->kv_heads};
   k.q_slices = (a->q_heads + paged::SLICE - 1) / paged::SLICE;
-  k.slices = k.q_slices + (c->kv_heads + paged::SLICE - 1) / paged::SLICE;
-  k.span = a->tokens < sms * paged::CTAS * paged::WARPS ? 1 : k.slices;
-  k.parts = (k.slices + k.span - 1) / k.span;
+  // all of a token's slices in one unit where there are tokens enough for the device's warps
+  k.span = a->tokens < sms * paged::CTAS * paged::WARPS ? 1 : k.q_slices > 0 ? k.q_slices : 1;
+  k.parts = k.q_slices > 0 ? (k.q_slices + k.span - 1) / k.span : 1;
   k.by_parts = paged::Divisor(k.parts);
-  const int64_t ctas = ((int64_t)a->tokens * k.parts + paged::WARPS - 1) / paged::WARPS, most = (int64_t)sms * paged::CTAS;
+  const int64_t kv_units = ((int64_t)k.s.rows + paged::SLICE - 1) / paged::SLICE, units = kv_units + (k.q_slices > 0 ? (int64_t)a->tokens * k.parts : 0);
+  k.units = (int)units;
+  k.kv_step = (((uint64_t)kv_units << 32) + (uint64_t)units - 1) / (uint64_t)units;
+  const int64_t ctas = (units + paged::WARPS - 1) / paged::WARPS, most = (int64_t)sms * paged::CTAS;
   const bool wide = paged::on_32(a->q, a->q_token_stride, a->q_head_stride) && paged::on_32(a->q_out, a->out_token_stride, a->out_head_stride) &&
                     paged::on_32(a->k, a->k_token_stride, a->k_head_stride) && paged::on_32(a->v, a->v_token_stride, a->v_head_stride);
   const auto pick = [&](auto type) {
