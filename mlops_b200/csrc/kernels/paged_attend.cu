@@ -42,8 +42,11 @@ template <int TYPE, int MODE> cudaError_t attend(const Call &k, bool tiles, int 
     if (e == cudaSuccess) e = few(second);
     return e != cudaSuccess ? e : launch_merge<TYPE>(k, sms, stream);
   }
+  // the tile kernel's CTAs begin where the stream's end: neither reads what the other leaves
   const cudaError_t e = few(k);
-  return e != cudaSuccess || !tiles ? e : launch_tile<TYPE, MODE>(k, sms, stream);
+  Call second = k;
+  second.wait_last = true;
+  return e != cudaSuccess || !tiles ? e : launch_tile<TYPE, MODE>(second, sms, stream);
 }
 
 template <int MODE> cudaError_t call(const mlops_paged_attend_args *a, const mlops_paged_common *common, const mlops_paged_cache *c, void *scratch, int sms, cudaStream_t stream) {

@@ -800,7 +800,7 @@ template <int TYPE, int MODE> __global__ void __launch_bounds__(THREADS, 1) tile
     sm.abort = sm.v_nan = sm.others = 0;
     fbla::mbar_init_fence();
   }
-  fbla::wait_previous_pass();
+  if (!k.wait_last) fbla::wait_previous_pass();
   fbla::allow_next_pass();
 
   const int items = items_of<MODE>(k);
@@ -843,7 +843,10 @@ template <int TYPE, int MODE> __global__ void __launch_bounds__(THREADS, 1) tile
   }
   __syncthreads();
   const int ctas = (int)min(total, (long long)(MODE == SHARED ? sm.share : gridDim.x));  // (each has a unit at least: a row's CTAs are consecutive)
-  if ((int)blockIdx.x >= ctas) return;
+  if ((int)blockIdx.x >= ctas) {
+    if (k.wait_last) fbla::wait_previous_pass();
+    return;
+  }
   const long long lo = total * blockIdx.x / ctas, hi = total * (blockIdx.x + 1) / ctas;
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(fbla::smem_u32(&sm.tmem)) : "memory");
@@ -883,7 +886,10 @@ template <int TYPE, int MODE> __global__ void __launch_bounds__(THREADS, 1) tile
   __syncwarp();
   __syncthreads();
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(sm.tmem) : "memory");
-  if (!tiles) return;
+  if (!tiles) {
+    if (k.wait_last) fbla::wait_previous_pass();
+    return;
+  }
   if (sm.v_nan) spoil_rows(k, sm, hi, tid);
 
   // the run's first and last rows of work, where they are cut (SHARED: merge_kernel joins them)
@@ -892,6 +898,7 @@ template <int TYPE, int MODE> __global__ void __launch_bounds__(THREADS, 1) tile
   if (w.n0 > 0 || w.n1 < w.tiles) join_row<TYPE, MODE>(k, sm, w, total, tid);
   const Row<MODE> end = sm.row[0];
   if (end.unit0 > w.unit0 && end.n1 < end.tiles) join_row<TYPE, MODE>(k, sm, end, total, tid);
+  if (k.wait_last) fbla::wait_previous_pass();
 }
 
 }  // namespace
