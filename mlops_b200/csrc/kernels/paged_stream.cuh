@@ -559,23 +559,48 @@ template <int TYPE, int NT, int MODE> __global__ void __launch_bounds__(THREADS<
     split_column(k, w.tile * 8 * NT + c, query, head);
     store_joined<TYPE, MODE>(k, w.r, w.r.start + query, w.head, w.head * k.group + head, lane, o, m, l);
   };
-  for (int f = warp; f < __popc(leaders) * 8 * NT; f += WARPS<NT>) {
-    const int nth = f / (8 * NT), c = f % (8 * NT);
-    const int p = __ffs(__ballot_sync(FULL, (leaders >> lane & 1) && __popc(leaders & ((1u << lane) - 1)) == nth)) - 1;
+  const int live = leaders >> lane & 1 ? sm.row[lane].columns : 0;  // columns of the row that piece `lane` leads
+  int through = live;                                               // of all rows up to it
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int x = __shfl_up_sync(FULL, through, d);
+    if (lane >= d) through += x;
+  }
+  const int columns = __shfl_sync(FULL, through, 31);
+  for (int f = warp; f < columns; f += WARPS<NT>) {
+    const int p = __popc(__ballot_sync(FULL, through <= f)), c = f - __shfl_sync(FULL, through - live, p);
     const int pieces = __popc(__shfl_sync(FULL, same, p));
     const Row<NT, MODE> &w = sm.row[p];
-    if (c >= w.columns) continue;
-    const float2 y = lane < pieces ? *reinterpret_cast<const float2 *>(piece(p, lane).o[c] + D) : make_float2(NOTHING, 0.f);
-    float m = y.x;
-#pragma unroll
-    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, d));
-    const float weight = ex2(y.x - m), l = fbla::warp_sum(y.y * weight);
+    float m, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (pieces <= 4) {  // (most rows lie in two warps: all that they are joined from is read at once, by every lane)
+      float2 y[4];
+      float4 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        y[i] = i < pieces ? *reinterpret_cast<const float2 *>(piece(p, i).o[c] + D) : make_float2(NOTHING, 0.f);
+        v[i] = i < pieces ? *reinterpret_cast<const float4 *>(piece(p, i).o[c] + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      m = fmaxf(fmaxf(y[0].x, y[1].x), fmaxf(y[2].x, y[3].x));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float g = ex2(y[i].x - m);
+        l = fmaf(y[i].y, g, l);
+        o = make_float4(fmaf(v[i].x, g, o.x), fmaf(v[i].y, g, o.y), fmaf(v[i].z, g, o.z), fmaf(v[i].w, g, o.w));
+      }
+    } else {
+      const float2 y = lane < pieces ? *reinterpret_cast<const float2 *>(piece(p, lane).o[c] + D) : make_float2(NOTHING, 0.f);
+      m = y.x;
+#pragma unroll
+      for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, d));
+      const float weight = ex2(y.x - m);
+      l = fbla::warp_sum(y.y * weight);
 #pragma unroll 4
-    for (int i = 0; i < pieces; ++i) {
-      const float f = __shfl_sync(FULL, weight, i);
-      const float4 v = *reinterpret_cast<const float4 *>(piece(p, i).o[c] + 4 * lane);
-      o = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w));
+      for (int i = 0; i < pieces; ++i) {
+        const float g = __shfl_sync(FULL, weight, i);
+        const float4 v = *reinterpret_cast<const float4 *>(piece(p, i).o[c] + 4 * lane);
+        o = make_float4(fmaf(v.x, g, o.x), fmaf(v.y, g, o.y), fmaf(v.z, g, o.z), fmaf(v.w, g, o.w));
+      }
     }
     if (is_cut(w)) {
       float *const slot = k.stream_part + (((size_t)blockIdx.x * 2 + (w.unit0 < cta_lo ? 0 : 1)) * 8 * NT + c) * PSTRIDE;
