@@ -107,8 +107,10 @@ template <int MODE> __device__ __forceinline__ Request<MODE> request(const Call 
     r.at = -1;
     r.common = true;
     const int start = k.a.starts ? min(max(__ldg(k.a.starts + x.first), 0), k.a.tokens) : x.first, end = k.a.starts ? min(__ldg(k.a.starts + x.end), k.a.tokens) : x.end;
+    Plain p = x.end > x.first ? plain_request(k, x.first) : Plain{0, 0, -1, 0};  // (its loads beside those of the group; mostly it is the one)
     for (int b = x.first; b < x.end && x.tokens > 0; ++b) {
-      if (!takes_part(plain_request(k, b), x.tokens)) continue;
+      if (b > x.first) p = plain_request(k, b);
+      if (!takes_part(p, x.tokens)) continue;
       // (the rows of requests that do not take part are computed with the others' and not used)
       r.row = b;
       r.tokens = x.tokens;
