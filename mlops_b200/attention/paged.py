@@ -338,7 +338,8 @@ def _attention(name, q, cache, table, lengths, starts, scale, return_lse, groups
         with scratch.lock:
             status = getattr(_lib, name)(call, pool, scratch.pointer, scratch.bytes, stream)
     else:
-        common = _COMMON.pack(shared.size(0), 0 if groups is None else _ints(groups, index, "groups", shared.size(0) + 1), _ints(shared, index, "shared", 1 if groups is None else None))
+        tokens_at = _ints(shared, index, "shared", 1 if groups is None else None)
+        common = _COMMON.pack(shared.size(0), 0 if groups is None else _ints(groups, index, "groups", shared.size(0) + 1), tokens_at)
         scratch = _scratch.get(q.device, stream, max(16, _lib.mlops_paged_attend_shared_scratch_bytes(call, common, kv_heads)))
         with scratch.lock:
             status = _lib.mlops_paged_attend_shared(call, common, pool, scratch.pointer, scratch.bytes, stream)

@@ -66,6 +66,7 @@ template <int MODE> cudaError_t call(const mlops_paged_attend_args *a, const mlo
   k.stream_part = reinterpret_cast<float *>(base + s.stream_part);
   k.tile_part = reinterpret_cast<float *>(base + s.tile_part);
   if (MODE == SHARED) {
+    k.part_rows = (int)((s.common_rows - s.stream_part) / (PSTRIDE * sizeof(float)));
     k.common = *common;
     k.common_rows = reinterpret_cast<float *>(base + s.common_rows);
     k.own_rows = reinterpret_cast<float *>(base + s.own_rows);

@@ -24,9 +24,10 @@ struct Call {
   int narrow;      // columns of the stream's rows of work
   float *stream_part, *tile_part;          // partial rows, see the kernels
   int *stream_counters, *tile_counters;    // one per CTA, zeros before and after every call
-  // SHARED: the groups, and the sums of every row of q and head over common and own tokens (RowEnd)
+  // SHARED: the groups, and the sums of every row of q and head over common and own tokens (row_end, pieces_end); rows of both kernels' parts
   mlops_paged_common common;
   float *common_rows, *own_rows;
+  int part_rows;
   bool wait_last;  // the kernel before in the stream is of the same call and leaves nothing that this one reads: waited for at the end
 };
 
@@ -73,10 +74,9 @@ __device__ __forceinline__ Plain plain_request(const Call &k, int b) {
   return r;
 }
 // group g's requests, and their common tokens: whole pages of the table, none for a single request, nor for requests of more than LONE columns on average, which fill rows of work by
-// themselves: they take their tokens in one row instead of two that are joined (16 requests behind 6 000 common tokens, us by themselves and together: 260 columns each 216 and 196, 512 287 and
-// 370; 256 fill rows just so: 165 and 201). (Whether a request's first query sees them all, so that it takes
-// part, is asked for each.)
-constexpr int LONE = 384;
+// themselves: they take their tokens in one row instead of two that are joined (16 requests behind 6 000 common tokens, us by themselves and together: 132 columns each 136 and 107, 260 216 and
+// 185, 384 235 and 247, 512 282 and 322, 1024 526 and 609). Whether a request's first query sees them all, so that it takes part, is asked for each.
+constexpr int LONE = 320;
 struct Group {
   int first, end, tokens;
 };
@@ -183,8 +183,8 @@ __device__ __forceinline__ int piece_row(int rows, int i) { return i ? (2 * i - 
 
 // Units of work. The stream's: two blocks of a row of work of `narrow` columns. The tile kernel's: a tile of 128 tokens of a row of work of 256 rows, and HEAD for the row.
 constexpr int UNIT = 2 * BT, TILE_ROWS = 256, TOKENS = 128;
-constexpr int HEAD = 4;  // what loading Q, the first tile and storing O cost (17 000 cycles beside 4 300 per tile; us for two prompts of 8192 with 0, 2, 4, 6, 8: 2006, 1833, 1732, 1757, 1754
-                         // when they were 26 000 and 5 300)
+constexpr int HEAD = 4;  // what a further row of work costs beside its tiles, as tiles (us with 3, 4, 5, 6, 7: two prompts of 8192 tokens 1 302, 1 240, 1 246, 1 256, 1 261; a mixed step of eight
+                         // 312, 305, 308, 301, 309; drafted tokens of 24 requests behind two prompts 60, 56, 59, 62, 68)
 __device__ __forceinline__ int units_of(const Plain &r) { return (r.tokens + UNIT - 1) / UNIT; }  // of each of the item's rows of work
 __device__ __forceinline__ int stream_units(const Call &k, const Plain &r, int columns) {
   return r.n * k.group > k.wide ? 0 : k.c.kv_heads * ((r.n * k.group + columns - 1) / columns) * units_of(r);

@@ -21,15 +21,18 @@ __device__ __forceinline__ void join(Part &a, float top, const Part &b) {
   a.l = a.l * f + (b.l == 0.f ? 0.f : b.l * g);
   a.m = top;
 }
-// a row's sums, from itself (x: the lane's channels) or from its pieces, in their order
+// a row's sums, from itself (x: the lane's channels) or from its pieces, in their order. (A row that starts or groups out of order have left out holds anything: it is zeros where its pieces
+// are none.)
 __device__ __forceinline__ Part part_of(const Call &k, const float4 &x, const float4 &end, int lane) {
   const int pieces = __float_as_int(end.w), rows = __float_as_int(end.y);
   if (!pieces) {
     if (end.y == 0.f) return Part{make_float4(0.f, 0.f, 0.f, 0.f), NOTHING, 0.f};
     return Part{x, end.x, end.y};
   }
-  const float *const first = k.stream_part + (size_t)__float_as_int(end.x) * PSTRIDE;
   Part p{make_float4(0.f, 0.f, 0.f, 0.f), NOTHING, 0.f};
+  const int at = __float_as_int(end.x);
+  if (pieces < 0 || pieces > PAGED_K_MAX_SMS || rows <= 0 || rows > TILE_ROWS || at < 0 || at >= k.part_rows - piece_row(rows, pieces - 1)) return p;
+  const float *const first = k.stream_part + (size_t)at * PSTRIDE;
   for (int i0 = 0; i0 < pieces; i0 += 32) {
     const int n = min(pieces - i0, 32);
     float2 z = make_float2(NOTHING, 0.f);

@@ -91,7 +91,8 @@ template <int TYPE, bool NEIGHBOURS> __device__ __forceinline__ void rotate(Two 
 template <int TYPE, bool NEIGHBOURS> __device__ __forceinline__ bool rotate_surely(Two &t, const Angles &k) {
   uint32_t unsure = 0;
   each_pair<TYPE, NEIGHBOURS>(t, k, [&](float x, float y, float c, float s, float u, float v, float d, float r) {
-    constexpr float OFF = 1.5f / (1 << 24);  // (the bounds' own roundings are within the half)
+    // (the half covers the bounds' own roundings: a - e is a number beside a at least, and within 2^-24 of itself)
+    constexpr float OFF = 1.5f / (1 << 24);
     const float p = __fmul_rn(y, s), q = __fmul_rn(v, r), a = __fmaf_rn(x, c, -p), b = __fmaf_rn(u, d, -q);
     const float e = __fmul_rn(__fadd_rn(fabsf(p), fabsf(a)), OFF), f = __fmul_rn(__fadd_rn(fabsf(q), fabsf(b)), OFF);
     const uint32_t lo = from_floats<TYPE>(__fsub_rn(a, e), __fsub_rn(b, f)), hi = from_floats<TYPE>(__fadd_rn(a, e), __fadd_rn(b, f));

@@ -1,6 +1,6 @@
 // Attention over the paged cache for few queries per request (mlops_paged_attend, mlops_paged_cross_attend, mlops_paged_attend_shared: paged_stream*.cu): the pages are streamed once, bound by their bytes.
 //
-// A row of work is (request, KV head, tile of 8 NT columns); a column is one of the request's queries with one of the KV head's query heads. A row's
+// A row of work is (item, KV head, tile of 8 NT columns; an item is a request, or a group's common tokens); a column is one of the item's queries with one of the KV head's query heads. A row's
 // unit is a pair of blocks, 32 tokens, 2304 contiguous bytes each. All rows' units form one list, which the grid's warps share out in equal contiguous runs,
 // so that ragged lengths cost nothing; a warp brings its run's blocks through a ring of its own in shared memory with bulk copies.
 //
@@ -14,12 +14,12 @@
 // tokens (the order of the K extent of a product is free as long as Q has the same); for V it takes channels 16 g .. 16 g + 15 of four tokens, and two
 // tokens' nibbles of a channel are put beside each other before the conversion, so that a converted pair is a register of V^T.
 //
-// Rows that several warps share are joined in shared memory, those that several CTAs share by the CTA that comes last (a counter per CTA), always in the
-// order of the tokens: the result does not depend on who that is.
+// Rows that several warps share are joined in shared memory, those that several CTAs share by the CTA that comes last (a counter per CTA) or by merge_kernel (mlops_paged_attend_shared), always in
+// the order of the tokens: the result does not depend on who that is.
 //
 // Bound by instructions beside the bytes: some 290 per block and tile of columns, of which a conversion and a scaling of every pair of codes are 128; no pipe is full
 // (issue 0.60 per cycle and scheduler, the ALU pipe 57 % active, shared memory 25 %), warps wait for results of a fixed time and for one another. On the device (a graph of
-// calls with a scratch of their own), 32 / 8 heads: 64 requests of 1K-64K tokens 176 us = 5.2 TB/s, 0.79 of the copy rate; 131 072 tokens 41 us, of which 28 are the
+// calls with a scratch of their own), 32 / 8 heads: 64 requests of 1K-64K tokens 174 us = 5.25 TB/s, 0.80 of the copy rate; 131 072 tokens 41 us, of which 28 are the
 // loop, 6.5 what comes before (lengths, table, queries: five dependent reads) and some 7 the joining; 4096 tokens 12 us. Without the products and conversions the 64
 // requests took 0.83 of the time, with units of one block instead of two (and rows shared out by 64-bit products) 1.18 times; twelve warps instead of sixteen: the same.
 #pragma once

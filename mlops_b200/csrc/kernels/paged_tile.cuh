@@ -1,25 +1,30 @@
-// Attention over the paged cache for many queries per request (mlops_paged_attend, mlops_paged_cross_attend, mlops_paged_attend_shared: paged_tile*.cu): chunks of prompts and whole prompts, on tcgen05 tensor cores with
-// TMEM accumulators.
+// Attention over the paged cache for many queries per request (mlops_paged_attend, mlops_paged_cross_attend, mlops_paged_attend_shared: paged_tile*.cu): chunks of prompts, whole prompts,
+// target texts, the common tokens of many requests, on tcgen05 tensor cores with TMEM accumulators.
 //
-// A row of work is (request, KV head, 256 rows); row c of a request and KV head is query c / group with query head c % group. Its units are HEAD and then the
+// A row of work is (item, KV head, 256 rows); row c of an item and KV head is query c / group with query head c % group. Its units are HEAD and then the
 // tiles of 128 tokens that its last row sees. All units form one list, of which every CTA has an equal contiguous run; a row of work that is cut is joined from
-// partial rows (o, m', l) by the CTA that comes last, in the order of the tokens.
+// partial rows (o, m', l), in the order of the tokens, by the CTA that comes last or (mlops_paged_attend_shared) by merge_kernel.
 //
 // Per tile of tokens and half X of the rows (128 each), with FP32 accumulators in tensor memory:
 //   S_X[128 x 128] = Q_X K^T,   O_X[128 x 128] += P_X V
 // K and V are code * scale, exact in FP16; Q is FP16 after a power of two per row (paged_attend.cuh); P = 2^(s - m') in FP16 takes S_X's place in tensor
-// memory, rounded as in paged_stream.cu. m' moves only where a score would pass 2^15, then O and l are rescaled; l sums the unrounded P. Rows of at most
+// memory, rounded as in paged_stream.cuh. m' moves only where a score would pass 2^15, then O and l are rescaled; l sums the unrounded P. Rows of at most
 // 128 use both halves too: the even tiles of tokens go to X = 0, the odd ones to X = 1, with the same queries, and the halves are joined at the end.
 //
-// The exponentials of a tile take as long as its two products: 16 per cycle and SM, 2048 cycles for both X. Eight warps do those of X = 0 and then those of X = 1, so that
-// the tensor cores work for one X while the other one's softmax runs. A tile then takes the softmax of one X (1800 cycles, of which the exponentials are 1024) and the way
-// of the other from P to its next scores (2500: two products of 512 among the other X's, three hand-overs through barriers): 4300 cycles where the products alone are
-// 2048. Two prompts of 8192 tokens, 32 / 8 heads: 1.40 ms = 785 TFLOP/s, 0.48 of the measured burst rate. Tried: a thread per row and both X's softmax at once
-// (7600 cycles: both wait for the tensor cores together); a third of the exponentials as polynomials on the FMA units (1.07 times the time: packed FP32, maxima and
-// conversions share their issue slots); operand warps that look up their blocks themselves (the registers spill, and every load is waited for at once). The kernel
-// stores 56 bytes of registers per thread to local memory and loads 200.
+// Everything goes 64 tokens of a tile at a time: while the softmax has the second half of a tile, the first half's P is multiplied and the next tile's first scores take its place, so that
+// the softmax finds scores whenever it is through. Each X has four warps, a thread per row, and a thread of its own that issues its products; the two X only share the operands.
+// A tile takes 3 850 cycles. Its exponentials are 2 048 (16 per cycle and SM), its products 2 048 at their rate, but the scores' with 64 tokens read Q again for each half and are
+// bound by shared memory: 2 560 in all, beside 512 of the operands' stores. Measured (clocks in the kernel): a thread's half takes 1 300 to 1 500 cycles, of which the exponentials, both X's
+// at once, are 1 100; some 250 are the way through barriers; the issuing threads wait for the tensor cores two thirds of the time. Two prompts of 8192 tokens, 32 / 8 heads: 1.24 ms = 890 TFLOP/s,
+// 0.53 of the measured burst rate. Tried: scores 128 tokens at a time (4 600 cycles: softmax and products of an X in turn), with both X's softmax in turn (5 000), with 32 scores on their way
+// while 32 are used (5 150); eight warps for X = 0 and then for X = 1, two threads per row (4 300); a third of the exponentials as polynomials on the FMA units, then 1.07 times the
+// time; operand warps that look up their blocks themselves (the registers spill, and every load is waited for at once). The kernel stores 48 to 72 bytes of registers per thread to
+// local memory and loads 128 to 216.
 //
-// Warps 0-7 (two threads per row): softmax. Warps 8-15: operands, from packed pages to two stages each of K and V in shared
+// Around the tiles a CTA spends some 45 000 cycles: its code comes from the L2 (10 cycles per instruction that is run for the first time), lengths, table, queries and pages are read one after the
+// other (16 000 until the first product), the first tile takes 9 000 more than the others, the sums' way out 7 000.
+//
+// Warps 0-7: softmax. Warps 8-15: operands, from packed pages to two stages each of K and V in shared
 // memory, token rows of 128 bytes (64 channels) with 16-byte chunk c of row r at c ^ (r % 8): for S that is K-major, for O V's MN-major. Warps 16, 17: one thread
 // each issues the products of its X. Warp 18 looks up where the tiles' blocks lie. Every wait is bounded: where one gives up, the rows become NaN.
 #pragma once
@@ -307,8 +312,8 @@ template <int MODE> __device__ __forceinline__ void produce(Smem<MODE> &sm, int 
 }
 
 // ---- products -------------------------------------------------------------------------------------------------------------------
-// The way from P to the next scores is what a tile takes: nothing else is waited for or released on it. A stage is free when both X have read it; where a tile
-// is one X's alone, that one arrives for the other.
+// The way from P to the next scores of the same half of a tile has to be shorter than the softmax of the other half: nothing else is waited for or released on it. A stage is free when both X
+// have read it; where a tile is one X's alone, that one arrives for the other.
 template <int MODE> __device__ __forceinline__ void issue(const Call &k, Smem<MODE> &sm, long long hi, int x) {  // by one thread
   const uint32_t s_at = sm.tmem + 128 * x, o_at = sm.tmem + 256 + 128 * x;
   uint32_t row_at = 0, mine = 0, items = 0;  // tiles of the run before the row, of this X; rows of work

@@ -321,3 +321,46 @@ def test_a_step_from_the_projection_to_both_attentions(paged):
                         assert bool(((got[first + i, x].double() - value).abs() <= 2.0 ** -10 * (p @ vd[:seen, x // group].abs()) + 2.0 ** -8 * value.abs() + 1e-7).all())
             first += m
     assert int(cursor[2]) == 0
+
+
+def through_c(paged, q, cache, table, lengths, starts, cuts, common, fill=0xFF):
+    """the C call with a scratch whose first 8192 bytes are zeros and the others `fill`, into outputs that hold 77"""
+    tokens, heads, _ = q.shape
+    out, lse = torch.full_like(q, 77.0), torch.full((tokens, heads), 77.0, device="cuda")
+    call = paged._ATTEND.pack(lengths.numel(), tokens, heads, paged._TYPES[q.dtype], q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
+                              lse.data_ptr(), table.data_ptr(), table.stride(0), table.shape[1], lengths.data_ptr(), 0 if starts is None else starts.data_ptr(), 0.0)
+    groups = paged._COMMON.pack(common.numel(), 0 if cuts is None else cuts.data_ptr(), common.data_ptr())
+    scratch = torch.full((paged._lib.mlops_paged_attend_shared_scratch_bytes(call, groups, cache.units.shape[1]),), fill, dtype=torch.uint8, device="cuda")
+    scratch[:8192] = 0
+    pool = paged._pool(cache)[0]
+    for _ in range(2):
+        status = paged._lib.mlops_paged_attend_shared(call, groups, pool, scratch.data_ptr(), scratch.numel(), torch.cuda.current_stream().cuda_stream)
+        assert status == 0, paged._lib.mlops_paged_last_error()
+    return out, lse
+
+
+@pytest.mark.parametrize("fill", [0xFF, 0x7F, 0x01])
+@pytest.mark.parametrize("counts", [[1, 1, 1, 1], [3, 0, 2, 5], [90, 2, 0, 150]])
+def test_a_scratch_that_held_anything(paged, counts, fill):
+    """zeros in front are all that a call asks for; requests that see nothing, rows of no request"""
+    lengths, groups = [700, 0, 650, 900], [(0, 4, 600)]
+    gen, table, cache = build(paged, 20, groups, lengths, 2, 64)
+    q = torch.randn((sum(counts) + 3, 8, 128), generator=gen, device="cuda").to(torch.bfloat16)
+    cuts, common = group_args(groups)
+    out, lse = through_c(paged, q, cache, table, ints(lengths), starts_of(counts), cuts, common, fill)
+    assert bool((out[sum(counts) :] == 0).all()) and bool(torch.isneginf(lse[sum(counts) :]).all())
+    want = pu.attend(q[: sum(counts)], cache.units, cache.k_scale, cache.v_scale, table, lengths, counts)
+    agree(out[: sum(counts)], lse[: sum(counts)], want, "bf16")
+
+
+@pytest.mark.parametrize("fill", [0xFF, 0x01])
+@pytest.mark.parametrize("starts, cuts", [([8, 2, 12, 12, 20], [0, 4]), ([0, 5, 3, 9, 20], [2, 1, 4]), ([0, 1, 2, 3, 4], [3, 0, 9]), ([0, 1000, -5, 20, 20], [0, 3, 1, 4]), ([0, 5, 10, 15, 20], [-7, 1 << 30])])
+def test_starts_and_groups_out_of_order(paged, starts, cuts, fill):
+    """no row means anything then, but each is written at most, and nothing beside them; the requests' rows that are in order are as they would be"""
+    lengths = [300, 310, 320, 330]
+    gen, table, cache = build(paged, 21, [(0, 4, 256)], lengths, 2, 64)
+    rows = torch.randn((26, 8, 128), generator=gen, device="cuda").to(torch.bfloat16)
+    out, lse = through_c(paged, rows[:20], cache, table, ints(lengths), ints(starts), ints(cuts), ints([256] * (len(cuts) - 1)), fill)
+    assert out.shape == (20, 8, 128)
+    if starts == [0, 5, 10, 15, 20]:
+        agree(out, lse, pu.attend(rows[:20], cache.units, cache.k_scale, cache.v_scale, table, lengths, [5] * 4), "bf16")
