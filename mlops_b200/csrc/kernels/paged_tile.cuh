@@ -13,13 +13,14 @@
 //
 // Everything goes 64 tokens of a tile at a time: while the softmax has the second half of a tile, the first half's P is multiplied and the next tile's first scores take its place, so that
 // the softmax finds scores whenever it is through. Each X has four warps, a thread per row, and a thread of its own that issues its products; the two X only share the operands.
-// A tile takes 3 850 cycles. Its exponentials are 2 048 (16 per cycle and SM), its products 2 048 at their rate, but the scores' with 64 tokens read Q again for each half and are
+// A tile takes 3 800 cycles. Its exponentials are 2 048 (16 per cycle and SM), its products 2 048 at their rate, but the scores' with 64 tokens read Q again for each half and are
 // bound by shared memory: 2 560 in all, beside 512 of the operands' stores. Measured (clocks in the kernel): a thread's half takes 1 300 to 1 500 cycles, of which the exponentials, both X's
-// at once, are 1 100; some 250 are the way through barriers; the issuing threads wait for the tensor cores two thirds of the time. Two prompts of 8192 tokens, 32 / 8 heads: 1.24 ms = 890 TFLOP/s,
-// 0.53 of the measured burst rate. Tried: scores 128 tokens at a time (4 600 cycles: softmax and products of an X in turn), with both X's softmax in turn (5 000), with 32 scores on their way
-// while 32 are used (5 150); eight warps for X = 0 and then for X = 1, two threads per row (4 300); a third of the exponentials as polynomials on the FMA units, then 1.07 times the
-// time; operand warps that look up their blocks themselves (the registers spill, and every load is waited for at once). The kernel stores 48 to 72 bytes of registers per thread to
-// local memory and loads 128 to 216.
+// at once, are 1 100; some 250 are the way through barriers; the issuing threads wait for the tensor cores two thirds of the time. Instructions are fetched at that rate too: the same code with
+// the two halves' softmax unrolled took 1.27 times the time, with the rare path's exponentials apart 1.02, with a mask that the compiler predicates 1.04. Two prompts of 8192 tokens, 32 / 8 heads:
+// 1.22 ms = 900 TFLOP/s, 0.54 of the measured burst rate. Tried: scores 128 tokens at a time (4 600 cycles: softmax and products of an X in turn), with both X's softmax in turn (5 000), with 32
+// scores on their way while 32 are used (5 150); eight warps for X = 0 and then for X = 1, two threads per row (4 300); all 64 scores in registers for both passes (1.03 times the time); a third of
+// the exponentials as polynomials on the FMA units, then 1.07 times the time; operand warps that look up their blocks themselves (the registers spill, and every load is waited for at once). The kernel
+// stores 28 to 60 bytes of registers per thread to local memory and loads 108 to 204.
 //
 // Around the tiles a CTA spends some 45 000 cycles: its code comes from the L2 (10 cycles per instruction that is run for the first time), lengths, table, queries and pages are read one after the
 // other (16 000 until the first product), the first tile takes 9 000 more than the others, the sums' way out 7 000.
@@ -434,42 +435,44 @@ template <int TYPE, int MODE> __device__ __forceinline__ void load_q(const Call 
   asm volatile("" : "+r"((r)[0]), "+r"((r)[1]), "+r"((r)[2]), "+r"((r)[3]), "+r"((r)[4]), "+r"((r)[5]), "+r"((r)[6]), "+r"((r)[7]), "+r"((r)[8]), "+r"((r)[9]), "+r"((r)[10]), "+r"((r)[11]), \
                     "+r"((r)[12]), "+r"((r)[13]), "+r"((r)[14]), "+r"((r)[15]), "+r"((r)[16]), "+r"((r)[17]), "+r"((r)[18]), "+r"((r)[19]), "+r"((r)[20]), "+r"((r)[21]), "+r"((r)[22]), \
                     "+r"((r)[23]), "+r"((r)[24]), "+r"((r)[25]), "+r"((r)[26]), "+r"((r)[27]), "+r"((r)[28]), "+r"((r)[29]), "+r"((r)[30]), "+r"((r)[31]))
-struct Half {  // 64 of a row's scores
-  uint32_t r[2][32];
+struct Scores {  // 32 of a row's
+  uint32_t r[32];
   __device__ __forceinline__ void load(uint32_t at) {
-    PAGED_LD32(at, r[0]);
-    PAGED_LD32(at + 32, r[1]);
+    PAGED_LD32(at, r);
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-    PAGED_HOLD32(r[0]);
-    PAGED_HOLD32(r[1]);
+    PAGED_HOLD32(r);
   }
-  __device__ __forceinline__ float score(int i) const { return __uint_as_float(r[i >> 5][i & 31]); }
+  __device__ __forceinline__ float score(int i) const { return __uint_as_float(r[i]); }
   // scores of tokens above `last` and of blocks whose byte in `there` is 0 become -infinity
   __device__ __forceinline__ void mask(int last, uint32_t there) {
+    __syncwarp();  // (a branch: the warps that need no mask do not run it)
+    const int n = min(max(last + 1, 0), 32);  // tokens that are seen
+    const uint32_t seen = (((there & 1) * 0xffffu) | ((there >> 8 & 1) * 0xffff0000u)) & (n ? ~0u >> (32 - n) : 0u);
 #pragma unroll
-    for (int i = 0; i < 64; ++i)
-      if (i > last || !(there >> (8 * (i >> 4)) & 1)) r[i >> 5][i & 31] = __float_as_uint(-FBLA_INF);
+    for (int i = 0; i < 32; ++i)
+      if (!(seen >> i & 1)) r[i] = __float_as_uint(-FBLA_INF);
   }
   __device__ __forceinline__ float largest() const {
     float top[4] = {NOTHING, NOTHING, NOTHING, NOTHING};
 #pragma unroll
-    for (int i = 0; i < 32; ++i) top[i & 3] = fbla::max3(top[i & 3], score(2 * i), score(2 * i + 1));
+    for (int i = 0; i < 16; ++i) top[i & 3] = fbla::max3(top[i & 3], score(2 * i), score(2 * i + 1));
     return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
   }
-  // 2^(score mult - m) as 32 words of FP16 pairs in r[0]; their sum, and the largest exponent.
-  __device__ __forceinline__ float exponentials(float mult, float m, float &high) {
+  // 2^(score mult - m) as 16 words of FP16 pairs in r; their sum
+  __device__ __forceinline__ float exponentials(float mult, float m) {
     float2 sum[2] = {};
-    float top[2] = {NOTHING, NOTHING};
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
+    for (int i = 0; i < 16; ++i) {
       const float2 e = __ffma2_rn(make_float2(score(2 * i), score(2 * i + 1)), make_float2(mult, mult), make_float2(-m, -m));
-      top[i & 1] = fbla::max3(top[i & 1], e.x, e.y);
       const float2 f = make_float2(ex2(e.x), ex2(e.y));
       sum[i & 1] = __fadd2_rn(sum[i & 1], f);
-      r[0][i] = from_floats<MLOPS_PAGED_FP16>(f.x, f.y);
+      r[i] = from_floats<MLOPS_PAGED_FP16>(f.x, f.y);
     }
-    high = fmaxf(top[0], top[1]);
     return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+  }
+  __device__ __forceinline__ void store(uint32_t at) const {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]),
+                 "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
   }
 };
 
@@ -480,25 +483,22 @@ struct Line {
   bool started;  // O holds sums, or will
 };
 
-// 64 tokens of a tile, from first_token on: scores in tensor memory at s become P there. o_done: of the products with the 64 tokens before.
+// 64 tokens of a tile, from first_token on: scores in tensor memory at s become P there. o_done: of the products with the 64 tokens before. The scores are read twice, for their maximum and
+// for their exponentials, 32 at a time.
 template <int MODE>
 __device__ __forceinline__ bool take_half(Smem<MODE> &sm, Line &q, uint32_t s, uint32_t o, int first_token, int low, uint32_t blocks, uint64_t *o_done, uint32_t o_parity) {
   const bool mask = first_token + 63 > low || blocks != 0x01010101u;  // some row does not see all of them
-  Half x;
-  bool ok = true, over = true;
-  float high, sum = 0.f;
-  x.load(s);
-  if (mask) x.mask(q.limit - first_token, blocks);
-  if (q.started) {  // as if m' may stay where it is
-    sum = x.exponentials(q.mult, q.m, high);
-    over = __any_sync(FULL, high > TOP);
+  bool ok = true;
+  float high = NOTHING, sum = 0.f;
+  Scores x;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    x.load(s + 32 * i);
+    if (mask) x.mask(q.limit - first_token - 32 * i, blocks >> (16 * i));
+    high = fmaxf(high, x.largest());
   }
-  if (over) {
-    if (q.started) {
-      x.load(s);
-      if (mask) x.mask(q.limit - first_token, blocks);
-    }
-    high = x.largest() * q.mult;  // (mult is positive)
+  high *= q.mult;  // (mult is positive)
+  if (__any_sync(FULL, high - q.m > TOP)) {
     float keep = 1.f;
     if (high - q.m > TOP) {
       keep = ex2(q.m - (high - REST));
@@ -520,11 +520,17 @@ __device__ __forceinline__ bool take_half(Smem<MODE> &sm, Line &q, uint32_t s, u
       }
       tc::tmem_st_wait();
     }
-    sum = x.exponentials(q.mult, q.m, high);
   }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    x.load(s + 32 * i);
+    if (mask) x.mask(q.limit - first_token - 32 * i, blocks >> (16 * i));
+    sum += x.exponentials(q.mult, q.m);
+    x.store(s + 16 * i);  // (where the thread's own scores have been read)
+  }
+  tc::tmem_st_wait();
   q.l += sum;
   q.started = true;
-  tc::tmem_st32(s, x.r[0]);  // (in the place of the thread's own scores)
   return ok;
 }
 
