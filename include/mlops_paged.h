@@ -144,7 +144,7 @@ typedef struct mlops_paged_common {
   const int *tokens;                   /* [groups] */
 } mlops_paged_common;
 /* What mlops_paged_attend gives, within rounding; the pages that a group's requests have in common are read once for all of them. A request whose first query does not see all of the
- * common tokens is attended by itself. The scratch is mlops_paged_attend's with 1056 bytes more per row of q and query head. */
+ * common tokens is attended by itself. (A group's first request that takes part is looked for in their order: idle places of a batch are better at a group's end.) The scratch is mlops_paged_attend's with 1056 bytes more per row of q and query head. */
 size_t mlops_paged_attend_shared_scratch_bytes(const mlops_paged_attend_args *args, const mlops_paged_common *common, int kv_heads);
 mlops_fbla_status mlops_paged_attend_shared(const mlops_paged_attend_args *args, const mlops_paged_common *common, const mlops_paged_cache *cache, void *scratch, size_t scratch_bytes,
                                             cudaStream_t stream);

@@ -443,7 +443,7 @@ template <int TYPE, int NT, int MODE> __global__ void __launch_bounds__(THREADS<
       if (lane == 0) sm.share = share;
     }
     __syncthreads();
-    ctas -= sm.share;
+    if (sm.share < ctas) ctas -= sm.share;  // (a device of two multiprocessors runs one kernel after the other)
     if (blockIdx.x >= ctas) return;  // (they begin when the tile kernel's CTAs are through; those with units wait for all of them)
   }
   __syncthreads();

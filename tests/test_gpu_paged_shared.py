@@ -364,3 +364,58 @@ def test_starts_and_groups_out_of_order(paged, starts, cuts, fill):
     assert out.shape == (20, 8, 128)
     if starts == [0, 5, 10, 15, 20]:
         agree(out, lse, pu.attend(rows[:20], cache.units, cache.k_scale, cache.v_scale, table, lengths, [5] * 4), "bf16")
+
+
+@pytest.mark.parametrize("batch, groups", [(1500, 500), (2047, 1), (1024, 1024)])
+def test_as_many_requests_and_groups_as_a_call_takes(paged, batch, groups):
+    size = -(-batch // groups)
+    cuts = [min(g * size, batch) for g in range(groups + 1)]
+    lengths = [33 + (7 * b) % 60 for b in range(batch)]
+    gen, table, cache = build(paged, 22, [(a, b, 32) for a, b in zip(cuts, cuts[1:])], lengths, 1, 16)
+    q = torch.randn((batch, 2, 128), generator=gen, device="cuda").to(torch.bfloat16)
+    out, lse = paged.attend_shared(q, cache, table, ints(lengths), None, ints(cuts), ints([32] * groups), return_lse=True)
+    agree(out, lse, pu.attend(q, cache.units, cache.k_scale, cache.v_scale, table, lengths, [1] * batch), "bf16")
+    with pytest.raises(ValueError, match="2048"):
+        paged.attend_shared(q, cache, table, ints(lengths), None, torch.zeros(2049 - batch + 1, dtype=torch.int32, device="cuda"), torch.zeros(2049 - batch, dtype=torch.int32, device="cuda"))
+
+
+@pytest.mark.parametrize("counts", [[1, 1, 1], [6, 2, 1], [150, 90, 3]])
+def test_a_pool_of_more_than_4_gib(paged, counts):
+    """pages far beyond 2^32 bytes from the pool's start: rotation and append, attention over common and own tokens, cross attention"""
+    from tests.test_gpu_paged_rotate import angles, rotate, round16
+    heads, P, lengths, unit = 2, 64, [500, 470, 400], 4 * 2304
+    gen, table, small = build(paged, 23, [(0, 3, 256)], lengths, heads, P)
+    pages = small.pages
+    stride = ((5 << 30) // pages + 4095) // 4096 * 4096
+    units = torch.zeros(pages * stride, dtype=torch.uint8, device="cuda").as_strided((pages, heads, P // 16, 2304), (stride, unit, 2304, 1))
+    units.copy_(small.units)
+    cache = paged.PagedCache(units, small.k_scale, small.v_scale)
+    q = torch.randn((sum(counts), heads * 4, 128), generator=gen, device="cuda").to(torch.bfloat16)
+    check(paged, q, cache, table, lengths, counts, starts_of(counts), [(0, 3, 256)], "bf16")
+    same = paged.cross_attend(q, small, table, ints(lengths), starts_of(counts))
+    assert torch.equal(same, paged.cross_attend(q, cache, table, ints(lengths), starts_of(counts)))
+    k = torch.randn((3, heads, 128), generator=gen, device="cuda").to(torch.bfloat16)
+    slots, cos_sin, positions = ints([(pages - 1) * P + 1, (pages - 1) * P + 63, (pages - 2) * P]), angles(600, 128), ints([5, 500, 599])
+    paged.append_rotated(cache, q[:3], k, k, slots, positions, cos_sin)
+    turned = round16(rotate(k, cos_sin[positions.long()], False)[0], "bf16")
+    for got, x in zip(pu.at_slots(units, slots), sum(zip(pu.quantise(turned, cache.k_scale), pu.quantise(k, cache.v_scale)), ())):
+        assert torch.equal(got.cpu(), x)
+
+
+def test_a_long_beginning(paged):
+    """200 000 common tokens, as one item of the stream and of the tile kernel"""
+    common = 200000
+    for batch in (3, 12):
+        lengths = [common + 1 + 50 * b for b in range(batch)]
+        gen, table, cache = build(paged, 24, [(0, batch, common)], lengths, 1, 256)
+        q = torch.randn((batch, 4, 128), generator=gen, device="cuda").to(torch.bfloat16)
+        check(paged, q, cache, table, lengths, [1] * batch, None, [(0, batch, common)], "bf16")
+
+
+@pytest.mark.parametrize("rows", [79, 80, 81, 82, 100])
+def test_on_both_sides_of_requests_that_fill_rows_of_work(paged, rows):
+    """80 queries of four heads each are 320 columns: up to there on average a group's tokens are taken together"""
+    lengths, counts, groups = [700, 720, 800, 300], [rows, 80, 80, 5], [(0, 3, 500), (3, 4, 100)]
+    gen, table, cache = build(paged, 25, groups, lengths, 2, 64)
+    q = torch.randn((sum(counts), 8, 128), generator=gen, device="cuda").to(torch.float16)
+    check(paged, q, cache, table, lengths, counts, starts_of(counts), groups, "fp16")
