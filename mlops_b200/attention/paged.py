@@ -262,7 +262,7 @@ def append_rotated(cache: PagedCache, q: torch.Tensor, k: torch.Tensor, v: torch
     shape, strides = cos_sin.shape, cos_sin.stride()
     if cos_sin.get_device() != index or cos_sin.dtype is not _F32 or len(shape) != 2 or strides[1] != 1 or (strides[0] % 4 and shape[0] > 1) or cos_sin.data_ptr() % 16:
         raise ValueError(f"cos_sin: expected a float32 [positions, rotated] tensor with dense rows on 16-byte boundaries on cuda:{index}; it is {cos_sin.dtype} {tuple(shape)}, strides {strides}, on {cos_sin.device}")
-    out = torch.empty((tokens, q_heads, HEAD_DIM), dtype=q.dtype, device=q.device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     status = _lib.mlops_paged_append_rotated(pool, _ROTATE.pack(tokens, q_heads, kind, shape[1], 1 if interleaved else 0, shape[0], cos_sin.data_ptr(), strides[0] if shape[0] > 1 else shape[1], q.data_ptr(), k.data_ptr(), v.data_ptr(),
                                                                 q_by_token, q_by_head, k_by_token, k_by_head, v_by_token, v_by_head, out.data_ptr(), q_heads * HEAD_DIM, HEAD_DIM,
                                                                 _ints(slots, index, "slots", tokens), _ints(positions, index, "positions", tokens)), _C._raw_stream(index))
@@ -328,7 +328,7 @@ def _attention(name, q, cache, table, lengths, starts, scale, return_lse, groups
     entries, stride, batch, width = _table(table, index)
     where = _ints(lengths, index, "lengths", batch)
     begins = 0 if starts is None else _ints(starts, index, "starts", batch + 1)
-    out = q.new_empty((tokens, heads, HEAD_DIM))
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = q.new_empty((tokens, heads), dtype=_F32) if return_lse else None
     call = _ATTEND.pack(batch, tokens, heads, kind, q.data_ptr(), by_token, by_head, out.data_ptr(), heads * HEAD_DIM, HEAD_DIM, lse.data_ptr() if return_lse else 0,
                         entries, stride, width, where, begins, scale)
