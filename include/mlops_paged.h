@@ -85,8 +85,8 @@ mlops_fbla_status mlops_paged_append(const mlops_paged_cache *cache, int tokens,
 /* A step's tokens as the projection leaves them: q and k rotated by the tokens' positions, q stored, k and v quantised into the slots as
  * mlops_paged_append does. Rotation of a pair (x, y) of channels by position p: (x c - y s, y c + x s) with c = angles[p][i], s = angles[p][rotated / 2 + i]
  * for pair i: channels (i, i + rotated / 2), or (2 i, 2 i + 1) where `interleaved`; channels from `rotated` on stay as they are. Rotated q is rounded once to the
- * type (FP32 arithmetic); rotated k is the exact rotation rounded once to the type (of
- * elements above 2^-100 in magnitude), so that the cache's bytes are those that mlops_paged_append stores of it.
+ * type (FP32 arithmetic); rotated k is the exact rotation rounded once to the type (BF16:
+ * where that is 0 or above 2^-100 in magnitude), so that the cache's bytes are those that mlops_paged_append stores of it.
  * A token without a slot of the pool has its q rotated and is not stored. A token of a negative position (a row that is no request's) has zeros as its
  * q and is not stored; one whose position is behind the table has NaN as its q, and its K is stored as NaN. q_out may be q with the same strides, and overlaps no other input
  * or q. */

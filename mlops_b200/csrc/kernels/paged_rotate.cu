@@ -3,9 +3,10 @@
 //
 // Rotation of a pair (x, y) by (c, s): (x c - y s, y c + x s). q takes it in FP32, rounded once to its type at the end. A stored code of k asks on which side of a border a value
 // lies, so k's rotation is correctly rounded to 16 bits: r = fl(x c - fl(y s)) is off by at most 2^-24 (|y s| + |r|), and where all numbers so near to r round to the same one, that is it. Where they do not
-// (some 2^-14 of the elements), the thread takes all of its products with their errors (an FMA gives them) and sums with theirs (TwoSum: D. Knuth, The
-// Art of Computer Programming 2, 4.2.2), and sets the last bit of a rounded sum that is not exact, so that rounding it again to 16 bits never meets a halfway case that is none (rounding to odd: S. Boldo,
-// G. Melquiond, Emulation of FMA and correctly rounded sums, 2008). What is stored is, bit for bit, what mlops_paged_append stores of the correctly rounded rotation.
+// (some 2^-14 of the elements), the thread takes all of its pairs in FP64, where the products are exact, and
+// sets the last bit of an FP32 sum that is not exact, so that rounding it again to 16 bits never meets a halfway case that is none (rounding to odd: S. Boldo,
+// G. Melquiond, Emulation of FMA and correctly rounded sums, 2008). FP16, whose numbers are eight times as close, takes all of K so: 16 384 tokens of 32 / 8 heads, halves and neighbours, 72 and
+// 74 us, in BF16 68 and 71. What is stored is, bit for bit, what mlops_paged_append stores of the correctly rounded rotation.
 //
 // Warps have units of two kinds, dealt evenly over each other so that the ones' memory and the others' arithmetic share a multiprocessor: a token's query heads, eight at a time, with the
 // token's angles in registers; eight (token, KV head), four threads each.
@@ -44,15 +45,12 @@ template <bool WIDE> __device__ __forceinline__ Channels load_shared(const uint1
   return x;
 }
 
-// x c - y s, rounded to odd: the nearest FP32 number, or where that is not exact the one beside the exact value whose last bit is set
-__device__ __forceinline__ float turned_exactly(float x, float c, float y, float s) {
-  const float a = __fmul_rn(x, c), a_off = __fmaf_rn(x, c, -a), b = -__fmul_rn(y, s), b_off = -__fmaf_rn(y, s, b);
-  const float sum = __fadd_rn(a, b), bb = __fsub_rn(sum, a);
-  const float off = __fadd_rn(__fadd_rn(__fsub_rn(a, __fsub_rn(sum, bb)), __fsub_rn(b, bb)), __fadd_rn(a_off, b_off));
-  const float r = __fadd_rn(sum, off), rest = __fsub_rn(off, __fsub_rn(r, sum));
-  uint32_t bits = __float_as_uint(r);
-  if (rest != 0.f && !(bits & 1) && (bits & 0x7f800000u) != 0x7f800000u) bits += (rest > 0.f) == (r > 0.f) ? 1u : ~0u;
-  return __uint_as_float(bits);
+// x c - y s, rounded to odd: the nearest FP32 number towards 0, with its last bit set where that is not exact. In FP64 both products are exact (x and y have 11 bits at most, c and s 24, and
+// no exponent comes near FP64's ends), so that the difference rounded down and up is one number or two beside each other.
+__device__ __forceinline__ float turned_exactly(double x, double c, double y, double s) {
+  const double b = -__dmul_rn(y, s), below = __fma_rd(x, c, b), above = __fma_ru(x, c, b), near = above <= 0. ? above : below;
+  const float r = __double2float_rz(near);
+  return __uint_as_float(__float_as_uint(r) | (below != above || (double)r != near));
 }
 // a thread's angles, of its 16 pairs
 struct Angles {

@@ -3,6 +3,9 @@
 The bound of q: fl(x c - fl(y s)) in FP32 is off by at most 2^-24 |y s| + 2^-24 |x c - y s|, below 2^-23 (|x c| + |y s|); the type's rounding adds half a step of the value, at
 least half its smallest number (2^-25 for FP16, 2^-134 for BF16)."""
 import math
+import random
+import struct
+from fractions import Fraction
 
 import pytest
 import torch
@@ -202,3 +205,98 @@ def test_a_captured_call_follows_positions_and_slots(paged):
             graph.replay()
             other = paged.PagedCache(units.clone(), ks, vs)
             assert torch.equal(out, paged.append_rotated(other, q, k, v, slots, positions, table)) and torch.equal(other.units, units)
+
+
+def nearest16(x, name):
+    """the number of the type nearest to a fraction, halfway to even"""
+    bits, least = (8, -133) if name == "bf16" else (11, -24)
+    if x == 0:
+        return 0.0
+    size = abs(x).numerator.bit_length() - abs(x).denominator.bit_length()  # floor(log2 |x|), or one above it
+    size -= abs(x) < Fraction(2) ** size
+    unit = Fraction(2) ** max(size - bits + 1, least)
+    return float(round(x / unit) * unit)
+
+
+def fp32(x):
+    return struct.unpack("f", struct.pack("f", x))[0]
+
+
+def beside_a_middle(rng, name):
+    """(x, c, y, s) whose x c - y s lies beside the middle of two numbers of the type, of which a code's border is one, by far less than FP32 tells apart: x c is off the middle, and rounds to it in
+    FP32, by what y s takes away again but for its own rounding; or x c is the middle and y s below what FP32 holds of a product's error"""
+    bits = 8 if name == "bf16" else 11
+    border, up = rng.choice([(0.75, False), (1.75, False), (3.5, False), (0.25, True), (1.25, True), (2.5, True), (5.0, True)])  # a border belongs to the even code beside it
+    middle = border + (1 if up else -1) * 2.0 ** (math.frexp(border)[1] - bits - 1)
+    number = lambda: rng.choice([-1, 1]) * (1 + rng.randrange(1 << (bits - 1)) / (1 << (bits - 1)))
+    if rng.random() < 0.2:
+        return 1.0, middle, 2.0 ** -7, rng.choice([-1, 1]) * 2.0 ** -rng.choice([30, 60, 100, 120, 126, 133, 142, 149])
+    while True:
+        x, y = number() * rng.choice([1, 2, 4]), number()
+        c = fp32(rng.choice([-1, 1]) * middle / x)
+        off = x * c - math.copysign(middle, x * c)  # (x c is exact in FP64, and so is the difference of numbers so near to each other)
+        s = fp32(off / y)
+        if off and fp32(x * c) == math.copysign(middle, x * c) and off != y * s:
+            return x, c, y, s
+
+
+@pytest.mark.parametrize("name", ["bf16", "fp16"])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotations_that_only_the_exact_sum_tells_from_a_middle(paged, name, interleaved):
+    """against whole-number fractions; the side of the middle decides a code where a block's scale is 1, as its 6 makes it mostly"""
+    tokens, rng = 96, random.Random(31 + interleaved)
+    k, table = torch.zeros((tokens, 1, 128), dtype=torch.float64), torch.zeros((tokens, 128), dtype=torch.float64)
+    want = torch.zeros((tokens, 1, 128), dtype=torch.float64)
+    middles = 0
+    for t in range(tokens):
+        for i in range(64):
+            a, b = (2 * i, 2 * i + 1) if interleaved else (i, i + 64)
+            if i % 8 == 0:
+                x, c, y, s = 6.0, 1.0, 6.0, 0.0
+            else:
+                x, c, y, s = beside_a_middle(rng, name)
+                if rng.random() < 0.5:  # y c + x s of the pair
+                    x, y, s = y, x, -s
+            k[t, 0, a], k[t, 0, b], table[t, i], table[t, 64 + i] = x, y, c, s
+            x, c, y, s = (Fraction(z) for z in (x, c, y, s))
+            want[t, 0, a], want[t, 0, b] = nearest16(x * c - y * s, name), nearest16(y * c + x * s, name)
+            middles += i % 8 > 0
+    kind, one, at = TYPES[name][0], torch.ones(1, device="cuda"), torch.arange(tokens, dtype=torch.int32, device="cuda")
+    assert torch.equal(k.to(kind).double(), k) and torch.equal(table.float().double(), table) and torch.equal(want.to(kind).double(), want) and middles == tokens * 56
+    units = torch.zeros((tokens // 16, 1, 1, 2304), dtype=torch.uint8, device="cuda")
+    k, table = k.to(kind).cuda(), table.float().cuda()
+    paged.append_rotated(paged.PagedCache(units, one, one), k[:, :0], k, k, at, at, table, interleaved=interleaved)
+    codes, scales = pu.quantise(want.to(kind), one)
+    assert float((scales == 0x38).double().mean()) > 0.9  # (some of the pairs' other sums are above 6)
+    got = pu.at_slots(units, at)
+    assert torch.equal(got[0].cpu(), codes) and torch.equal(got[2].cpu(), scales)
+
+
+@pytest.mark.parametrize("name, x, c, y, s, right", [("bf16", 1.09375, "0x1.933334p-1", 1.0859375, "0x1.9c8bf8p-26", 0.86328125), ("bf16", 1.8359375, "0x1.c1e808p-2", 1.171875, "-0x1.1eb852p-26", 0.80859375),
+                                                     ("fp16", 1.5322265625, "0x1.552b90p-2", 1.6044921875, "-0x1.84e878p-28", 0.51025390625)])
+def test_rotations_whose_products_errors_cancel(paged, name, x, c, y, s, right):
+    """what is left behind both products' errors decides. The head's factor puts the border of the codes 0 and 0.5 between the two numbers"""
+    kind, bits = TYPES[name][0], 8 if name == "bf16" else 11
+    c, s = float.fromhex(c), float.fromhex(s)
+    exact = Fraction(x) * Fraction(c) - Fraction(y) * Fraction(s)
+    assert nearest16(exact, name) == right
+    unit = 2.0 ** (math.frexp(right)[1] - bits)
+    other = right - unit if exact < right else right + unit
+    low, high = min(right, other), max(right, other)
+    k, table = torch.zeros((1, 1, 128)), torch.ones((1, 128))
+    table[:, 64:] = 0
+    k[0, 0, 0], k[0, 0, 64], table[0, 0], table[0, 64] = x, y, c, s
+    factor = 2 * (low + high)
+    k[0, 0, 1] = 6 * factor  # (rounded to the type: the block's scale is 1 all the same)
+    one, at = torch.full((1,), factor, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    units, k = torch.zeros((1, 1, 1, 2304), dtype=torch.uint8, device="cuda"), k.to(kind).cuda()
+    cache = paged.PagedCache(units, one, one)
+    paged.append_rotated(cache, k[:, :0], k, k, at, at, table.cuda())
+    got = [z.cpu() for z in pu.at_slots(units, at)]
+    codes = []
+    for z in (low, high):
+        turned = k.cpu().clone()
+        turned[0, 0, 0], turned[0, 0, 64] = z, nearest16(Fraction(y) * Fraction(c) + Fraction(x) * Fraction(s), name)
+        codes.append(pu.quantise(turned, one))
+    assert not torch.equal(codes[0][0], codes[1][0])  # (the border tells them apart)
+    assert torch.equal(got[0], codes[right == high][0]) and torch.equal(got[2], codes[right == high][1])
