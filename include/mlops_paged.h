@@ -137,7 +137,8 @@ mlops_fbla_status mlops_paged_cross_attend(const mlops_paged_attend_args *args, 
 
 /* Requests that begin with the same tokens: group g is the requests starts[g] .. starts[g + 1] - 1 (ascending; requests of no group share nothing), whose first tokens[g] tokens
  * are the same. Of these whole pages count, and these pages' entries in the table's rows of the group's requests are the same (those of any one of them may be read for all).
- * Both arrays live on the device. */
+ * Both arrays live on the device. Where groups or the requests' starts do not ascend, rows of q that belong to two requests, or lie in the rows of two groups, hold anything; the others
+ * are as they would be. */
 typedef struct mlops_paged_common {
   int groups;                          /* batch + groups at most 2048 */
   const int *starts;                   /* [groups + 1], or null: all requests are one group (groups 1) */

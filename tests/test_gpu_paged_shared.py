@@ -419,3 +419,58 @@ def test_on_both_sides_of_requests_that_fill_rows_of_work(paged, rows):
     gen, table, cache = build(paged, 25, groups, lengths, 2, 64)
     q = torch.randn((sum(counts), 8, 128), generator=gen, device="cuda").to(torch.float16)
     check(paged, q, cache, table, lengths, counts, starts_of(counts), groups, "fp16")
+
+
+def guarded(shape, kind, value):
+    """an array between two stretches of sentinels, and the whole"""
+    n, around = math.prod(shape), 4096
+    whole = torch.full((n + 2 * around,), value, dtype=kind, device="cuda")
+    return whole[around : around + n].view(shape), whole, around
+
+
+@pytest.mark.parametrize("fill", [0xFF, 0x01])
+@pytest.mark.parametrize("starts", [[0, 5, 10, 15, 20], [8, 2, 12, 12, 20], [0, 5, 3, 9, 20], [0, 1, 2, 3, 4], [0, 1000, -5, 20, 20], [3, 9, 20, 31, 60], [6, 0, 90, 95, 200]])
+@pytest.mark.parametrize("cuts", [[0, 4], [2, 1, 4], [3, 0, 9], [0, 3, 1, 4], [-7, 1 << 30], [2, 4, 0, 2]])
+def test_rows_that_only_one_request_and_group_name(paged, starts, cuts, fill):
+    """starts and groups in any order: a row that belongs to one request, and lies in the rows of one group at most, has what attention by itself gives; nothing is written around the arrays or into
+    what a call reads"""
+    lengths, heads, tokens, batch = [300, 310, 320, 330], 2, 20, 4
+    gen, table, cache = build(paged, 26, [(0, 4, 256)], lengths, heads, 64)
+    rows = torch.randn((tokens, 8, 128), generator=gen, device="cuda").to(torch.bfloat16)
+    common = [256 - 64 * (g % 3) for g in range(len(cuts) - 1)]
+    out, out_whole, around = guarded((tokens, 8, 128), torch.bfloat16, 77.0)
+    lse, lse_whole, _ = guarded((tokens, 8), torch.float32, 77.0)
+    held, begins, groups_at, common_at = ints(lengths), ints(starts), ints(cuts), ints(common)
+    call = paged._ATTEND.pack(batch, tokens, 8, 0, rows.data_ptr(), 1024, 128, out.data_ptr(), 1024, 128, lse.data_ptr(), table.data_ptr(), table.stride(0), table.shape[1], held.data_ptr(),
+                              begins.data_ptr(), 0.0)
+    groups = paged._COMMON.pack(len(common), groups_at.data_ptr(), common_at.data_ptr())
+    scratch, scratch_whole, _ = guarded((paged._lib.mlops_paged_attend_shared_scratch_bytes(call, groups, heads),), torch.uint8, fill)
+    scratch[:8192] = 0
+    inputs = [x.clone() for x in (rows, cache.units, table, held, begins, groups_at, common_at)]
+    for _ in range(2):
+        assert paged._lib.mlops_paged_attend_shared(call, groups, paged._pool(cache)[0], scratch.data_ptr(), scratch.numel(), torch.cuda.current_stream().cuda_stream) == 0
+    for x, y in zip(inputs, (rows, cache.units, table, held, begins, groups_at, common_at)):
+        assert torch.equal(x, y)
+    for whole, value in ((out_whole, 77.0), (lse_whole, 77.0), (scratch_whole, fill)):
+        assert bool((whole[:around] == value).all()) and bool((whole[-around:] == value).all())
+    assert bool((scratch[:8192] == 0).all())
+
+    clip = lambda x, lo, hi: min(max(x, lo), hi)
+    mine = [(clip(starts[b], 0, tokens), min(starts[b + 1], tokens)) for b in range(batch)]
+    firsts = [(clip(cuts[g], 0, batch), clip(cuts[g + 1], 0, batch)) for g in range(len(common))]
+    theirs = [(clip(starts[a], 0, tokens), min(starts[b], tokens)) for a, b in firsts if b - a > 1]
+    edges = clip(starts[0], 0, tokens), min(max(starts[-1], starts[0], 0), tokens)  # rows of no request are before and behind
+    once = [edges[0] <= i < edges[1] and sum(a <= i < b for a, b in mine) == 1 and sum(a <= i < b for a, b in theirs) <= 1 for i in range(tokens)]
+    checked = 0
+    for b, (first, end) in enumerate(mine):
+        n = max(end - first, 0)
+        if n == 0:
+            continue
+        value, weight, log = pu.attend(rows[first:end], cache.units, cache.k_scale, cache.v_scale, table[b : b + 1], [max(lengths[b] - starts[b + 1] + end, 0)], [n])
+        keep = torch.tensor(once[first:end], device="cuda")
+        agree(out[first:end][keep], lse[first:end][keep], [x[keep] for x in (value, weight, log)], "bf16")
+        checked += int(keep.sum())
+    assert checked == sum(once)
+    for free in (slice(0, edges[0]), slice(edges[1], tokens)):
+        untouched = [i for i in range(tokens)[free] if not any(a <= i < b for a, b in mine)]
+        assert bool((out[untouched] == 0).all()) and bool(torch.isneginf(lse[untouched]).all())
