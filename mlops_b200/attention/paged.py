@@ -316,6 +316,8 @@ def attend_shared(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, lengt
     Group g is the requests ``groups[g] .. groups[g + 1] - 1`` (``groups`` int32 [n + 1], ascending; None: all requests are one group); their first ``shared[g]`` tokens are the same
     (``shared`` int32 [n]). Of these whole pages count, and the requests' rows of ``table`` name the same pages for them; ``lengths`` and positions count the common tokens like
     the others. A request whose first query does not see all of the common tokens is attended by itself, as are requests of no group."""
+    if shared is None:
+        raise ValueError("shared: expected an int32 [n] tensor of the groups' common tokens, not None (attend takes requests that have none)")
     return _attention("mlops_paged_attend_shared", q, cache, table, lengths, starts, scale, return_lse, groups, shared)
 
 

@@ -79,3 +79,11 @@ def test_python_refusals(paged):  # noqa: F811
                  lambda: paged.attend_shared(x, cache, one.view(1, 1), one, None, None, one)):
         with pytest.raises(ValueError, match="CUDA"):
             call()
+
+
+def test_groups_without_their_common_tokens(paged):  # noqa: F811
+    cache = paged.empty(3, 2, 32, device="cpu")
+    x, one = torch.zeros((1, 2, 128), dtype=torch.bfloat16), torch.zeros(1, dtype=torch.int32)
+    for groups in (None, torch.zeros(2, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="shared"):
+            paged.attend_shared(x, cache, one.view(1, 1), one, None, groups, None)
