@@ -132,7 +132,7 @@ size_t mlops_paged_attend_scratch_bytes(const mlops_paged_attend_args *args, int
 mlops_fbla_status mlops_paged_attend(const mlops_paged_attend_args *args, const mlops_paged_cache *cache, void *scratch, size_t scratch_bytes, cudaStream_t stream);
 
 /* Cross attention: as mlops_paged_attend, but every query of a request sees all of the request's lengths[b] tokens (the states of an encoder; queries may outnumber them, as those of
- * several beams do). Scratch: mlops_paged_attend_scratch_bytes; one that serves mlops_paged_attend serves this too. */
+ * several beams do). For requests of one query each, with starts or without, it is mlops_paged_attend. Scratch: mlops_paged_attend_scratch_bytes; one that serves mlops_paged_attend serves this too. */
 mlops_fbla_status mlops_paged_cross_attend(const mlops_paged_attend_args *args, const mlops_paged_cache *cache, void *scratch, size_t scratch_bytes, cudaStream_t stream);
 
 /* Requests that begin with the same tokens: group g is the requests starts[g] .. starts[g + 1] - 1 (ascending; requests of no group share nothing), whose first tokens[g] tokens
@@ -145,7 +145,10 @@ typedef struct mlops_paged_common {
   const int *tokens;                   /* [groups] */
 } mlops_paged_common;
 /* What mlops_paged_attend gives, within rounding; the pages that a group's requests have in common are read once for all of them. A request whose first query does not see all of the
- * common tokens is attended by itself. (A group's first request that takes part is looked for in their order: idle places of a batch are better at a group's end.) The scratch is mlops_paged_attend's with 1056 bytes more per row of q and query head. */
+ * common tokens is attended by itself; its rows are multiplied with the common tokens all the same where it stands in a group, so that one of many queries is better left out of it. So are, all of them, the requests of
+ * a group whose queries times query heads per KV head are more than 320 on average, a long chunk among few decodes for instance: nothing is shared in such a group. (A group's first request that takes
+ * part is looked for in their order: idle places of a batch are better at a group's end.) Scratch, what the function returns: 1056 bytes per row of q and query head, beside them what mlops_paged_attend asks
+ * for, without starts too that of a call with starts where `tokens` times the query heads per KV head are more than 32. */
 size_t mlops_paged_attend_shared_scratch_bytes(const mlops_paged_attend_args *args, const mlops_paged_common *common, int kv_heads);
 mlops_fbla_status mlops_paged_attend_shared(const mlops_paged_attend_args *args, const mlops_paged_common *common, const mlops_paged_cache *cache, void *scratch, size_t scratch_bytes,
                                             cudaStream_t stream);

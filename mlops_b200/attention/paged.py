@@ -305,7 +305,8 @@ def attend(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, lengths: tor
 def cross_attend(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor] = None, *, scale: float = 0.0,
                  return_lse: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """Cross attention: as `attend`, but every query of request b sees all ``lengths[b]`` tokens that the request has in the pool, for instance the states of its encoder, which
-    `append` has stored. The queries' own tokens are elsewhere; there may be more of them than states (several beams of a request are rows of one request)."""
+    `append` has stored. The queries' own tokens are elsewhere; there may be more of them than states (several beams of a request are rows of one request). For requests of one query each
+    it is `attend`."""
     return _attention("mlops_paged_cross_attend", q, cache, table, lengths, starts, scale, return_lse)
 
 
@@ -315,7 +316,8 @@ def attend_shared(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, lengt
 
     Group g is the requests ``groups[g] .. groups[g + 1] - 1`` (``groups`` int32 [n + 1], ascending; None: all requests are one group); their first ``shared[g]`` tokens are the same
     (``shared`` int32 [n]). Of these whole pages count, and the requests' rows of ``table`` name the same pages for them; ``lengths`` and positions count the common tokens like
-    the others. A request whose first query does not see all of the common tokens is attended by itself, as are requests of no group."""
+    the others. A request whose first query does not see all of the common tokens is attended by itself, as are requests of no group, and all requests of a group that has more than 320
+    rows per KV head (queries times query heads per KV head) and request on average. ``batch`` and groups are 2048 together at most, and there is one group at least."""
     if shared is None:
         raise ValueError("shared: expected an int32 [n] tensor of the groups' common tokens, not None (attend takes requests that have none)")
     return _attention("mlops_paged_attend_shared", q, cache, table, lengths, starts, scale, return_lse, groups, shared)

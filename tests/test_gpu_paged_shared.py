@@ -474,3 +474,14 @@ def test_rows_that_only_one_request_and_group_name(paged, starts, cuts, fill):
     for free in (slice(0, edges[0]), slice(edges[1], tokens)):
         untouched = [i for i in range(tokens)[free] if not any(a <= i < b for a, b in mine)]
         assert bool((out[untouched] == 0).all()) and bool(torch.isneginf(lse[untouched]).all())
+
+
+@pytest.mark.parametrize("tokens, heads, kv_heads, with_starts", [(1, 8, 8, False), (8, 32, 8, False), (9, 32, 8, False), (64, 32, 8, False), (8, 32, 8, True), (9, 32, 8, True), (3, 40, 1, False), (1, 40, 1, True)])
+def test_the_scratch_that_a_call_asks_for(paged, tokens, heads, kv_heads, with_starts):
+    """1056 bytes per row of q and query head beside attend's: that of a call with starts where there are more than 32 rows per KV head, that of one without where there are no more"""
+    def attend(starts, heads=heads):
+        return paged._lib.mlops_paged_attend_scratch_bytes(paged._ATTEND.pack(tokens, tokens, heads, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 4096 if starts else 0, 0.0), kv_heads)
+    call = paged._ATTEND.pack(tokens, tokens, heads, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 4096 if with_starts else 0, 0.0)
+    many = tokens * heads // kv_heads > 32
+    beside = attend(True) if many else attend(False, kv_heads)
+    assert paged._lib.mlops_paged_attend_shared_scratch_bytes(call, paged._COMMON.pack(1, 0, 4096), kv_heads) == beside + 1056 * tokens * heads
