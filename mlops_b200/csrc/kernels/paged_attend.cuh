@@ -75,7 +75,8 @@ __device__ __forceinline__ Plain plain_request(const Call &k, int b) {
 }
 // group g's requests, and their common tokens: whole pages of the table, none for a single request, nor for requests of more than LONE columns on average, which fill rows of work by
 // themselves: they take their tokens in one row instead of two that are joined (16 requests behind 6 000 common tokens, us by themselves and together: 132 columns each 136 and 107, 260 216 and
-// 185, 384 235 and 247, 512 282 and 322, 1024 526 and 609). Whether a request's first query sees them all, so that it takes part, is asked for each.
+// 185, 384 235 and 247, 512 282 and 322, 1024 526 and 609). The average of mixed groups: a chunk of 2 048 queries of four heads
+// and 15 decodes behind 16 384 tokens (516 columns) take 702 with each by itself and 735 so, the chunk and 31 decodes (260) 780 and 707. Whether a request's first query sees them all, so that it takes part, is asked for each.
 constexpr int LONE = 320;
 struct Group {
   int first, end, tokens;

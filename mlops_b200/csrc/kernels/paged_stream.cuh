@@ -29,7 +29,7 @@
 namespace paged {
 namespace {
 
-// One tile of columns: sixteen warps of 128 registers (12 bytes of them spilled). Two: eight of 243; with twelve of 168 the registers do not hold a block's words (1.04 times
+// One tile of columns: sixteen warps of 128 registers (12 bytes of them spilled, 40 in cross attention). Two: eight of 240 or 241; with twelve of 168 the registers do not hold a block's words (1.04 times
 // the time of drafted tokens of 16 requests). Three do not pay: requests of 24 columns take 0.85 of the time, but those of 16 columns 1.14 and of 32 1.15.
 template <int NT> constexpr int WARPS = NT == 1 ? 16 : 8;
 template <int NT> constexpr int STAGES = NT == 1 ? 2 : 3;

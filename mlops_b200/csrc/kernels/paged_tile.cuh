@@ -425,7 +425,7 @@ template <int TYPE, int MODE> __device__ __forceinline__ void load_q(const Call 
   }
 }
 
-// 64 columns of the thread's lane from `at` on, to be waited for by arrived64, which every use of the values follows
+// 32 columns of the thread's lane from `at` on, to be waited for (tcgen05.wait::ld); PAGED_HOLD32 behind the wait keeps every use of them behind it
 #define PAGED_LD32(at, r) \
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];" \
                : "=r"((r)[0]), "=r"((r)[1]), "=r"((r)[2]), "=r"((r)[3]), "=r"((r)[4]), "=r"((r)[5]), "=r"((r)[6]), "=r"((r)[7]), "=r"((r)[8]), "=r"((r)[9]), "=r"((r)[10]), "=r"((r)[11]), \
