@@ -60,6 +60,8 @@ template <int MODE> cudaError_t call(const mlops_paged_attend_args *a, const mlo
   k.group = a->q_heads / c->kv_heads;
   k.by_group = Divisor(k.group);
   k.wide = WIDE;
+  const int64_t room = (int64_t)a->width * c->page_size;
+  k.room = (int)(room < INT32_MAX - 255 ? room : INT32_MAX - 255);
   k.narrow = (int64_t)a->tokens * k.group <= (int64_t)8 * a->batch ? 8 : 16;
   k.stream_counters = reinterpret_cast<int *>(base + s.stream_counters);
   k.tile_counters = reinterpret_cast<int *>(base + s.tile_counters);

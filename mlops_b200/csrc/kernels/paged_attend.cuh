@@ -22,6 +22,7 @@ struct Call {
   Divisor by_group;
   int wide;        // requests with more than so many columns (queries times group) are the tile kernel's
   int narrow;      // columns of the stream's rows of work
+  int room;        // tokens that a row of the table can name; at most 2^31 - 256, so that they can be rounded up to units and tiles
   float *stream_part, *tile_part;          // partial rows, see the kernels
   int *stream_counters, *tile_counters;    // one per CTA, zeros before and after every call
   // SHARED: the groups, and the sums of every row of q and head over common and own tokens (row_end, pieces_end); rows of both kernels' parts
@@ -70,13 +71,13 @@ __device__ __forceinline__ Plain plain_request(const Call &k, int b) {
   }
   const int length = max(__ldg(k.a.lengths + b), 0);
   r.at = length - e + r.start;
-  r.tokens = (int)min((long long)length, (long long)k.a.width * k.c.page_size);
+  r.tokens = min(length, k.room);
   return r;
 }
 // group g's requests, and their common tokens: whole pages of the table, none for a single request, nor for requests of more than LONE columns on average, which fill rows of work by
 // themselves: they take their tokens in one row instead of two that are joined (16 requests behind 6 000 common tokens, us by themselves and together: 132 columns each 136 and 107, 260 216 and
 // 185, 384 235 and 247, 512 282 and 322, 1024 526 and 609). The average of mixed groups: a chunk of 2 048 queries of four heads
-// and 15 decodes behind 16 384 tokens (516 columns) take 702 with each by itself and 735 so, the chunk and 31 decodes (260) 780 and 707. Whether a request's first query sees them all, so that it takes part, is asked for each.
+// and 15 decodes behind 16 384 tokens (516 columns) take 702 in mlops_paged_attend and 735 here, the chunk and 31 decodes (260) 780 and 707. Whether a request's first query sees them all, so that it takes part, is asked for each.
 constexpr int LONE = 320;
 struct Group {
   int first, end, tokens;

@@ -240,3 +240,18 @@ def test_one_score_far_above_a_long_context(paged, counts, at):
     want, weight, want_lse = pu.attend(q, cache.units, cache.k_scale, cache.v_scale, table, [length], counts, scale)
     assert bool(((out.double() - want).abs() <= 2.0 ** -10 * weight + length * 2.0 ** -34 * 2.5 + TYPES["bf16"][1] * want.abs()).all())
     assert float(want[..., :64].min()) > 2.0 ** -16 and bool(((lse.double() - want_lse).abs() <= 2.0 ** -12 * (1 + want_lse.abs() / 8)).all())
+
+
+@pytest.mark.parametrize("name", ["attend", "cross_attend", "attend_shared"])
+def test_a_length_at_the_end_of_its_type(paged, name):
+    """2^31 - 1 tokens, which a row of the table could name (`assign` ends there): those whose pages there are are seen"""
+    from tests.test_gpu_paged import factors
+    P, width, heads = 2048, 1 << 20, 1
+    gen = generator(41)
+    cache = paged.PagedCache(pu.random_units(gen, 3, heads, P), *factors(gen, heads))
+    table = torch.full((2, width), -1, dtype=torch.int32, device="cuda")
+    table[0, :2], table[1, 0] = ints([2, 0]), 1
+    q = torch.randn((2, 4, 128), generator=gen, device="cuda").to(torch.bfloat16)
+    more = (None, None, ints([0])) if name == "attend_shared" else (None,)
+    out, lse = getattr(paged, name)(q, cache, table, ints([(1 << 31) - 1, 700]), *more, return_lse=True)
+    agree(out, lse, pu.attend(q, cache.units, cache.k_scale, cache.v_scale, table[:, :2], [2 * P, 700], [1, 1]), "bf16")
